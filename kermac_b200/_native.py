@@ -41,6 +41,19 @@ EXPORTED_SYMBOLS = (
     "kermac_b200_build_id",
 )
 
+# declared in include/kermac_b200_attention.h
+TYPE_FLOAT32, TYPE_BFLOAT16, TYPE_FLOAT16 = 0, 1, 2
+ATTENTION_CROSS, ATTENTION_PREFIX, ATTENTION_GRAD = 0, 1, 2
+ATTENTION_SYMBOLS = (
+    "kermac_b200_cross_attention",
+    "kermac_b200_prefix_attention",
+    "kermac_b200_cross_attention_grad",
+    "kermac_b200_cross_attention_scratch_bytes",
+    "kermac_b200_prefix_attention_scratch_bytes",
+    "kermac_b200_cross_attention_grad_scratch_bytes",
+    "kermac_b200_describe_attention",
+)
+
 
 class KmHyper(C.Structure):
     _fields_ = [("ptr", C.c_void_p), ("value", C.c_float), ("batch_stride", C.c_int64)]
@@ -100,6 +113,28 @@ class KmMatvecArgs(C.Structure):
     ]
 
 
+class KmHeads(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("stride_l", C.c_int64), ("stride_row", C.c_int64), ("stride_head", C.c_int64)]
+
+
+class KmAttentionArgs(C.Structure):
+    _fields_ = [
+        ("l", C.c_int32), ("n", C.c_int32), ("m", C.c_int32),
+        ("heads", C.c_int32), ("key_heads", C.c_int32), ("d", C.c_int32),
+        ("type", C.c_int32),
+        ("prefix", C.c_int32),
+        ("q", KmHeads), ("k", KmHeads), ("v", KmHeads), ("out", KmHeads),
+        ("k_prefix", KmHeads), ("v_prefix", KmHeads),
+        ("lengths", C.c_void_p), ("lengths_stride", C.c_int64),
+        ("lse", C.c_void_p), ("lse_stride_l", C.c_int64), ("lse_stride_head", C.c_int64),
+        ("scale", C.c_float),
+        ("kv_batch", C.c_int32),
+        ("q_batch", C.c_int32),
+        ("grad_out", KmHeads), ("grad_q", KmHeads), ("grad_k", KmHeads), ("grad_v", KmHeads),
+        ("scratch", C.c_void_p), ("scratch_bytes", C.c_int64),
+    ]
+
+
 class NativeLibraryError(RuntimeError):
     """libkermac_b200.so is missing, unloadable or of the wrong ABI version."""
 
@@ -153,6 +188,12 @@ def _declare(lib: C.CDLL) -> None:
     lib.kermac_b200_abi_version.restype = C.c_int
     lib.kermac_b200_build_id.argtypes = []
     lib.kermac_b200_build_id.restype = C.c_char_p
+    for name in ATTENTION_SYMBOLS[:3]:
+        getattr(lib, name).argtypes, getattr(lib, name).restype = [C.POINTER(KmAttentionArgs), C.c_void_p], C.c_int
+    for name in ATTENTION_SYMBOLS[3:6]:
+        getattr(lib, name).argtypes, getattr(lib, name).restype = [C.POINTER(KmAttentionArgs)], C.c_int64
+    lib.kermac_b200_describe_attention.argtypes = [C.POINTER(KmAttentionArgs), C.c_int32, C.c_char_p, C.c_int32]
+    lib.kermac_b200_describe_attention.restype = C.c_int
 
 
 def lib() -> C.CDLL:
@@ -172,7 +213,7 @@ def lib() -> C.CDLL:
             handle = C.CDLL(path)
         except OSError as exc:
             raise NativeLibraryError(f"cannot load {path}: {exc}") from exc
-        missing = [s for s in EXPORTED_SYMBOLS if not hasattr(handle, s)]
+        missing = [s for s in EXPORTED_SYMBOLS + ATTENTION_SYMBOLS if not hasattr(handle, s)]
         if missing:
             raise NativeLibraryError(f"{path} lacks symbols {missing}")
         _declare(handle)
@@ -307,6 +348,20 @@ def launch_grad_static(args: KmGradArgs, stream_ptr: int) -> None:
 
 def launch_matvec(args: KmMatvecArgs, stream_ptr: int) -> None:
     check(lib().kermac_b200_kernel_matvec(C.byref(args), C.c_void_p(stream_ptr)), "kermac_b200_kernel_matvec")
+
+
+def attention_scratch_bytes(args: KmAttentionArgs, kind: int) -> int:
+    return int(getattr(lib(), ATTENTION_SYMBOLS[3 + kind])(C.byref(args)))
+
+
+def launch_attention(args: KmAttentionArgs, kind: int, stream_ptr: int) -> None:
+    check(getattr(lib(), ATTENTION_SYMBOLS[kind])(C.byref(args), C.c_void_p(stream_ptr)), ATTENTION_SYMBOLS[kind])
+
+
+def describe_attention(args: KmAttentionArgs, kind: int) -> str:
+    buf = C.create_string_buffer(256)
+    check(lib().kermac_b200_describe_attention(C.byref(args), kind, buf, 256), "kermac_b200_describe_attention")
+    return buf.value.decode()
 
 
 def describe_build(args: KmBuildArgs) -> str:

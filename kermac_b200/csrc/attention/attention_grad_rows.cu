@@ -1,0 +1,377 @@
+// Gradient of the attention for any layout, type and width up to 256 channels, with mma.sync.
+//
+// With p = exp(s - lse) recomputed from the forward pass's lse and delta = sum_d dout * out,
+//   dv = p^T dout,   ds = p * (dout v^T - delta),   dk = scale ds^T q,   dq = scale ds k.
+// Two kernels, so that every sum has one owner and a fixed order: one holds 64 keys and streams the queries (dk, dv), one holds 64
+// queries and streams the keys (dq).  The price is that s and dout v^T are computed twice, 7 products instead of 5.
+#include "attention_mma.cuh"
+
+namespace km {
+namespace att {
+namespace {
+
+// float16 weights are multiplied by this before they are rounded: they are at most 1, and float16 ends at 6e-8.
+constexpr float F16_WEIGHT = 256.0f;
+
+template <typename T> constexpr bool is_f16 = std::is_same<T, __half>::value;
+
+template <typename T, int DP>
+struct GradShape {
+    static constexpr int ROWS   = ATT_GRAD_ROWS;
+    static constexpr int STREAM = sizeof(T) == 2 && DP <= 128 ? 32 : 16;
+    static constexpr int CT     = (DP > 128 ? 128 : DP) / 8;             // channel groups of a block's dk and dv
+    static constexpr int HELD   = Tile<T, DP>::bytes(ROWS);
+    static constexpr int MOVED  = Tile<T, DP>::bytes(STREAM);
+    static constexpr int STATS  = 2 * 2 * STREAM * 4;                    // two stages of lse and delta
+    static constexpr int SMEM   = 2 * HELD + 2 * 2 * MOVED + STATS;
+};
+
+// 2^-e with 2^e the power of two at or below the largest of the given peaks; 1 when they are zero, infinite or NaN.
+// Called by the whole block.
+template <typename T>
+__device__ __forceinline__ float find_factor(const AttentionGradParams& p, int l0, int l1, int h0, int h1) {
+    if constexpr (!is_f16<T>) {
+        return 1.0f;
+    } else {
+        __shared__ float of_warp[WARPS];
+        float best = 0.0f;
+        const int per_l = (h1 - h0) * p.peak_count;
+        for (int l = l0; l < l1; ++l)
+            for (int i = threadIdx.x; i < per_l; i += THREADS)
+                best = fmaxf(best, p.peaks[(static_cast<long long>(l) * p.H + h0) * p.peak_count + i]);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
+        if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = best;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WARPS; ++i) best = fmaxf(best, of_warp[i]);
+        const uint32_t e = __float_as_uint(best) >> 23;                  // best is a float16 magnitude: 2^-24 .. 65504
+        return (best > 0.0f && e < 255) ? __uint_as_float((254u - e) << 23) : 1.0f;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ const T* head_of(const Heads& t, int l, int h) {
+    return reinterpret_cast<const T*>(t.ptr) + l * t.sl + h * t.sh;
+}
+
+// Channels (c, c + 1) of a gradient: into the tensor, or into a slice's 32-bit sums [l][row][head][D].
+template <typename T>
+__device__ __forceinline__ void put_grad(const Heads& to, float* part, int l, int row, int h, int rows, int heads, int D, int c,
+                                         float x, float y) {
+    if (c >= D) return;
+    if (part) {
+        float* o = part + ((static_cast<long long>(l) * rows + row) * heads + h) * D + c;
+        o[0] = x;
+        if (c + 1 < D) o[1] = y;
+    } else {
+        T* o = reinterpret_cast<T*>(to.ptr) + l * to.sl + row * to.sr + h * to.sh + c;
+        o[0] = Type<T>::to(x);
+        if (c + 1 < D) o[1] = Type<T>::to(y);
+    }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS) attention_grad_keys_kernel(const AttentionGradParams p) {
+    typedef GradShape<T, DP> S;
+    typedef Tile<T, DP>      TL;
+    constexpr int NT = S::STREAM / 8, CT = S::CT;
+    extern __shared__ __align__(16) char smem[];
+    T* const     held_k = reinterpret_cast<T*>(smem);
+    T* const     held_v = reinterpret_cast<T*>(smem + S::HELD);
+    char* const  ring   = smem + 2 * S::HELD;
+    float* const stats  = reinterpret_cast<float*>(ring + 4 * S::MOVED);
+    const int    warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    after_previous_grid();
+
+    // (key tile, slice, key head, batch entry of k and v); channel part in y
+    const int tiles = (p.M + S::ROWS - 1) / S::ROWS;
+    int       block = blockIdx.x;
+    const int tile = block % tiles;   block /= tiles;
+    const int slice = block % p.kv_slices; block /= p.kv_slices;
+    const int hk = block % p.Hk, kl = block / p.Hk;
+    const int c0 = blockIdx.y * CT * 8, key0 = tile * S::ROWS;
+
+    // the sum runs over (batch entries of a broadcast k, heads of the group, query tiles): this block's piece of it
+    const int l_count = p.kv_batch == 1 ? p.L : 1, l_first = p.kv_batch == 1 ? 0 : kl;
+    const int q_tiles = (p.N + S::STREAM - 1) / S::STREAM;
+    const int all     = l_count * p.G * q_tiles;
+    const int from    = static_cast<int>(static_cast<long long>(all) * slice / p.kv_slices);
+    const int to      = static_cast<int>(static_cast<long long>(all) * (slice + 1) / p.kv_slices);
+    int longest = 0;                               // keys from here on are in no sum of this block: their gradient is zero
+    if (from < to)
+        for (int l = l_first + from / (p.G * q_tiles); l <= l_first + (to - 1) / (p.G * q_tiles); ++l) {
+            const int n = key_count(p.lengths, p.lengths_stride, l, p.M);
+            longest = n > longest ? n : longest;
+        }
+    const bool  idle   = key0 >= longest;
+    const float factor = find_factor<T>(p, l_first, l_first + l_count, hk * p.G, hk * p.G + p.G);
+    const float by     = is_f16<T> ? factor / F16_WEIGHT : 1.0f;
+
+    float dk[CT][4], dv[CT][4];
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+        dk[c][0] = dk[c][1] = dk[c][2] = dk[c][3] = dv[c][0] = dv[c][1] = dv[c][2] = dv[c][3] = 0.0f;
+
+    if (!idle) {
+        copy_rows<T, DP>(held_k, head_of<T>(p.k, kl, hk), p.k.sr, key0, longest, S::ROWS, p.D, p.vec, threadIdx.x, THREADS);
+        copy_rows<T, DP>(held_v, head_of<T>(p.v, kl, hk), p.v.sr, key0, longest, S::ROWS, p.D, p.vec, threadIdx.x, THREADS);
+        auto load = [&](int i) {
+            if (i < to) {
+                const int qt = i % q_tiles, lg = i / q_tiles, h = hk * p.G + lg % p.G, l = l_first + lg / p.G, n0 = qt * S::STREAM;
+                T* const  dst = reinterpret_cast<T*>(ring + (i & 1) * 2 * S::MOVED);
+                copy_rows<T, DP>(dst, head_of<T>(p.q, l, h), p.q.sr, n0, p.N, S::STREAM, p.D, p.vec, threadIdx.x, THREADS);
+                copy_rows<T, DP>(dst + S::STREAM * TL::LD, head_of<T>(p.dout, l, h), p.dout.sr, n0, p.N, S::STREAM, p.D, p.vec,
+                                 threadIdx.x, THREADS);
+                if (threadIdx.x < 2 * S::STREAM) {
+                    const int    r = threadIdx.x % S::STREAM, which = threadIdx.x / S::STREAM;
+                    const bool   valid = n0 + r < p.N;
+                    const float* src = which == 0 ? p.lse + l * p.lse_sl + h * p.lse_sh : p.delta + (static_cast<long long>(l) * p.H + h) * p.N;
+                    copy_async_4(smem_addr(stats + ((i & 1) * 2 + which) * S::STREAM + r), valid ? src + n0 + r : src, valid);
+                }
+            }
+            copy_commit();
+        };
+        load(from);
+        for (int i = from; i < to; ++i) {
+            load(i + 1);
+            copy_wait<1>();
+            __syncthreads();
+            const T* const     q     = reinterpret_cast<const T*>(ring + (i & 1) * 2 * S::MOVED);
+            const T* const     dout  = q + S::STREAM * TL::LD;
+            const float* const lse   = stats + (i & 1) * 2 * S::STREAM;
+            const float* const delta = lse + S::STREAM;
+            const int          l     = l_first + i / (q_tiles * p.G), n0 = (i % q_tiles) * S::STREAM;
+            const int          count = key_count(p.lengths, p.lengths_stride, l, p.M);
+            float s[NT][4], ds[NT][4];
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                s[j][0] = s[j][1] = s[j][2] = s[j][3] = ds[j][0] = ds[j][1] = ds[j][2] = ds[j][3] = 0.0f;
+            product_nt<T, DP, NT>(s, held_k + warp * 16 * TL::LD, q);
+            product_nt<T, DP, NT>(ds, held_v + warp * 16 * TL::LD, dout);
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int   col  = j * 8 + 2 * t + (e & 1);
+                    const bool  seen = key0 + warp * 16 + g + 8 * (e >> 1) < count && n0 + col < p.N;
+                    const float w    = ex2_approx(fmaf(s[j][e], p.scale_log2, (is_f16<T> ? 8.0f : 0.0f) - lse[col] * (1.0f / LN2)));
+                    ds[j][e] = seen ? w * ((ds[j][e] - delta[col]) * by) : 0.0f;
+                    s[j][e]  = seen ? w : 0.0f;
+                }
+            product_nn<T, DP, NT, CT>(dv, s, dout + c0);
+            product_nn<T, DP, NT, CT>(dk, ds, q + c0);
+            __syncthreads();
+        }
+        copy_wait<0>();
+    }
+    float* const dk_part = p.kv_slices > 1 ? p.dk_part + static_cast<long long>(slice) * p.kv_batch * p.M * p.Hk * p.D : nullptr;
+    float* const dv_part = p.kv_slices > 1 ? p.dv_part + static_cast<long long>(slice) * p.kv_batch * p.M * p.Hk * p.D : nullptr;
+    const float  k_by = p.scale / factor, v_by = is_f16<T> ? 1.0f / F16_WEIGHT : 1.0f;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int key = key0 + warp * 16 + g + 8 * r;
+        if (key >= p.M) continue;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            const int at = c0 + c * 8 + 2 * t;
+            put_grad<T>(p.dk, dk_part, kl, key, hk, p.M, p.Hk, p.D, at, dk[c][2 * r] * k_by, dk[c][2 * r + 1] * k_by);
+            put_grad<T>(p.dv, dv_part, kl, key, hk, p.M, p.Hk, p.D, at, dv[c][2 * r] * v_by, dv[c][2 * r + 1] * v_by);
+        }
+    }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS) attention_grad_queries_kernel(const AttentionGradParams p) {
+    typedef GradShape<T, DP> S;
+    typedef Tile<T, DP>      TL;
+    constexpr int NT = S::STREAM / 8, CT = DP / 8;
+    extern __shared__ __align__(16) char smem[];
+    T* const    held_q = reinterpret_cast<T*>(smem);
+    T* const    held_d = reinterpret_cast<T*>(smem + S::HELD);
+    char* const ring   = smem + 2 * S::HELD;
+    const int   warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    after_previous_grid();
+
+    const int tiles = (p.N + S::ROWS - 1) / S::ROWS;
+    int       block = blockIdx.x;
+    const int n0 = block % tiles * S::ROWS; block /= tiles;
+    const int h = block % p.H, l = block / p.H, hk = h / p.G;
+    const int   count  = key_count(p.lengths, p.lengths_stride, l, p.M);
+    const int   kl     = p.kv_batch == 1 ? 0 : l;
+    const float factor = find_factor<T>(p, l, l + 1, h, h + 1);
+
+    copy_rows<T, DP>(held_q, head_of<T>(p.q, l, h), p.q.sr, n0, p.N, S::ROWS, p.D, p.vec, threadIdx.x, THREADS);
+    copy_rows<T, DP>(held_d, head_of<T>(p.dout, l, h), p.dout.sr, n0, p.N, S::ROWS, p.D, p.vec, threadIdx.x, THREADS);
+    auto load = [&](int i) {
+        const int first = i * S::STREAM;
+        if (first < count) {
+            T* const dst = reinterpret_cast<T*>(ring + (i & 1) * 2 * S::MOVED);
+            copy_rows<T, DP>(dst, head_of<T>(p.k, kl, hk), p.k.sr, first, count, S::STREAM, p.D, p.vec, threadIdx.x, THREADS);
+            copy_rows<T, DP>(dst + S::STREAM * TL::LD, head_of<T>(p.v, kl, hk), p.v.sr, first, count, S::STREAM, p.D, p.vec, threadIdx.x,
+                             THREADS);
+        }
+        copy_commit();
+    };
+    float lse[2], delta[2], dq[CT][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int n = n0 + warp * 16 + g + 8 * r;
+        lse[r]   = n < p.N ? p.lse[l * p.lse_sl + h * p.lse_sh + n] * (1.0f / LN2) : 0.0f;
+        delta[r] = n < p.N ? p.delta[(static_cast<long long>(l) * p.H + h) * p.N + n] : 0.0f;
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) dq[c][0] = dq[c][1] = dq[c][2] = dq[c][3] = 0.0f;
+
+    load(0);
+    for (int i = 0; i * S::STREAM < count; ++i) {
+        load(i + 1);
+        copy_wait<1>();
+        __syncthreads();
+        const T* const k = reinterpret_cast<const T*>(ring + (i & 1) * 2 * S::MOVED);
+        float s[NT][4], ds[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+            s[j][0] = s[j][1] = s[j][2] = s[j][3] = ds[j][0] = ds[j][1] = ds[j][2] = ds[j][3] = 0.0f;
+        product_nt<T, DP, NT>(s, held_q + warp * 16 * TL::LD, k);
+        product_nt<T, DP, NT>(ds, held_d + warp * 16 * TL::LD, k + S::STREAM * TL::LD);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float w = ex2_approx(fmaf(s[j][e], p.scale_log2, -lse[e >> 1]));
+                ds[j][e] = i * S::STREAM + j * 8 + 2 * t + (e & 1) < count ? w * ((ds[j][e] - delta[e >> 1]) * factor) : 0.0f;
+            }
+        product_nn<T, DP, NT, CT>(dq, ds, k);
+        __syncthreads();
+    }
+    copy_wait<0>();
+    // slice l of a broadcast q's partial sums
+    float* const part = p.q_slices > 1 ? p.dq_part + static_cast<long long>(l) * p.N * p.H * p.D : nullptr;
+    const float  by = p.scale / factor;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int n = n0 + warp * 16 + g + 8 * r;
+        if (n >= p.N) continue;
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+            put_grad<T>(p.dq, part, part ? 0 : l, n, h, p.N, p.H, p.D, c * 8 + 2 * t, dq[c][2 * r] * by, dq[c][2 * r + 1] * by);
+    }
+}
+
+// delta[l][h][n], and for float16 the largest |dout| of ATT_PEAK_ROWS queries.  One block for ATT_PEAK_ROWS queries of a head.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) attention_delta_kernel(const AttentionGradParams p) {
+    __shared__ float of_warp[WARPS];
+    after_previous_grid();
+    int       block = blockIdx.x;
+    const int groups = (p.N + ATT_PEAK_ROWS - 1) / ATT_PEAK_ROWS, group = block % groups;
+    block /= groups;
+    const int h = block % p.H, l = block / p.H, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const T * out = head_of<T>(p.out, l, h), *dout = head_of<T>(p.dout, l, h);
+    float     peak = 0.0f;
+    for (int r = warp; r < ATT_PEAK_ROWS; r += WARPS) {
+        const int n = group * ATT_PEAK_ROWS + r;
+        if (n >= p.N) break;
+        float sum = 0.0f;
+        for (int c = lane; c < p.D; c += 32) {
+            const float x = Type<T>::from(dout[n * p.dout.sr + c]);
+            sum  = fmaf(x, Type<T>::from(out[n * p.out.sr + c]), sum);
+            peak = fmaxf(peak, fabsf(x));
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) p.delta[(static_cast<long long>(l) * p.H + h) * p.N + n] = sum;
+    }
+    if (p.peaks) {
+#pragma unroll
+        for (int d = 16; d; d >>= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, d));
+        if (lane == 0) of_warp[warp] = peak;
+        __syncthreads();
+        if (threadIdx.x == 0)
+            p.peaks[(static_cast<long long>(l) * p.H + h) * p.peak_count + group] =
+                fmaxf(fmaxf(of_warp[0], of_warp[1]), fmaxf(of_warp[2], of_warp[3]));
+    }
+}
+
+// dst[l][row][head][c] = sum over the slices, in their order.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) attention_reduce_kernel(const float* src, int slices, const Heads dst, int L, int rows,
+                                                                  int heads, int D) {
+    after_previous_grid();
+    const long long total = static_cast<long long>(L) * rows * heads * D;
+    for (long long i = static_cast<long long>(blockIdx.x) * THREADS + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * THREADS) {
+        float sum = 0.0f;
+        for (int s = 0; s < slices; ++s) sum += src[s * total + i];
+        const int       c = static_cast<int>(i % D);
+        const long long at = i / D;
+        const int       h = static_cast<int>(at % heads), row = static_cast<int>(at / heads % rows), l = static_cast<int>(at / heads / rows);
+        reinterpret_cast<T*>(dst.ptr)[l * dst.sl + row * dst.sr + h * dst.sh + c] = Type<T>::to(sum);
+    }
+}
+
+int check_blocks(long long blocks) {
+    return blocks > 0x7fffffffLL ? fail(KM_ERR_TOO_LARGE, "attention: more than 2^31 - 1 blocks") : 0;
+}
+
+template <typename T, int DP>
+int launch_grad(const AttentionGradParams& p, cudaStream_t st) {
+    typedef GradShape<T, DP> S;
+    static_assert(S::SMEM <= 227 * 1024, "more shared memory than a block has");
+    auto* const keys    = &attention_grad_keys_kernel<T, DP>;
+    auto* const queries = &attention_grad_queries_kernel<T, DP>;
+    int rc = cuda_status(cudaFuncSetAttribute(keys, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "cudaFuncSetAttribute");
+    if (!rc) rc = cuda_status(cudaFuncSetAttribute(queries, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "cudaFuncSetAttribute");
+    const long long kb = ceil_div_ll(p.M, S::ROWS) * p.kv_slices * p.Hk * p.kv_batch;
+    const long long qb = ceil_div_ll(p.N, S::ROWS) * p.H * p.L;
+    if (!rc) rc = check_blocks(kb > qb ? kb : qb);
+    if (!rc && kb)
+        rc = cuda_status(launch_overlapped(keys, dim3(static_cast<unsigned>(kb), DP / (S::CT * 8)), THREADS, S::SMEM, st, p),
+                         "attention_grad_keys_kernel");
+    if (!rc && qb)
+        rc = cuda_status(launch_overlapped(queries, dim3(static_cast<unsigned>(qb)), THREADS, S::SMEM, st, p), "attention_grad_queries_kernel");
+    return rc;
+}
+template <typename T>
+int launch_type(const AttentionGradParams& p, cudaStream_t st) {
+    switch (padded_channels(p.D)) {
+        case 64: return launch_grad<T, 64>(p, st);
+        case 128: return launch_grad<T, 128>(p, st);
+        default: return launch_grad<T, 256>(p, st);
+    }
+}
+
+}  // namespace
+}  // namespace att
+
+int attention_grad_rows_launch(const AttentionGradParams& p, int type, cudaStream_t st) {
+    using namespace att;
+    if (type == ATT_F32) return launch_type<float>(p, st);
+    return type == ATT_BF16 ? launch_type<__nv_bfloat16>(p, st) : launch_type<__half>(p, st);
+}
+
+int attention_delta_launch(const AttentionGradParams& p, int type, cudaStream_t st) {
+    using namespace att;
+    const long long blocks = ceil_div_ll(p.N, ATT_PEAK_ROWS) * p.H * p.L;
+    if (int rc = check_blocks(blocks)) return rc;
+    const dim3 grid(static_cast<unsigned>(blocks));
+    const cudaError_t e = type == ATT_F32    ? launch_overlapped(&attention_delta_kernel<float>, grid, THREADS, 0, st, p)
+                          : type == ATT_BF16 ? launch_overlapped(&attention_delta_kernel<__nv_bfloat16>, grid, THREADS, 0, st, p)
+                                             : launch_overlapped(&attention_delta_kernel<__half>, grid, THREADS, 0, st, p);
+    return cuda_status(e, "attention_delta_kernel");
+}
+
+int attention_reduce_launch(const float* src, int slices, const Heads& dst, int L, int rows, int heads, int D, int type,
+                            cudaStream_t st) {
+    using namespace att;
+    long long blocks = ceil_div_ll(static_cast<long long>(L) * rows * heads * D, THREADS);
+    if (blocks > 65536) blocks = 65536;                     // the kernel strides over the rest
+    const dim3 grid(static_cast<unsigned>(blocks));
+    const cudaError_t e =
+        type == ATT_F32    ? launch_overlapped(&attention_reduce_kernel<float>, grid, THREADS, 0, st, src, slices, dst, L, rows, heads, D)
+        : type == ATT_BF16 ? launch_overlapped(&attention_reduce_kernel<__nv_bfloat16>, grid, THREADS, 0, st, src, slices, dst, L, rows, heads, D)
+                           : launch_overlapped(&attention_reduce_kernel<__half>, grid, THREADS, 0, st, src, slices, dst, L, rows, heads, D);
+    return cuda_status(e, "attention_reduce_kernel");
+}
+
+}  // namespace km

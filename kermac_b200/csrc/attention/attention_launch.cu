@@ -1,0 +1,282 @@
+// Attention behind the C-ABI: checks of arguments, the plan of a call (which kernel, how many pieces) and its launches.
+#include <algorithm>
+#include <cmath>
+
+#include "attention_params.h"
+
+namespace km {
+namespace {
+
+enum Kind { CROSS = 0, PREFIX = 1, GRAD = 2 };
+
+constexpr long long MAX_STRIDE = 1LL << 40;
+
+int check_heads(const char* name, const KmHeads& t, long long rows, long long heads, long long batch) {
+    if (batch * rows * heads > 0 && !t.ptr) return fail(KM_ERR_NULL_POINTER, "%s must not be NULL", name);
+    if (t.stride_l < 0 || t.stride_row < 0 || t.stride_head < 0)
+        return fail(KM_ERR_BAD_STRIDE, "%s must not have a negative stride", name);
+    if (t.stride_l >= MAX_STRIDE || t.stride_row >= MAX_STRIDE || t.stride_head >= MAX_STRIDE)
+        return fail(KM_ERR_BAD_STRIDE, "%s has a stride of 2^40 elements or more", name);
+    return 0;
+}
+// A written tensor must not hold two elements in one place: sorted by stride, each dimension spans the ones before it.
+int check_written(const char* name, const KmHeads& t, long long rows, long long heads, long long batch, int d) {
+    if (int rc = check_heads(name, t, rows, heads, batch)) return rc;
+    std::pair<long long, long long> dims[3] = {{t.stride_l, batch}, {t.stride_row, rows}, {t.stride_head, heads}};
+    std::sort(dims, dims + 3);
+    long long span = d;
+    for (const auto& dim : dims) {
+        if (dim.second <= 1) continue;
+        if (dim.first < span) return fail(KM_ERR_BAD_STRIDE, "%s has strides that put two elements in one place", name);
+        span = dim.first * (dim.second - 1) + span;
+    }
+    return 0;
+}
+
+int check(const KmAttentionArgs* a, Kind kind) {
+    if (!a) return fail(KM_ERR_NULL_POINTER, "args must not be NULL");
+    if (a->l < 0 || a->n < 0 || a->m < 0 || a->prefix < 0) return fail(KM_ERR_BAD_SHAPE, "extents must not be negative");
+    if (a->heads < 0 || a->key_heads < 1 || a->heads % a->key_heads != 0)
+        return fail(KM_ERR_BAD_SHAPE, "heads (%d) must be a multiple of key_heads (%d)", a->heads, a->key_heads);
+    if (a->d < 1 || a->d > 256) return fail(KM_ERR_BAD_SHAPE, "the number of channels must be in [1, 256], got %d", a->d);
+    if (a->type < ATT_F32 || a->type > ATT_F16) return fail(KM_ERR_BAD_ENUM, "type must be a KM_TYPE_*");
+    if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return fail(KM_ERR_BAD_HYPERPARAM, "scale must be finite and not negative");
+    if (kind != PREFIX && a->prefix != 0) return fail(KM_ERR_BAD_SHAPE, "only prefix_attention has a prefix");
+    if (a->m > (1 << 30) || a->prefix > (1 << 30)) return fail(KM_ERR_TOO_LARGE, "more than 2^30 keys");
+    const long long rows = static_cast<long long>(a->l) * a->n * a->heads;
+    if (static_cast<long long>(a->l) * a->n > 0x7fffffffLL || rows > 0x7fffffffLL) return fail(KM_ERR_TOO_LARGE, "batch * queries * heads must be below 2^31");
+    if ((a->k.stride_l == 0) != (a->v.stride_l == 0) && a->l > 1 && a->m > 0)
+        return fail(KM_ERR_BAD_STRIDE, "k and v must both be broadcast over the batch, or neither");
+    const bool any = rows > 0;
+    int rc = check_heads("q", a->q, a->n, a->heads, a->l);
+    if (!rc && any) rc = check_heads("k", a->k, a->m, a->key_heads, a->l);
+    if (!rc && any) rc = check_heads("v", a->v, a->m, a->key_heads, a->l);
+    if (!rc && any && kind == PREFIX) rc = check_heads("k_prefix", a->k_prefix, a->prefix, a->key_heads, 1);
+    if (!rc && any && kind == PREFIX) rc = check_heads("v_prefix", a->v_prefix, a->prefix, a->key_heads, 1);
+    if (rc) return rc;
+    if (a->lengths && a->lengths_stride < 0) return fail(KM_ERR_BAD_STRIDE, "lengths must not have a negative stride");
+    if (a->lse && (a->lse_stride_l < 0 || a->lse_stride_head < 0)) return fail(KM_ERR_BAD_STRIDE, "lse must not have a negative stride");
+    if (kind != GRAD) {
+        if (a->lse && any) {
+            const KmHeads lse = {a->lse, a->lse_stride_l, a->lse_stride_head, 1};       // [l][head][n]
+            if (int bad = check_written("lse", lse, a->heads, a->n, a->l, 1)) return bad;
+        }
+        return check_written("out", a->out, a->n, a->heads, a->l, a->d);
+    }
+    if (any && !a->lse) return fail(KM_ERR_NULL_POINTER, "lse must not be NULL");
+    if ((a->q_batch != a->l && a->q_batch != 1) || (a->kv_batch != a->l && a->kv_batch != 1))
+        return fail(KM_ERR_BAD_SHAPE, "q_batch and kv_batch must be 1 or l");
+    if (a->l > 1 && ((a->q_batch == 1 && a->q.stride_l != 0) || (a->kv_batch == 1 && a->k.stride_l != 0)))
+        return fail(KM_ERR_BAD_STRIDE, "a batch of 1 must have a batch stride of 0");
+    rc = check_heads("out", a->out, a->n, a->heads, a->l);
+    if (!rc) rc = check_heads("grad_out", a->grad_out, a->n, a->heads, a->l);
+    if (!rc) rc = check_written("grad_q", a->grad_q, a->n, a->heads, a->q_batch, a->d);
+    if (!rc) rc = check_written("grad_k", a->grad_k, a->m, a->key_heads, a->kv_batch, a->d);
+    if (!rc) rc = check_written("grad_v", a->grad_v, a->m, a->key_heads, a->kv_batch, a->d);
+    return rc;
+}
+
+Heads heads(const KmHeads& t) { return {static_cast<char*>(t.ptr), t.stride_l, t.stride_row, t.stride_head}; }
+
+// Every row of every head starts on a 16-byte boundary and is a whole number of 16-byte units.
+bool rows_aligned(const KmHeads& t, int type, int d) {
+    const long long unit = 16 / type_bytes(type);
+    return aligned16(t.ptr) && t.stride_l % unit == 0 && t.stride_row % unit == 0 && t.stride_head % unit == 0 && d % unit == 0;
+}
+
+struct Plan {
+    bool few_own, few_prefix;
+    AttentionParams p;
+    long long bytes;
+};
+
+// How many pieces the keys of `blocks` blocks are split into: enough to give every SM `per_sm` blocks, no piece shorter than
+// `least` keys.
+int pieces(long long blocks, long long keys, int per_sm, int least) {
+    if (blocks <= 0 || keys <= 0) return 1;
+    const long long wanted = ceil_div_ll(static_cast<long long>(sm_count()) * per_sm, blocks);
+    return static_cast<int>(std::max(1LL, std::min({wanted, keys / least, 256LL})));
+}
+
+Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool scratch) {
+    Plan plan = {};
+    AttentionParams& p = plan.p;
+    p.L = a.l, p.N = a.n, p.H = a.heads, p.Hk = a.key_heads, p.G = a.heads / a.key_heads, p.D = a.d, p.M = a.m, p.P = a.prefix;
+    p.q = heads(a.q), p.k = heads(a.k), p.v = heads(a.v), p.out = heads(a.out), p.kp = heads(a.k_prefix), p.vp = heads(a.v_prefix);
+    p.lengths = a.lengths, p.lengths_stride = a.lengths_stride;
+    p.lse = a.lse, p.lse_sl = a.lse_stride_l, p.lse_sh = a.lse_stride_head;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.causal = kind == PREFIX;
+    // Keys that a whole batch shares are a prefix without own keys.
+    if (kind == CROSS && a.l > 1 && a.k.stride_l == 0 && !a.lengths && a.m > 0) {
+        p.P = a.m, p.M = 0, p.kp = p.k, p.vp = p.v;
+    }
+    p.vec = rows_aligned(a.q, a.type, a.d) && (p.M == 0 || (rows_aligned(a.k, a.type, a.d) && rows_aligned(a.v, a.type, a.d)));
+    if (p.P > 0) {
+        const KmHeads &k = kind == PREFIX ? a.k_prefix : a.k, &v = kind == PREFIX ? a.v_prefix : a.v;
+        p.vec = p.vec && rows_aligned(k, a.type, a.d) && rows_aligned(v, a.type, a.d);
+    }
+    const long long own_rows = static_cast<long long>(p.N) * p.G, prefix_rows = own_rows * p.L;
+    plan.few_own    = own_rows <= ATT_FEW_ROWS;
+    plan.few_prefix = prefix_rows <= ATT_FEW_ROWS;
+    if (p.M > 0 || p.P == 0) {
+        p.own_tiles  = static_cast<int>(ceil_div_ll(own_rows, plan.few_own ? ATT_FEW_ROWS : ATT_TILE_ROWS));
+        p.own_splits = scratch ? pieces(static_cast<long long>(p.own_tiles) * p.L * p.Hk, p.M, 2, plan.few_own ? 256 : 512) : 1;
+    }
+    if (p.P > 0) {
+        p.prefix_tiles  = static_cast<int>(ceil_div_ll(prefix_rows, plan.few_prefix ? ATT_FEW_ROWS : ATT_TILE_ROWS));
+        p.prefix_splits = scratch ? pieces(static_cast<long long>(p.prefix_tiles) * p.Hk, p.P, 2, plan.few_prefix ? 256 : 512) : 1;
+    }
+    p.parts = p.own_splits + p.prefix_splits;
+    if (p.parts > 1) plan.bytes = static_cast<long long>(p.parts) * p.L * p.N * p.H * (p.D + 1) * 4;
+    return plan;
+}
+
+bool empty(const KmAttentionArgs& a) { return a.l == 0 || a.n == 0 || a.heads == 0; }
+
+// The largest scratch that a call asks for: a plan that wants more takes a single piece for each set of keys.
+constexpr long long MOST_SCRATCH = 512LL << 20;
+
+Plan plan_within(const KmAttentionArgs& a, Kind kind, long long most) {
+    Plan plan = plan_forward(a, kind, true);
+    if (plan.bytes > most) plan = plan_forward(a, kind, false);
+    return plan;
+}
+
+int64_t forward_scratch(const KmAttentionArgs* a, Kind kind) {
+    if (check(a, kind) || empty(*a)) return 0;
+    return plan_within(*a, kind, MOST_SCRATCH).bytes;
+}
+
+int forward(const KmAttentionArgs* a, Kind kind, void* stream) {
+    int rc = check(a, kind);
+    if (rc) return rc;
+    if (empty(*a)) return 0;
+    rc = require_sm100();
+    if (rc) return rc;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    Plan plan = plan_within(*a, kind, a->scratch ? std::min<long long>(MOST_SCRATCH, a->scratch_bytes) : 0);
+    if (plan.bytes > 0) {
+        if (!a->scratch || a->scratch_bytes < plan.bytes || !aligned16(a->scratch))
+            return fail(KM_ERR_NULL_POINTER, "attention: %lld bytes of 16-byte aligned scratch are needed", plan.bytes);
+        plan.p.part_o   = static_cast<float*>(a->scratch);
+        plan.p.part_lse = plan.p.part_o + static_cast<long long>(plan.p.parts) * plan.p.L * plan.p.N * plan.p.H * plan.p.D;
+    }
+    const bool own = plan.p.own_splits > 0, prefix = plan.p.prefix_splits > 0;
+    if (own && prefix && plan.few_own != plan.few_prefix) {
+        AttentionParams p = plan.p;
+        p.own_tiles = 0;                                   // the blocks of the prefix alone
+        rc = attention_rows_launch(p, a->type, plan.few_prefix, st);
+        p = plan.p, p.prefix_tiles = 0;
+        if (!rc) rc = attention_rows_launch(p, a->type, plan.few_own, st);
+    } else {
+        rc = attention_rows_launch(plan.p, a->type, own ? plan.few_own : plan.few_prefix, st);
+    }
+    if (!rc && plan.p.parts > 1) rc = attention_join_launch(plan.p, a->type, st);
+    return rc;
+}
+
+struct GradPlan {
+    AttentionGradParams p;
+    long long delta, peaks, dq, dkv;     // floats of scratch, each a multiple of 4
+    long long bytes() const { return 4 * (delta + peaks + dq + 2 * dkv); }
+};
+long long round4(long long n) { return (n + 3) & ~3LL; }
+
+GradPlan plan_grad(const KmAttentionArgs& a) {
+    GradPlan plan = {};
+    AttentionGradParams& p = plan.p;
+    p.L = a.l, p.N = a.n, p.H = a.heads, p.Hk = a.key_heads, p.G = a.heads / a.key_heads, p.D = a.d, p.M = a.m;
+    p.q = heads(a.q), p.k = heads(a.k), p.v = heads(a.v), p.out = heads(a.out), p.dout = heads(a.grad_out);
+    p.dq = heads(a.grad_q), p.dk = heads(a.grad_k), p.dv = heads(a.grad_v);
+    p.lengths = a.lengths, p.lengths_stride = a.lengths_stride;
+    p.lse = a.lse, p.lse_sl = a.lse_stride_l, p.lse_sh = a.lse_stride_head;
+    p.scale = a.scale, p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.vec = rows_aligned(a.q, a.type, a.d) && rows_aligned(a.k, a.type, a.d) && rows_aligned(a.v, a.type, a.d) &&
+            rows_aligned(a.grad_out, a.type, a.d);
+    p.q_slices = a.q_batch == 1 && a.l > 1 ? a.l : 1;
+    p.kv_batch = a.kv_batch;
+    // The sum over queries of a key tile is split where the key tiles alone do not fill the SMs.
+    const long long tiles = ceil_div_ll(a.m, ATT_GRAD_ROWS) * a.key_heads * a.kv_batch;
+    const long long sum   = static_cast<long long>(a.kv_batch == 1 ? a.l : 1) * p.G * a.n;
+    p.kv_slices = pieces(tiles, sum, 2, 512);
+    if (static_cast<long long>(p.kv_slices) * a.kv_batch * a.m * a.key_heads * a.d > (MOST_SCRATCH >> 3)) p.kv_slices = 1;
+    plan.delta = round4(static_cast<long long>(a.l) * a.heads * a.n);
+    if (a.type == ATT_F16) {
+        p.peak_count = static_cast<int>(ceil_div_ll(a.n, ATT_PEAK_ROWS));
+        plan.peaks   = round4(static_cast<long long>(a.l) * a.heads * p.peak_count);
+    }
+    if (p.q_slices > 1) plan.dq = round4(static_cast<long long>(p.q_slices) * a.n * a.heads * a.d);
+    if (p.kv_slices > 1) plan.dkv = round4(static_cast<long long>(p.kv_slices) * a.kv_batch * a.m * a.key_heads * a.d);
+    return plan;
+}
+
+// Zeros for a gradient that no pair of query and key reaches.
+int clear(const Heads& t, int batch, int rows, int n_heads, int d, int type, cudaStream_t st) {
+    if (static_cast<long long>(batch) * rows * n_heads == 0) return 0;
+    return attention_reduce_launch(nullptr, 0, t, batch, rows, n_heads, d, type, st);
+}
+
+int gradient(const KmAttentionArgs* a, void* stream) {
+    int rc = check(a, GRAD);
+    if (rc) return rc;
+    if (empty(*a) && (a->m == 0 || a->kv_batch == 0)) return 0;
+    rc = require_sm100();
+    if (rc) return rc;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    GradPlan plan = plan_grad(*a);
+    AttentionGradParams& p = plan.p;
+    if (empty(*a) || a->m == 0) {
+        rc = clear(p.dq, a->q_batch, p.N, p.H, p.D, a->type, st);
+        if (!rc) rc = clear(p.dk, p.kv_batch, p.M, p.Hk, p.D, a->type, st);
+        if (!rc) rc = clear(p.dv, p.kv_batch, p.M, p.Hk, p.D, a->type, st);
+        return rc;
+    }
+    if (!a->scratch || a->scratch_bytes < plan.bytes() || !aligned16(a->scratch))
+        return fail(KM_ERR_NULL_POINTER, "attention gradient: %lld bytes of 16-byte aligned scratch are needed", plan.bytes());
+    float* at = static_cast<float*>(a->scratch);
+    p.delta = at, at += plan.delta;
+    if (plan.peaks) p.peaks = at, at += plan.peaks;
+    if (plan.dq) p.dq_part = at, at += plan.dq;
+    if (plan.dkv) p.dk_part = at, p.dv_part = at + plan.dkv;
+    rc = attention_delta_launch(p, a->type, st);
+    if (!rc) rc = attention_grad_rows_launch(p, a->type, st);
+    if (!rc && p.q_slices > 1) rc = attention_reduce_launch(p.dq_part, p.q_slices, p.dq, 1, p.N, p.H, p.D, a->type, st);
+    if (!rc && p.kv_slices > 1) rc = attention_reduce_launch(p.dk_part, p.kv_slices, p.dk, p.kv_batch, p.M, p.Hk, p.D, a->type, st);
+    if (!rc && p.kv_slices > 1) rc = attention_reduce_launch(p.dv_part, p.kv_slices, p.dv, p.kv_batch, p.M, p.Hk, p.D, a->type, st);
+    return rc;
+}
+
+}  // namespace
+}  // namespace km
+
+extern "C" {
+
+int kermac_b200_cross_attention(const KmAttentionArgs* args, void* stream) { return km::forward(args, km::CROSS, stream); }
+int kermac_b200_prefix_attention(const KmAttentionArgs* args, void* stream) { return km::forward(args, km::PREFIX, stream); }
+int kermac_b200_cross_attention_grad(const KmAttentionArgs* args, void* stream) { return km::gradient(args, stream); }
+int64_t kermac_b200_cross_attention_scratch_bytes(const KmAttentionArgs* args) { return km::forward_scratch(args, km::CROSS); }
+int64_t kermac_b200_prefix_attention_scratch_bytes(const KmAttentionArgs* args) { return km::forward_scratch(args, km::PREFIX); }
+int64_t kermac_b200_cross_attention_grad_scratch_bytes(const KmAttentionArgs* args) {
+    if (km::check(args, km::GRAD) || km::empty(*args) || args->m == 0) return 0;
+    return km::plan_grad(*args).bytes();
+}
+
+int kermac_b200_describe_attention(const KmAttentionArgs* args, int32_t kind, char* buf, int32_t buf_len) {
+    using namespace km;
+    if (kind < CROSS || kind > GRAD) return fail(KM_ERR_BAD_ENUM, "kind must be 0 (cross), 1 (prefix) or 2 (gradient)");
+    if (int rc = check(args, static_cast<Kind>(kind))) return rc;
+    if (!buf || buf_len <= 0) return fail(KM_ERR_NULL_POINTER, "buf must not be NULL");
+    if (kind == GRAD) {
+        const GradPlan plan = plan_grad(*args);
+        snprintf(buf, buf_len, "grad=rows q_slices=%d kv_slices=%d scratch=%lld", plan.p.q_slices, plan.p.kv_slices, plan.bytes());
+    } else {
+        const Plan plan = plan_within(*args, static_cast<Kind>(kind), MOST_SCRATCH);
+        snprintf(buf, buf_len, "own=%s tiles=%d splits=%d prefix=%s tiles=%d splits=%d scratch=%lld", plan.few_own ? "few" : "rows",
+                 plan.p.own_tiles, plan.p.own_splits, plan.few_prefix ? "few" : "rows", plan.p.prefix_tiles, plan.p.prefix_splits,
+                 plan.bytes);
+    }
+    return 0;
+}
+
+}  // extern "C"

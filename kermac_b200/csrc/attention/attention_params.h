@@ -1,0 +1,74 @@
+// Parameter blocks and launchers of the attention kernels, shared by their translation units.
+#pragma once
+
+#include "../../../include/kermac_b200_attention.h"
+#include "../km_host.h"
+
+namespace km {
+
+// One argument of heads [l][row][head][channel], channels contiguous; strides in elements, stride_l 0 broadcasts.
+struct Heads {
+    char*     ptr;
+    long long sl, sr, sh;
+};
+
+// Forward pass.  For one batch entry and key head the G = H / Hk query heads of N queries are N * G rows (row = n * G + g)
+// against the entry's own keys; against a shared prefix the rows of all batch entries are one matrix (row =
+// (l * N + n) * G + g), so its keys are read once for the whole batch.  Each of the two sets of keys may be split among
+// blocks; every piece leaves a normalised sum and its log2-sum-exp2 (a "part"), which join_kernel adds up.
+struct AttentionParams {
+    int L, N, H, Hk, G, D, M, P;
+    Heads q, k, v, kp, vp, out;
+    const int* lengths; long long lengths_stride;
+    float* lse; long long lse_sl, lse_sh;
+    float scale_log2;                    // scale * log2(e)
+    int   causal;                        // own key j is seen by query n when j <= length - N + n
+    int   own_tiles, own_splits;         // row tiles of one (l, key head), pieces of its keys; 0 pieces: no own keys
+    int   prefix_tiles, prefix_splits;
+    int   parts;                         // pieces of one row: own_splits + prefix_splits; 1: results are written directly
+    float* part_o;                       // [part][l][n][h][D]
+    float* part_lse;                     // [part][l][n][h], log2 domain
+    int   vec;                           // every row of k, v, kp, vp and q can be read 16 bytes at a time
+    int   vec_out;                       // rows of out can be written 16 bytes at a time
+};
+
+// Backward pass: dq, dk and dv from the forward pass's output and lse.
+struct AttentionGradParams {
+    int L, N, H, Hk, G, D, M;
+    Heads q, k, v, out, dout;
+    const int* lengths; long long lengths_stride;
+    const float* lse; long long lse_sl, lse_sh;
+    float scale, scale_log2;
+    float* delta;                        // [l][h][n]: sum over channels of dout * out
+    // float16 only, else null: [l][h][peaks], the largest |dout| of ATT_PEAK_ROWS queries.  The weights' gradients are
+    // multiplied by the power of two that brings the largest |dout| of the sum they enter to [1, 2) before they are rounded
+    // to 16 bits, and the sums divided by it: float16 ends at 6e-8, and a weight of 1e-4 times a gradient of 1e-3 does not.
+    float* peaks; int peak_count;
+    // Destinations.  slices 1: the gradients in the inputs' type.  More: 32-bit partial sums [slice][...] that
+    // grad_reduce adds up, where a broadcast input's gradient is a sum over the batch or the sum is split.
+    Heads dq, dk, dv;
+    float *dq_part, *dk_part, *dv_part;
+    int   q_slices;                      // 1, or L for a broadcast q
+    int   kv_batch;                      // batch entries of k and v: 1 or L
+    int   kv_slices;                     // pieces of the sum over (l of a broadcast k, head of the group, query tile)
+    int   vec;
+};
+
+enum { ATT_F32 = KM_TYPE_FLOAT32, ATT_BF16 = KM_TYPE_BFLOAT16, ATT_F16 = KM_TYPE_FLOAT16 };
+
+// attention_rows.cu (mma.sync): any layout and type.  rows_tile() rows per block; `few` is the form whose warps share 16 rows.
+int  attention_rows_launch(const AttentionParams& p, int type, bool few, cudaStream_t st);
+constexpr int ATT_FEW_ROWS = 16, ATT_TILE_ROWS = 64;
+int  attention_join_launch(const AttentionParams& p, int type, cudaStream_t st);
+// attention_grad_rows.cu
+constexpr int ATT_GRAD_ROWS = 64, ATT_PEAK_ROWS = 64;
+int  attention_delta_launch(const AttentionGradParams& p, int type, cudaStream_t st);
+int  attention_grad_rows_launch(const AttentionGradParams& p, int type, cudaStream_t st);
+// dst[i] = sum over slices of src[slice][i] for a [rows_l][rows][heads][D] array
+int  attention_reduce_launch(const float* src, int slices, const Heads& dst, int L, int rows, int heads, int D, int type,
+                             cudaStream_t st);
+
+inline int padded_channels(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+inline int type_bytes(int type) { return type == ATT_F32 ? 4 : 2; }
+
+}  // namespace km

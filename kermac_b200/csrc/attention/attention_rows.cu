@@ -1,0 +1,335 @@
+// Attention for any layout, type and width up to 256 channels: softmax(scale Q K^T) V with mma.sync, and the kernel that joins
+// the parts of a split.
+//
+// One pass over the keys with a running maximum m and sum l per row: a tile's scores S = Q K^T raise m, what was summed under
+// the old one is scaled by exp2(m_old - m_new), and P = exp2(S - m) is multiplied with V straight from the registers it was
+// computed in (the accumulator layout of one product is the operand layout of the next).
+#include "attention_mma.cuh"
+
+namespace km {
+namespace att {
+namespace {
+
+// How a block works.  FEW: one tile of 16 rows, the four warps take key tiles of their own in turn and add up at the end
+// (decoding steps: bound by reading the keys, so the warps wait for no one and have three tiles each under way).  Otherwise:
+// 64 rows, 16 a warp, and one key tile for all.
+template <typename T, int DP, bool FEW>
+struct Shape {
+    static constexpr int ROWS   = FEW ? ATT_FEW_ROWS : ATT_TILE_ROWS;
+    static constexpr int KEYS   = sizeof(T) == 2 ? (FEW ? (DP > 128 ? 16 : 32) : (DP > 128 ? 32 : 64))
+                                                 : (FEW ? (DP > 128 ? 8 : 16) : (DP > 128 ? 16 : 32));
+    static constexpr int STAGES = FEW ? 3 : 2;
+    static constexpr int GROUPS = FEW ? WARPS : 1;                 // sets of threads with key tiles of their own
+    static constexpr int TILE   = Tile<T, DP>::bytes(KEYS);
+    static constexpr int Q      = Tile<T, DP>::bytes(ROWS);
+    static constexpr int MERGE  = FEW ? WARPS * ROWS * (DP + 2) * 4 : 0;
+    static constexpr int RING   = GROUPS * STAGES * 2 * TILE;
+    static constexpr int SMEM   = Q + (RING > MERGE ? RING : MERGE);
+};
+
+// What one block computes.
+struct Work {
+    const char *k, *v;            // first key of the head
+    long long   k_sr, v_sr;
+    int         l, hk;            // l: the batch entry, or -1 for rows of all entries
+    int         row0, rows;       // rows of the (l, key head) matrix, and how many there are
+    int         first, end;       // keys
+    int         length, part;
+    bool        causal;
+};
+
+template <typename T>
+__device__ __forceinline__ Work find_work(const AttentionParams& p, int block, int rows_per_block, int keys_per_tile) {
+    Work w;
+    const int prefix_blocks = p.Hk * p.prefix_tiles * p.prefix_splits;
+    int       tile, split, splits;
+    if (block < prefix_blocks) {
+        split  = block % p.prefix_splits, block /= p.prefix_splits;
+        tile   = block % p.prefix_tiles, w.hk = block / p.prefix_tiles;
+        splits = p.prefix_splits;
+        w.l = -1, w.rows = p.L * p.N * p.G, w.length = p.P, w.part = split, w.causal = false;
+        w.k = p.kp.ptr + w.hk * p.kp.sh * static_cast<long long>(sizeof(T)), w.k_sr = p.kp.sr;
+        w.v = p.vp.ptr + w.hk * p.vp.sh * static_cast<long long>(sizeof(T)), w.v_sr = p.vp.sr;
+    } else {
+        block -= prefix_blocks;
+        split = block % p.own_splits, block /= p.own_splits;
+        tile  = block % p.own_tiles, block /= p.own_tiles;
+        w.hk = block % p.Hk, w.l = block / p.Hk;
+        splits = p.own_splits;
+        w.rows = p.N * p.G, w.length = key_count(p.lengths, p.lengths_stride, w.l, p.M), w.part = p.prefix_splits + split;
+        w.causal = p.causal;
+        w.k = p.k.ptr + (w.l * p.k.sl + w.hk * p.k.sh) * static_cast<long long>(sizeof(T)), w.k_sr = p.k.sr;
+        w.v = p.v.ptr + (w.l * p.v.sl + w.hk * p.v.sh) * static_cast<long long>(sizeof(T)), w.v_sr = p.v.sr;
+    }
+    w.row0 = tile * rows_per_block;
+    // pieces of whole tiles, from the length that the entry has
+    const int tiles = (w.length + keys_per_tile - 1) / keys_per_tile;
+    const int each  = (tiles + splits - 1) / splits;
+    const long long first = static_cast<long long>(split) * each * keys_per_tile, end = first + static_cast<long long>(each) * keys_per_tile;
+    w.first = static_cast<int>(first < w.length ? first : w.length);
+    w.end   = static_cast<int>(end < w.length ? end : w.length);
+    return w;
+}
+
+struct Row { int l, n, h; };
+__device__ __forceinline__ Row find_row(const AttentionParams& p, const Work& w, int r) {
+    Row row;
+    const int q = r / p.G;
+    row.h = w.hk * p.G + r - q * p.G;
+    row.l = w.l >= 0 ? w.l : q / p.N;
+    row.n = w.l >= 0 ? q : q - row.l * p.N;
+    return row;
+}
+// First own key that the row does not see.
+__device__ __forceinline__ int row_limit(const AttentionParams& p, const Work& w, int r) {
+    return w.causal ? w.length - p.N + r / p.G + 1 : w.length;
+}
+
+// The two columns (c, c + 1) of a finished row: into out, or into its part.
+template <typename T>
+__device__ __forceinline__ void put_pair(const AttentionParams& p, const Work& w, const Row& row, int c, float x, float y) {
+    if (c >= p.D) return;
+    if (p.parts == 1) {
+        T* o = reinterpret_cast<T*>(p.out.ptr) + row.l * p.out.sl + row.n * p.out.sr + row.h * p.out.sh + c;
+        o[0] = Type<T>::to(x);
+        if (c + 1 < p.D) o[1] = Type<T>::to(y);
+    } else {
+        float* o = p.part_o + ((((static_cast<long long>(w.part) * p.L + row.l) * p.N + row.n) * p.H) + row.h) * p.D + c;
+        o[0] = x;
+        if (c + 1 < p.D) o[1] = y;
+    }
+}
+// lse2: log2 of the sum of exp2; -inf for a row without keys.
+__device__ __forceinline__ void put_lse(const AttentionParams& p, const Work& w, const Row& row, float lse2) {
+    if (p.parts != 1)
+        p.part_lse[((static_cast<long long>(w.part) * p.L + row.l) * p.N + row.n) * p.H + row.h] = lse2;
+    else if (p.lse)
+        p.lse[row.l * p.lse_sl + row.h * p.lse_sh + row.n] = lse2 * LN2;
+}
+
+template <typename T, int DP, bool FEW>
+__global__ void __launch_bounds__(THREADS) attention_rows_kernel(const AttentionParams p) {
+    typedef Shape<T, DP, FEW> S;
+    typedef Tile<T, DP>       TL;
+    constexpr int NT = S::KEYS / 8, CT = DP / 8;
+    extern __shared__ __align__(16) char smem[];
+    T* const  tile_q = reinterpret_cast<T*>(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    after_previous_grid();
+
+    const Work w = find_work<T>(p, blockIdx.x, S::ROWS, S::KEYS);
+    const T *  k = reinterpret_cast<const T*>(w.k), *v = reinterpret_cast<const T*>(w.v);
+
+    for (int i = threadIdx.x; i < S::ROWS * TL::CHUNKS; i += THREADS) {
+        const int r = i / TL::CHUNKS, c = (i % TL::CHUNKS) * Type<T>::CHUNK;
+        const T*  q = nullptr;
+        if (w.row0 + r < w.rows) {
+            const Row row = find_row(p, w, w.row0 + r);
+            q = reinterpret_cast<const T*>(p.q.ptr) + row.l * p.q.sl + row.n * p.q.sr + row.h * p.q.sh;
+        }
+        copy_chunk(tile_q + r * TL::LD + c, q, reinterpret_cast<const T*>(p.q.ptr), c, p.D, p.vec);
+    }
+    copy_commit();
+
+    // the key tiles of this group: `step` tiles apart
+    const int group = FEW ? warp : 0, index = FEW ? lane : static_cast<int>(threadIdx.x), members = FEW ? 32 : THREADS;
+    char* const ring  = smem + S::Q + group * S::STAGES * 2 * S::TILE;
+    const int   tiles = (w.end - w.first + S::KEYS - 1) / S::KEYS;
+    const int   mine  = (tiles - group + S::GROUPS - 1) / S::GROUPS;
+    auto load = [&](int i) {
+        if (i < mine) {
+            T* const  dst   = reinterpret_cast<T*>(ring + (i % S::STAGES) * 2 * S::TILE);
+            const int first = w.first + (i * S::GROUPS + group) * S::KEYS;
+            copy_rows<T, DP>(dst, k, w.k_sr, first, w.end, S::KEYS, p.D, p.vec, index, members);
+            copy_rows<T, DP>(dst + S::KEYS * TL::LD, v, w.v_sr, first, w.end, S::KEYS, p.D, p.vec, index, members);
+        }
+        copy_commit();
+    };
+    auto group_sync = [] {
+        if (FEW) __syncwarp(); else __syncthreads();
+    };
+
+    float o[CT][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < CT; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.0f;
+    const int my_row = (FEW ? 0 : warp * 16) + g;
+    int       limit[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        limit[i] = row_limit(p, w, w.row0 + my_row + 8 * i);
+        limit[i] = limit[i] < w.end ? limit[i] : w.end;
+    }
+
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; ++i) load(i);
+    copy_wait<S::STAGES - 1>();              // Q has arrived
+    __syncthreads();
+    const T* const my_q = tile_q + (FEW ? 0 : warp * 16) * TL::LD;
+
+    for (int i = 0; i < mine; ++i) {
+        load(i + S::STAGES - 1);
+        copy_wait<S::STAGES - 1>();
+        group_sync();
+        const T* const tile_k = reinterpret_cast<const T*>(ring + (i % S::STAGES) * 2 * S::TILE);
+        const int      first  = w.first + (i * S::GROUPS + group) * S::KEYS;
+        float s[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+        product_nt<T, DP, NT>(s, my_q, tile_k);
+
+        float best[2] = {top[0], top[1]};
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int key = first + j * 8 + 2 * t + (e & 1);
+                s[j][e] = key < limit[e >> 1] ? s[j][e] * p.scale_log2 : -INFINITY;
+                best[e >> 1] = fmaxf(best[e >> 1], s[j][e]);
+            }
+        float base[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            best[r] = quad_max(best[r]);
+            base[r] = best[r] == -INFINITY ? 0.0f : best[r];     // a row that has seen no key yet: exp2(-inf - 0) = 0
+            const float shrink = ex2_approx(top[r] - base[r]);
+            top[r] = best[r];
+            sum[r] *= shrink;
+#pragma unroll
+            for (int c = 0; c < CT; ++c) o[c][2 * r] *= shrink, o[c][2 * r + 1] *= shrink;
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[j][e] = ex2_approx(s[j][e] - base[e >> 1]);
+                sum[e >> 1] += s[j][e];
+            }
+        product_nn<T, DP, NT, CT>(o, s, tile_k + S::KEYS * TL::LD);
+        group_sync();
+    }
+    sum[0] = quad_sum(sum[0]), sum[1] = quad_sum(sum[1]);
+
+    if constexpr (!FEW) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int at = w.row0 + my_row + 8 * r;
+            if (at >= w.rows) continue;
+            const Row   row = find_row(p, w, at);
+            const float by  = sum[r] == 0.0f ? 0.0f : 1.0f / sum[r];
+            if (t == 0) put_lse(p, w, row, top[r] + lg2_approx(sum[r]));
+#pragma unroll
+            for (int c = 0; c < CT; ++c) put_pair<T>(p, w, row, c * 8 + 2 * t, o[c][2 * r] * by, o[c][2 * r + 1] * by);
+        }
+    } else {
+        copy_wait<0>();
+        __syncthreads();                     // the ring is free: the warps' sums go there
+        float* const sums = reinterpret_cast<float*>(smem + S::Q);
+        constexpr int W = DP + 2;            // DP channels, the maximum and the sum
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float* const mine_at = sums + (warp * S::ROWS + g + 8 * r) * W;
+#pragma unroll
+            for (int c = 0; c < CT; ++c) *reinterpret_cast<float2*>(mine_at + c * 8 + 2 * t) = make_float2(o[c][2 * r], o[c][2 * r + 1]);
+            if (t == 0) mine_at[DP] = top[r], mine_at[DP + 1] = sum[r];
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < S::ROWS * (DP / 2); i += THREADS) {
+            const int r = i / (DP / 2), c = (i % (DP / 2)) * 2;
+            if (w.row0 + r >= w.rows || c >= p.D) continue;
+            float best = -INFINITY, total = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
+            for (int j = 0; j < WARPS; ++j) best = fmaxf(best, sums[(j * S::ROWS + r) * W + DP]);
+            const float base = best == -INFINITY ? 0.0f : best;
+#pragma unroll
+            for (int j = 0; j < WARPS; ++j) {
+                const float* const from   = sums + (j * S::ROWS + r) * W;
+                const float        weight = ex2_approx(from[DP] - base);
+                total += weight * from[DP + 1], x += weight * from[c], y += weight * from[c + 1];
+            }
+            const Row   row = find_row(p, w, w.row0 + r);
+            const float by  = total == 0.0f ? 0.0f : 1.0f / total;
+            if (c == 0) put_lse(p, w, row, best + lg2_approx(total));
+            put_pair<T>(p, w, row, c, x * by, y * by);
+        }
+    }
+}
+
+// Adds up the parts of each row, in the order of the parts: out = sum_i 2^(lse_i - lse) o_i.  One warp a row.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) attention_join_kernel(const AttentionParams p) {
+    after_previous_grid();
+    const long long rows = static_cast<long long>(p.L) * p.N * p.H;
+    const long long row  = static_cast<long long>(blockIdx.x) * WARPS + (threadIdx.x >> 5);
+    const int       lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    float best = -INFINITY;
+    for (int i = lane; i < p.parts; i += 32) best = fmaxf(best, p.part_lse[i * rows + row]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
+    const float base = best == -INFINITY ? 0.0f : best;
+    float total = 0.0f, x[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) x[c] = 0.0f;
+    for (int i = 0; i < p.parts; ++i) {
+        const float lse = p.part_lse[i * rows + row];
+        if (lse == -INFINITY) continue;      // a part without keys has written no sum
+        const float  weight = ex2_approx(lse - base);
+        const float* from   = p.part_o + (i * rows + row) * p.D;
+        total += weight;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            if (c * 32 + lane < p.D) x[c] += weight * from[c * 32 + lane];
+    }
+    const int       h = static_cast<int>(row % p.H);
+    const long long ln = row / p.H;
+    const int       l = static_cast<int>(ln / p.N), n = static_cast<int>(ln - static_cast<long long>(l) * p.N);
+    const float     by = total == 0.0f ? 0.0f : 1.0f / total;
+    T* const        o  = reinterpret_cast<T*>(p.out.ptr) + l * p.out.sl + n * p.out.sr + h * p.out.sh;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        if (c * 32 + lane < p.D) o[c * 32 + lane] = Type<T>::to(x[c] * by);
+    if (p.lse && lane == 0) p.lse[l * p.lse_sl + h * p.lse_sh + n] = (best + lg2_approx(total)) * LN2;
+}
+
+template <typename T, int DP, bool FEW>
+int launch_rows(const AttentionParams& p, cudaStream_t st) {
+    constexpr int smem = Shape<T, DP, FEW>::SMEM;
+    static_assert(smem <= 227 * 1024, "more shared memory than a block has");
+    auto* const kernel = &attention_rows_kernel<T, DP, FEW>;
+    int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute");
+    if (rc) return rc;
+    const long long blocks = static_cast<long long>(p.Hk) * p.prefix_tiles * p.prefix_splits +
+                             static_cast<long long>(p.L) * p.Hk * p.own_tiles * p.own_splits;
+    if (blocks > 0x7fffffffLL) return fail(KM_ERR_TOO_LARGE, "attention: more than 2^31 - 1 blocks");
+    return cuda_status(launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks)), THREADS, smem, st, p), "attention_rows_kernel");
+}
+template <typename T>
+int launch_type(const AttentionParams& p, bool few, cudaStream_t st) {
+    switch (padded_channels(p.D)) {
+        case 64: return few ? launch_rows<T, 64, true>(p, st) : launch_rows<T, 64, false>(p, st);
+        case 128: return few ? launch_rows<T, 128, true>(p, st) : launch_rows<T, 128, false>(p, st);
+        default: return few ? launch_rows<T, 256, true>(p, st) : launch_rows<T, 256, false>(p, st);
+    }
+}
+
+}  // namespace
+}  // namespace att
+
+int attention_rows_launch(const AttentionParams& p, int type, bool few, cudaStream_t st) {
+    using namespace att;
+    if (type == ATT_F32) return launch_type<float>(p, few, st);
+    return type == ATT_BF16 ? launch_type<__nv_bfloat16>(p, few, st) : launch_type<__half>(p, few, st);
+}
+
+int attention_join_launch(const AttentionParams& p, int type, cudaStream_t st) {
+    using namespace att;
+    const long long blocks = ceil_div_ll(static_cast<long long>(p.L) * p.N * p.H, WARPS);
+    if (blocks > 0x7fffffffLL) return fail(KM_ERR_TOO_LARGE, "attention: more than 2^31 - 1 blocks");
+    const dim3 grid(static_cast<unsigned>(blocks));
+    const cudaError_t e = type == ATT_F32    ? launch_overlapped(&attention_join_kernel<float>, grid, THREADS, 0, st, p)
+                          : type == ATT_BF16 ? launch_overlapped(&attention_join_kernel<__nv_bfloat16>, grid, THREADS, 0, st, p)
+                                             : launch_overlapped(&attention_join_kernel<__half>, grid, THREADS, 0, st, p);
+    return cuda_status(e, "attention_join_kernel");
+}
+
+}  // namespace km

@@ -1,0 +1,243 @@
+"""cross_attention, its gradient and prefix_attention without a GPU: the oracle against autograd, the C-ABI's layout, what calls
+are refused, and the plans."""
+import ctypes
+import glob
+import math
+import os
+import re
+import subprocess
+
+import pytest
+import torch
+
+import kermac_b200 as kermac
+from kermac_b200 import _native, attention
+from oracle import attention_oracle as ao
+from test_abi import ROOT
+
+HEADER = os.path.join(ROOT, "include", "kermac_b200_attention.h")
+
+
+def test_oracle_gradient_is_the_gradient_of_the_oracle():
+    torch.manual_seed(0)
+    L, N, M, H, Hk, D, scale = 2, 5, 7, 4, 2, 3, 0.7
+    q, k, v = (torch.randn(L, n, h, D, dtype=torch.float64, requires_grad=True) for n, h in ((N, H), (M, Hk), (M, Hk)))
+    lengths = [7, 4]
+    s = torch.einsum("lnhd,lmhd->lhnm", q, k.repeat_interleave(2, dim=2)) * scale
+    for l, n in enumerate(lengths):
+        mask = torch.arange(M) >= n
+        s = s.masked_fill(mask[None, None, None, :] & (torch.arange(L) == l)[:, None, None, None], -math.inf)
+    out = torch.einsum("lhnm,lmhd->lnhd", torch.softmax(s, dim=-1), v.repeat_interleave(2, dim=2))
+    g = torch.randn_like(out)
+    grads = torch.autograd.grad(out, (q, k, v), g)
+    f = [t.detach().float() for t in (q, k, v, g)]
+    want, _, bound, _ = ao.attention(*f[:3], lengths, scale)
+    assert (want - out.detach()).abs().max() < 1e-5
+    found = ao.attention_grad(*f, lengths, scale)
+    for name, grad in zip(("grad_q", "grad_k", "grad_v"), grads):
+        assert (found[name][0] - grad).abs().max() < 1e-5
+        assert found[name][1].shape == grad.shape and torch.all(found[name][1] < 1e-3)
+
+
+def _c_args(**kw):
+    """Arguments of a call that would be accepted; the pointers are never followed, because these tests launch nothing."""
+    a = _native.KmAttentionArgs()
+    a.l, a.n, a.m, a.heads, a.key_heads, a.d, a.type = 2, 3, 5, 4, 2, 8, _native.TYPE_BFLOAT16
+    a.scale, a.q_batch, a.kv_batch = 0.5, 2, 2
+    for name, rows, heads in (("q", 3, 4), ("k", 5, 2), ("v", 5, 2), ("out", 3, 4), ("grad_out", 3, 4), ("grad_q", 3, 4),
+                              ("grad_k", 5, 2), ("grad_v", 5, 2), ("k_prefix", 6, 2), ("v_prefix", 6, 2)):
+        setattr(a, name, _native.KmHeads(4096, rows * heads * 8, heads * 8, 8))
+    a.lse, a.lse_stride_l, a.lse_stride_head = 4096, 12, 3
+    for name, value in kw.items():
+        if isinstance(value, tuple):
+            tensor = getattr(a, name)
+            setattr(tensor, *value)
+            setattr(a, name, tensor)
+        else:
+            setattr(a, name, value)
+    return a
+
+
+REFUSED = [
+    (dict(l=-1), 0, -2), (dict(n=-1), 1, -2), (dict(m=-1), 2, -2), (dict(prefix=-1), 1, -2), (dict(prefix=3), 0, -2),
+    (dict(prefix=3), 2, -2), (dict(key_heads=0), 0, -2), (dict(key_heads=3), 0, -2), (dict(d=0), 0, -2), (dict(d=257), 2, -2),
+    (dict(type=3), 0, -4), (dict(type=-1), 0, -4), (dict(scale=math.nan), 0, -5), (dict(scale=math.inf), 0, -5),
+    (dict(scale=-1.0), 2, -5), (dict(q=("ptr", None)), 0, -1), (dict(k=("ptr", None)), 1, -1), (dict(v=("ptr", None)), 2, -1),
+    (dict(out=("ptr", None)), 0, -1), (dict(lse=None), 2, -1), (dict(grad_out=("ptr", None)), 2, -1),
+    (dict(grad_k=("ptr", None)), 2, -1), (dict(prefix=6, k_prefix=("ptr", None)), 1, -1),
+    (dict(q=("stride_row", -8)), 0, -3), (dict(v=("stride_l", -8)), 2, -3), (dict(k=("stride_head", 1 << 40)), 0, -3),
+    (dict(out=("stride_row", 8)), 0, -3), (dict(out=("stride_l", 0)), 0, -3), (dict(grad_v=("stride_head", 4)), 2, -3),
+    (dict(lse_stride_head=2), 0, -3), (dict(lse_stride_l=-1), 1, -3), (dict(k=("stride_l", 0)), 0, -3),
+    (dict(lengths=4096, lengths_stride=-1), 0, -3), (dict(q_batch=3), 2, -2), (dict(kv_batch=0), 2, -2),
+    (dict(q_batch=1), 2, -3), (dict(kv_batch=1), 2, -3), (dict(m=(1 << 30) + 1), 0, -6), (dict(l=1 << 20, n=1 << 20), 0, -6),
+]
+
+
+@pytest.mark.parametrize("changes, kind, code", REFUSED, ids=str)
+def test_the_c_abi_refuses(changes, kind, code):
+    args = _c_args(**changes)
+    assert getattr(_native.lib(), _native.ATTENTION_SYMBOLS[kind])(ctypes.byref(args), None) == code
+    assert _native.last_error()
+    assert _native.attention_scratch_bytes(args, kind) == 0
+    with pytest.raises(ValueError):
+        _native.launch_attention(args, kind, 0)
+    with pytest.raises(ValueError):
+        _native.describe_attention(args, kind)
+
+
+def test_the_c_abi_refuses_no_arguments_at_all():
+    for kind in range(3):
+        assert getattr(_native.lib(), _native.ATTENTION_SYMBOLS[kind])(None, None) == -1
+        assert getattr(_native.lib(), _native.ATTENTION_SYMBOLS[3 + kind])(None) == 0
+    assert _native.lib().kermac_b200_describe_attention(ctypes.byref(_c_args()), 3, None, 0) == -4
+    assert _native.lib().kermac_b200_describe_attention(ctypes.byref(_c_args()), 0, None, 0) == -1
+
+
+def test_calls_without_work_need_no_device():
+    for kind, changes in ((0, dict(l=0)), (0, dict(n=0)), (1, dict(heads=0)), (2, dict(l=0, q_batch=0, kv_batch=0))):
+        assert getattr(_native.lib(), _native.ATTENTION_SYMBOLS[kind])(ctypes.byref(_c_args(**changes)), None) == 0
+
+
+def test_binding_matches_the_compiled_header(tmp_path):
+    text = open(HEADER).read()
+    body = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
+    assert set(re.findall(r"\b(kermac_b200_[a-z0-9_]+)\s*\(", body)) == set(_native.ATTENTION_SYMBOLS)
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "kermac_b200_attention.h"', 'int main(void) {']
+    classes = {"KmHeads": _native.KmHeads, "KmAttentionArgs": _native.KmAttentionArgs}
+    for name, cls in classes.items():
+        lines.append(f'printf("{name} %zu\\n", sizeof({name}));')
+        lines += [f'printf("{name} {f} %zu %zu\\n", offsetof({name}, {f}), sizeof((({name}*)0)->{f}));' for f, _ in cls._fields_]
+    (tmp_path / "layout.c").write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(tmp_path / "layout.c"), "-o",
+                    str(tmp_path / "layout")], check=True)
+    got = [line.split() for line in subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.splitlines()]
+    want = []
+    for name, cls in classes.items():
+        want.append([name, str(ctypes.sizeof(cls))])
+        want += [[name, f, str(getattr(cls, f).offset), str(getattr(cls, f).size)] for f, _ in cls._fields_]
+    assert got == want
+    fields = re.findall(r"typedef struct KmAttentionArgs \{(.*?)\}", body, flags=re.S)[0]
+    declared = [n.replace("*", "").split()[-1] for part in fields.split(";") if part.strip() for n in part.split(",")]
+    assert declared == [f for f, _ in _native.KmAttentionArgs._fields_]
+
+
+def _t(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def _called(monkeypatch):
+    monkeypatch.setattr(attention, "_is_cuda", lambda t: True)
+
+    def launched(*args):
+        raise AssertionError("the call was not refused")
+    monkeypatch.setattr(attention, "_launch", launched)
+
+
+def test_tensors_must_be_on_a_cuda_device():
+    with pytest.raises(ValueError, match="CUDA device"):
+        kermac.cross_attention(_t(2, 1, 8), _t(3, 1, 8), _t(3, 1, 8))
+    with pytest.raises(TypeError, match="q must be a PyTorch tensor"):
+        kermac.prefix_attention([1.0], _t(3, 1, 8), _t(3, 1, 8), _t(3, 1, 8), _t(3, 1, 8))
+
+
+Q, K = (2, 3, 4, 8), (2, 5, 2, 8)
+BAD_CROSS = [
+    (dict(q=_t(3, 8)), ValueError, "dimensions"),
+    (dict(q=_t(*Q, dtype=torch.float64)), TypeError, "dtype"),
+    (dict(k=_t(*K, dtype=torch.bfloat16)), TypeError, "dtype"),
+    (dict(v=None), TypeError, "v must be"),
+    (dict(q=_t(2, 3, 8, 4).transpose(2, 3)), ValueError, "stride 1"),
+    (dict(k=_t(2, 5, 2, 9)), ValueError, "channels"),
+    (dict(q=_t(2, 3, 4, 300), k=_t(2, 5, 2, 300), v=_t(2, 5, 2, 300)), ValueError, r"\[1, 256\]"),
+    (dict(v=_t(2, 6, 2, 8)), ValueError, "shape of k"),
+    (dict(k=_t(2, 5, 3, 8), v=_t(2, 5, 3, 8)), ValueError, "multiple"),
+    (dict(k=_t(2, 5, 0, 8), v=_t(2, 5, 0, 8)), ValueError, "multiple"),
+    (dict(k=_t(3, 5, 2, 8), v=_t(3, 5, 2, 8)), ValueError, "batch size"),
+    (dict(v=_t(1, 5, 2, 8).expand(2, 5, 2, 8)), ValueError, "both be broadcast"),
+    (dict(lengths=[5, 5]), TypeError, "lengths"),
+    (dict(lengths=_t(2)), TypeError, "int32"),
+    (dict(lengths=_t(3, dtype=torch.int32)), ValueError, "lengths must have shape"),
+    (dict(lengths=_t(2, 1, dtype=torch.int32)), ValueError, "lengths must have shape"),
+    (dict(scale=-1.0), ValueError, "scale"),
+    (dict(scale=math.nan), ValueError, "scale"),
+    (dict(out=_t(2, 3, 4, 9)), ValueError, "out must have shape"),
+    (dict(out=_t(3, 4, 8)), ValueError, "dimensions"),
+    (dict(out=_t(*Q, dtype=torch.float16)), TypeError, "dtype"),
+    (dict(lse=_t(2, 3, 4)), ValueError, "lse must have shape"),
+    (dict(lse=_t(2, 4, 3, dtype=torch.float16)), TypeError, "lse must have dtype"),
+    (dict(lse=_t(2, 3, 4).transpose(1, 2)), ValueError, "stride 1"),
+]
+
+
+@pytest.mark.parametrize("changes, error, match", BAD_CROSS, ids=lambda x: None if not isinstance(x, dict) else "-".join(x))
+def test_cross_attention_refuses(changes, error, match, monkeypatch):
+    _called(monkeypatch)
+    given = dict(dict(q=_t(*Q), k=_t(*K), v=_t(*K)), **changes)
+    with pytest.raises(error, match=match):
+        kermac.cross_attention(given.pop("q"), given.pop("k"), given.pop("v"), **given)
+
+
+BAD_PREFIX = [
+    (dict(k_prefix=_t(1, 6, 2, 8)), ValueError, "dimensions"),
+    (dict(k_prefix=_t(6, 2, 9)), ValueError, "k_prefix must have shape"),
+    (dict(v_prefix=_t(6, 4, 8)), ValueError, "v_prefix must have shape"),
+    (dict(v_prefix=_t(7, 2, 8)), ValueError, "shape of k_prefix"),
+    (dict(v_prefix=_t(6, 2, 8, dtype=torch.float16)), TypeError, "dtype"),
+]
+
+
+@pytest.mark.parametrize("changes, error, match", BAD_PREFIX, ids=lambda x: None if not isinstance(x, dict) else "-".join(x))
+def test_prefix_attention_refuses(changes, error, match, monkeypatch):
+    _called(monkeypatch)
+    given = dict(dict(q=_t(*Q), k_prefix=_t(6, 2, 8), v_prefix=_t(6, 2, 8), k=_t(*K), v=_t(*K)), **changes)
+    with pytest.raises(error, match=match):
+        kermac.prefix_attention(**given)
+
+
+BAD_GRAD = [
+    (dict(out=_t(3, 4, 8)), ValueError, "dimensions"),
+    (dict(out=_t(2, 3, 4, 9)), ValueError, "out must have shape"),
+    (dict(grad_out=_t(1, 3, 4, 8)), ValueError, "grad_out must have shape"),
+    (dict(grad_out=_t(*Q, dtype=torch.bfloat16)), TypeError, "dtype"),
+    (dict(lse=_t(2, 3, 4)), ValueError, "lse must have shape"),
+    (dict(lse=None), TypeError, "lse"),
+    (dict(grad_q=_t(1, 3, 4, 8)), ValueError, "grad_q must have shape"),
+    (dict(grad_k=_t(5, 2, 8)), ValueError, "dimensions"),
+    (dict(grad_v=_t(2, 2, 5, 8)), ValueError, "grad_v must have shape"),
+    (dict(k=_t(1, 5, 2, 8)), ValueError, "shape of k"),
+]
+
+
+@pytest.mark.parametrize("changes, error, match", BAD_GRAD, ids=lambda x: None if not isinstance(x, dict) else "-".join(x))
+def test_cross_attention_grad_refuses(changes, error, match, monkeypatch):
+    _called(monkeypatch)
+    given = dict(dict(q=_t(*Q), k=_t(*K), v=_t(*K), out=_t(*Q), lse=_t(2, 4, 3), grad_out=_t(*Q)), **changes)
+    with pytest.raises(error, match=match):
+        kermac.cross_attention_grad(**given)
+
+
+def test_the_reference_name_serves_them():
+    import kermac as served
+    for name in ("cross_attention", "cross_attention_grad", "prefix_attention"):
+        assert getattr(served, name) is getattr(kermac, name)
+
+
+def _attention_kernels():
+    """(name, parameters, body) of the kernels under csrc/attention."""
+    for path in sorted(glob.glob(os.path.join(ROOT, "kermac_b200", "csrc", "attention", "*.cu*"))):
+        text = re.sub(r"//[^\n]*|/\*.*?\*/", "", open(path).read(), flags=re.S)
+        for head in re.finditer(r"__global__\s+void(?:\s+__launch_bounds__\((?:[^()]|\([^()]*\))*\))?\s+(\w+)\s*\(([^)]*)\)\s*\{", text):
+            depth, end = 1, head.end()
+            while depth:
+                depth += {"{": 1, "}": -1}.get(text[end], 0)
+                end += 1
+            yield head.group(1), head.group(2), text[head.end():end]
+
+
+def test_kernels_keep_the_order_of_overlapped_launches():
+    kernels = list(_attention_kernels())
+    assert len(kernels) >= 6
+    for name, parameters, body in kernels:
+        before, wait, _ = body.partition("after_previous_grid();")
+        assert wait and "return;" not in before and "tmem_alloc" not in before, name
+        assert "__restrict__" not in parameters + body and "__ldg" not in body, name

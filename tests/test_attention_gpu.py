@@ -1,0 +1,396 @@
+"""cross_attention, its gradient and prefix_attention on the GPU, each value against the 64-bit oracle and the bound that the
+oracle derives for it."""
+import itertools
+import math
+
+import pytest
+import torch
+
+import kermac_b200 as kermac
+from kermac_b200 import _native
+from oracle import attention_oracle as ao
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def make(seed, *shape, dtype, by=1.0, layout="nhd"):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(*shape, generator=g) * by).to(dtype)
+    if layout == "hnd":                                     # heads first in memory
+        return x.cuda().transpose(-3, -2).contiguous().transpose(-3, -2)
+    if layout == "odd":                                     # rows that start on no 16-byte boundary
+        wide = torch.zeros(*shape[:-1], shape[-1] + 3, dtype=dtype, device="cuda")
+        wide[..., 1:-2] = x.cuda()
+        return wide[..., 1:-2]
+    return x.cuda()
+
+
+def spoil(t, lengths):
+    """NaN and infinities behind each length."""
+    if lengths is not None and t.shape[0] == len(lengths):
+        for l, n in enumerate(lengths):
+            n = max(0, min(t.shape[1], n))
+            t[l, n::2] = math.nan
+            t[l, n + 1::2] = math.inf
+    return t
+
+
+def assert_within(got, want, bound, what):
+    got = got.cpu().double()
+    assert got.shape == want.shape, what
+    same = (got == want) | (torch.isnan(got) & torch.isnan(want))
+    off = torch.where(same, torch.zeros_like(got), (got - want).abs())
+    worst = (off / bound.clamp_min(2.0 ** -149)).max() if off.numel() else torch.zeros(())
+    assert not torch.isnan(off).any() and worst <= 1.0, f"{what}: {float(worst):.3g} of the bound"
+
+
+def check_forward(dtype, L, N, M, H, Hk, D, lengths, layout="nhd", scale=None, by=1.0):
+    q = make(1, L, N, H, D, dtype=dtype, by=by, layout=layout)
+    k, v = (spoil(make(s, L, M, Hk, D, dtype=dtype, layout=layout), lengths) for s in (2, 3))
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out, lse = kermac.cross_attention(q, k, v, lengths=lens, scale=scale, return_lse=True)
+    want, want_lse, bound, lse_bound = ao.attention(q, k, v, lengths, scale)
+    assert_within(out, want, bound, "out")
+    assert_within(lse, want_lse, lse_bound, "lse")
+    assert _native.device_error_flag() == 0
+
+
+SHAPES = [          # L, N, M, H, Hk, lengths
+    (1, 1, 1, 1, 1, None),
+    (2, 1, 700, 4, 4, [700, 333]),
+    (3, 2, 129, 8, 1, [0, 129, 64]),
+    (2, 17, 40, 6, 2, [39, 1]),
+    (1, 130, 257, 2, 2, None),
+    (2, 200, 300, 4, 1, [256, 300]),
+    (2, 65, 128, 3, 3, [-5, 1000]),
+    (1, 300, 1, 2, 1, None),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("D", [64, 128])
+def test_forward(dtype, shape, D):
+    L, N, M, H, Hk, lengths = shape
+    check_forward(dtype, L, N, M, H, Hk, D, lengths)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("D", [1, 2, 7, 8, 40, 72, 80, 96, 100, 112, 136, 200, 250, 256])
+@pytest.mark.parametrize("N", [1, 140])
+def test_forward_widths(dtype, D, N):
+    check_forward(dtype, 2, N, 150, 4, 2, D, [150, 77])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("layout", ["hnd", "odd"])
+@pytest.mark.parametrize("N, D", [(1, 64), (9, 40), (150, 64), (260, 128)])
+def test_forward_layouts(dtype, layout, N, D):
+    check_forward(dtype, 2, N, 200, 4, 2, D, [200, 131], layout=layout)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("N, M", [(1, 20000), (16, 9001), (128, 4000)])
+def test_split_keys(dtype, N, M):
+    # few blocks and many keys: the keys are divided, some pieces of the shorter entry are empty
+    check_forward(dtype, 2, N, M, 2, 1, 64, [M, 40])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("N", [1, 256])
+@pytest.mark.parametrize("scale, by", [(0.0, 1.0), (3.0, 2.0), (0.125, 30.0)])
+def test_scales(dtype, N, scale, by):
+    # weights that are all equal, and weights that are almost all zero
+    check_forward(dtype, 1, N, 300, 2, 2, 64, None, scale=scale, by=by)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("N", [1, 140])
+def test_rising_scores(dtype, N):
+    # keys in the order of their scores: the running maximum rises with every tile, far beyond any fixed margin
+    q = torch.ones(1, N, 1, 64, device="cuda").to(dtype)
+    k = (torch.linspace(-40, 40, 1000, device="cuda")[None, :, None, None] / 8).expand(1, 1000, 1, 64).to(dtype).contiguous()
+    v = make(3, 1, 1000, 1, 64, dtype=dtype)
+    out, lse = kermac.cross_attention(q, k, v, scale=1.0, return_lse=True)
+    want, want_lse, bound, lse_bound = ao.attention(q, k, v, scale=1.0)
+    assert_within(out, want, bound, "out")
+    assert_within(lse, want_lse, lse_bound, "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("N", [1, 150])
+def test_shared_states_and_shared_queries(dtype, N):
+    L, M, H, Hk, D = 3, 170, 4, 2, 64
+    q, q1 = make(1, L, N, H, D, dtype=dtype), make(4, N, H, D, dtype=dtype)
+    k, v = make(2, M, Hk, D, dtype=dtype), make(3, M, Hk, D, dtype=dtype)
+    lengths = torch.tensor([100, 0, 170], dtype=torch.int32, device="cuda")
+    want, _, bound, _ = ao.attention(q, k[None], v[None])
+    assert_within(kermac.cross_attention(q, k, v), want, bound, "shared states")
+    assert_within(kermac.cross_attention(q, k.expand(L, M, Hk, D), v.expand(L, M, Hk, D)), want, bound, "expanded states")
+    want, _, bound, _ = ao.attention(q, k[None], v[None], lengths)
+    assert_within(kermac.cross_attention(q, k, v, lengths=lengths), want, bound, "shared states, lengths")
+    kk, vv = make(5, L, M, Hk, D, dtype=dtype), make(6, L, M, Hk, D, dtype=dtype)
+    want, _, bound, _ = ao.attention(q1[None], kk, vv, lengths)
+    assert_within(kermac.cross_attention(q1, kk, vv, lengths=lengths), want, bound, "shared queries")
+
+
+PREFIXES = [        # L, N, M, P, H, Hk, lengths
+    (1, 1, 1, 1, 1, 1, None),
+    (4, 1, 64, 500, 8, 8, [1, 64, 13, 40]),
+    (3, 5, 90, 300, 8, 2, [5, 90, 47]),
+    (2, 3, 20, 0, 2, 1, [2, 20]),              # no prefix; one query before the first key
+    (2, 3, 20, 40, 2, 1, [0, 1]),              # fewer keys than queries: the prefix alone
+    (3, 2, 0, 129, 4, 4, None),                # no own keys
+    (40, 1, 30, 700, 4, 2, None),
+    (2, 70, 300, 260, 4, 4, [70, 290]),        # a chunk of a prompt
+    (2, 1, 9000, 9000, 2, 1, [9000, 3]),
+    (1, 2, 0, 0, 2, 1, None),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", PREFIXES, ids=str)
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_prefix(dtype, shape, D):
+    L, N, M, P, H, Hk, lengths = shape
+    q = make(1, L, N, H, D, dtype=dtype)
+    k, v = (spoil(make(s, L, M, Hk, D, dtype=dtype), lengths) for s in (2, 3))
+    kp, vp = make(4, P, Hk, D, dtype=dtype), make(5, P, Hk, D, dtype=dtype)
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out, lse = kermac.prefix_attention(q, kp, vp, k, v, lengths=lens, return_lse=True)
+    want, want_lse, bound, lse_bound = ao.attention(q, k, v, lengths, prefix=(kp, vp))
+    assert_within(out, want, bound, "out")
+    assert_within(lse, want_lse, lse_bound, "lse")
+    assert _native.device_error_flag() == 0
+
+
+def check_grad(dtype, q, k, v, lengths, L, g_by=0.5, layout="nhd", scale=None):
+    N, H, D = q.shape[-3:]
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out, lse = kermac.cross_attention(q, k, v, lengths=lens, scale=scale, return_lse=True)
+    g = make(9, L, N, H, D, dtype=dtype, by=g_by, layout=layout)
+    grads = kermac.cross_attention_grad(q, k, v, out, lse, g, lengths=lens, scale=scale)
+    four = [t if t.dim() == 4 else t[None] for t in (q, k, v)]
+    want = ao.attention_grad(*four, g, lengths, scale)
+    for name, got in zip(("grad_q", "grad_k", "grad_v"), grads):
+        assert_within(got, *want[name], name)
+    assert _native.device_error_flag() == 0
+
+
+GRAD_SHAPES = SHAPES + [(1, 700, 40, 4, 2, None), (2, 300, 520, 2, 1, [520, 200])]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", GRAD_SHAPES, ids=str)
+@pytest.mark.parametrize("D", [64, 128])
+def test_grad(dtype, shape, D):
+    L, N, M, H, Hk, lengths = shape
+    q = make(1, L, N, H, D, dtype=dtype)
+    k, v = (spoil(make(s, L, M, Hk, D, dtype=dtype), lengths) for s in (2, 3))
+    check_grad(dtype, q, k, v, lengths, L)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("D", [1, 7, 40, 80, 100, 200, 256])
+@pytest.mark.parametrize("layout", ["nhd", "hnd", "odd"])
+def test_grad_widths_and_layouts(dtype, D, layout):
+    L, N, M, H, Hk, lengths = 2, 70, 150, 4, 2, [150, 77]
+    q, k, v = (make(s, L, n, h, D, dtype=dtype, layout=layout) for s, n, h in ((1, N, H), (2, M, Hk), (3, M, Hk)))
+    check_grad(dtype, q, spoil(k, lengths), spoil(v, lengths), lengths, L, layout=layout)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("N, M", [(20, 140), (150, 300)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_grad_of_broadcast_inputs(dtype, N, M, D):
+    L, H, Hk = 3, 4, 2
+    lengths = [M, 0, M // 3]
+    q, q1 = make(1, L, N, H, D, dtype=dtype), make(4, N, H, D, dtype=dtype)
+    k, v = make(2, L, M, Hk, D, dtype=dtype), make(3, L, M, Hk, D, dtype=dtype)
+    k1, v1 = make(5, M, Hk, D, dtype=dtype), make(6, M, Hk, D, dtype=dtype)
+    check_grad(dtype, q1, k, v, lengths, L)
+    check_grad(dtype, q, k1[None], v1[None], None, L)
+    check_grad(dtype, q, k1, v1, lengths, L)
+    check_grad(dtype, q1, k1, v1, lengths, L)
+
+
+@pytest.mark.parametrize("N, M", [(40, 90), (256, 2000)])
+@pytest.mark.parametrize("by", [1e-4, 300.0])
+def test_float16_gradients_keep_their_range(N, M, by):
+    # weights of 1/2000 times gradients of 1e-4 lie below the smallest float16
+    q, k, v = (make(s, 1, n, 2, 64, dtype=torch.float16) for s, n in ((1, N), (2, M), (3, M)))
+    check_grad(torch.float16, q, k, v, None, 1, g_by=by, scale=0.02)
+
+
+def test_gradient_against_differences():
+    # float32, so that a difference of the result has some digits: 1e-2 steps, error of the difference about 1e-4
+    L, N, M, H, Hk, D = 1, 6, 9, 2, 1, 8
+    q, k, v = (make(s, L, n, h, D, dtype=torch.float32) for s, n, h in ((1, N, H), (2, M, Hk), (3, M, Hk)))
+    g = make(9, L, N, H, D, dtype=torch.float32)
+    out, lse = kermac.cross_attention(q, k, v, return_lse=True)
+    grads = kermac.cross_attention_grad(q, k, v, out, lse, g)
+
+    def loss(*x):
+        return float((kermac.cross_attention(*x).double() * g.double()).sum())
+
+    step = 1e-2
+    for which, grad in enumerate(grads):
+        for at in itertools.islice(range(0, grad.numel(), 7), 12):
+            x = [t.clone() for t in (q, k, v)]
+            x[which].view(-1)[at] += step
+            up = loss(*x)
+            x[which].view(-1)[at] -= 2 * step
+            difference = (up - loss(*x)) / (2 * step)
+            # third derivatives of the softmax times step^2, and 2^-20 of a loss of about 10 over the step
+            assert abs(difference - float(grad.view(-1)[at])) < 5e-3
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_equal_calls_give_equal_bits(dtype):
+    L, N, M, H, Hk, D = 2, 200, 3000, 4, 2, 64
+    q, k, v = (make(s, L, n, h, D, dtype=dtype) for s, n, h in ((1, N, H), (2, M, Hk), (3, M, Hk)))
+    g = make(9, L, N, H, D, dtype=dtype)
+    first = None
+    for _ in range(3):
+        out, lse = kermac.cross_attention(q, k, v, return_lse=True)
+        now = (out, lse, *kermac.cross_attention_grad(q, k, v, out, lse, g), kermac.prefix_attention(q, k[0], v[0], k, v))
+        first = first or now
+        assert all(torch.equal(a, b) for a, b in zip(first, now))
+
+
+def test_destinations_and_rows_that_are_not_there():
+    L, N, M, H, Hk, D = 2, 5, 60, 4, 2, 64
+    q, k, v = (make(s, L, n, h, D, dtype=torch.bfloat16) for s, n, h in ((1, N, H), (2, M, Hk), (3, M, Hk)))
+    lengths = torch.tensor([60, 11], dtype=torch.int32, device="cuda")
+    big = torch.full((L, N + 2, H + 1, D + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = big[:, 1:-1, 1:, 4:-4]                                  # rows on 8-byte boundaries
+    lse = torch.full((L, H, N + 3), 7.0, device="cuda")[..., :N]
+    got, got_lse = kermac.cross_attention(q, k, v, lengths=lengths, out=out, lse=lse, return_lse=True)
+    assert got is out and got_lse is lse
+    want, want_lse = kermac.cross_attention(q, k, v, lengths=lengths, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    kept = big.clone()
+    kept[:, 1:-1, 1:, 4:-4] = 7.0
+    assert torch.all(kept == 7.0)                                 # nothing beside the view was written
+    g = make(9, L, N, H, D, dtype=torch.bfloat16)
+    plain = kermac.cross_attention_grad(q, k, v, want, want_lse, g, lengths=lengths)
+    into = [torch.full((L, n, h + 1, D + 2), 7.0, dtype=torch.bfloat16, device="cuda") for n, h in ((N, H), (M, Hk), (M, Hk))]
+    views = [t[:, :, :-1, 1:-1] for t in into]
+    given = kermac.cross_attention_grad(q, k, v, out, lse, g, lengths=lengths, grad_q=views[0], grad_k=views[1], grad_v=views[2])
+    for a, b, view, whole in zip(plain, given, views, into):
+        assert b is view and torch.equal(a, b)
+        assert torch.all(whole[:, :, -1] == 7.0) and torch.all(whole[..., 0] == 7.0) and torch.all(whole[..., -1] == 7.0)
+    assert torch.all(plain[1][1, 11:] == 0) and torch.all(plain[2][1, 11:] == 0)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_empty_extents(dtype):
+    def t(*shape):
+        return torch.zeros(*shape, dtype=dtype, device="cuda")
+    assert kermac.cross_attention(t(0, 3, 2, 8), t(0, 4, 2, 8), t(0, 4, 2, 8)).shape == (0, 3, 2, 8)
+    assert kermac.cross_attention(t(2, 0, 2, 8), t(2, 4, 2, 8), t(2, 4, 2, 8)).shape == (2, 0, 2, 8)
+    q, k = t(2, 3, 2, 8) + 1, t(2, 0, 2, 8)
+    out, lse = kermac.cross_attention(q, k, k, return_lse=True)
+    assert torch.all(out == 0) and torch.all(lse == -math.inf)
+    grads = kermac.cross_attention_grad(q, k, k, out, lse, q)
+    assert torch.all(grads[0] == 0) and grads[1].shape == k.shape and grads[2].shape == k.shape
+    none, k = t(2, 0, 2, 8), t(2, 3, 2, 8) + 1
+    out, lse = kermac.cross_attention(none, k, k, return_lse=True)
+    grads = kermac.cross_attention_grad(none, k, k, out, lse, none)
+    assert torch.all(grads[1] == 0) and torch.all(grads[2] == 0) and grads[0].shape == none.shape
+
+
+@pytest.mark.parametrize("N", [1, 200])
+def test_streams_and_graphs(N):
+    L, M, H, Hk, D, P = 2, 2000, 4, 2, 64, 600
+    q, k, v = (make(s, L, n, h, D, dtype=torch.bfloat16) for s, n, h in ((1, N, H), (2, M, Hk), (3, M, Hk)))
+    g, kp, vp = make(9, L, N, H, D, dtype=torch.bfloat16), make(4, P, Hk, D, dtype=torch.bfloat16), make(5, P, Hk, D, dtype=torch.bfloat16)
+
+    def step():
+        out, lse = kermac.cross_attention(q, k, v, return_lse=True)
+        return (out, lse, *kermac.cross_attention_grad(q, k, v, out, lse, g), kermac.prefix_attention(q, kp, vp, k, v))
+
+    want = [t.clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    # two graphs with workspaces of their own, replayed in turn and at the same time
+    graphs, results = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results.append(step())
+        graphs.append(graph)
+    for _ in range(3):
+        for result in results:
+            for t in result:
+                t.fill_(math.nan)
+        torch.cuda.synchronize()
+        side.wait_stream(torch.cuda.current_stream())
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        for result in results:
+            assert all(torch.equal(a, b) for a, b in zip(want, result))
+    # new inputs in the captured buffers
+    q.mul_(0.5)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(step(), results[0]))
+
+
+@pytest.mark.parametrize("N", [1, 200])
+def test_offsets_beyond_32_bits(N):
+    # heads 2^31 elements apart: a cache of 2 * 4.3 GB in which every fourth row of the second head lies behind 2^31
+    M, D = 300, 64
+    if torch.cuda.mem_get_info()[0] < 14 << 30:
+        pytest.skip("needs 14 GB")
+    store = torch.empty((1 << 31) + (1 << 20), dtype=torch.bfloat16, device="cuda")
+    small = make(2, 1, M, 2, D, dtype=torch.bfloat16)
+    k = store.as_strided((1, M, 2, D), (0, D, 1 << 31, 1))
+    k.copy_(small)
+    q = make(1, 1, N, 2, D, dtype=torch.bfloat16)
+    want, _, bound, _ = ao.attention(q, small, small)
+    out, lse = kermac.cross_attention(q, k, k, return_lse=True)
+    assert_within(out, want, bound, "out")
+    grads = kermac.cross_attention_grad(q, k, k, out, lse, q)
+    same = kermac.cross_attention_grad(q, small, small, out, lse, q)
+    assert all(torch.equal(a, b) for a, b in zip(grads, same))
+
+
+def test_a_run_of_them_together():
+    """A decoder layer's step as it is used: training against padded states, then tokens written one by one below a shared
+    prompt, which must see what one pass over the whole sequence sees."""
+    dtype, L, M, H, Hk, D = torch.bfloat16, 3, 90, 8, 2, 64
+    lengths = torch.tensor([90, 41, 7], dtype=torch.int32, device="cuda")
+    states = make(2, L, M, 2, Hk, D, dtype=dtype)                 # projected keys and values side by side
+    k, v = states[:, :, 0], states[:, :, 1]
+    q = make(1, L, 20, H, D, dtype=dtype)
+    out, lse = kermac.cross_attention(q, k, v, lengths=lengths, return_lse=True)
+    grads = kermac.cross_attention_grad(q, k, v, out, lse, out, lengths=lengths)      # of |out|^2 / 2
+    found = ao.attention_grad(q, k, v, out, lengths)
+    for name, got in zip(("grad_q", "grad_k", "grad_v"), grads):
+        assert_within(got, *found[name], name)
+    moved = [(t.float() - 0.1 * d.float()).to(dtype) for t, d in zip((q, k, v), grads)]
+    want, _, bound, _ = ao.attention(*moved, lengths)
+    assert_within(kermac.cross_attention(*moved, lengths=lengths), want, bound, "after a step")
+
+    P, steps = 150, 6
+    kp, vp = make(4, P, Hk, D, dtype=dtype), make(5, P, Hk, D, dtype=dtype)
+    own_k, own_v = (torch.zeros(L, steps, Hk, D, dtype=dtype, device="cuda") for _ in range(2))
+    new_q, new_k, new_v = (make(s, L, steps, h, D, dtype=dtype) for s, h in ((6, H), (7, Hk), (8, Hk)))
+    for t in range(steps):
+        own_k[:, t], own_v[:, t] = new_k[:, t], new_v[:, t]
+        there = torch.full((L,), t + 1, dtype=torch.int32, device="cuda")
+        one = kermac.prefix_attention(new_q[:, t:t + 1], kp, vp, own_k, own_v, lengths=there)
+        whole_k, whole_v = (torch.cat([a.expand(L, P, Hk, D), b[:, :t + 1]], dim=1) for a, b in ((kp, new_k), (vp, new_v)))
+        want, _, bound, _ = ao.attention(new_q[:, t:t + 1], whole_k, whole_v)
+        assert_within(one, want, bound, f"token {t}")
+    many = kermac.prefix_attention(new_q, kp, vp, new_k, new_v)
+    want, _, bound, _ = ao.attention(new_q, new_k, new_v, prefix=(kp, vp))
+    assert_within(many, want, bound, "all tokens at once")
