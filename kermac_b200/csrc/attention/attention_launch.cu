@@ -2,9 +2,23 @@
 #include <algorithm>
 #include <cmath>
 
+#include "../km_build_tma.cuh"
 #include "attention_params.h"
 
 namespace km {
+namespace att {
+int encode_rows(CUtensorMap* map, const Heads& t, int rows, int heads, int L, int D, int type) {
+    // an extent of one may come with any stride; a broadcast batch is one entry
+    const long long dense = (D + 7) & ~7;
+    const cuuint64_t dims[4]    = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(heads),
+                                   static_cast<cuuint64_t>(t.sl == 0 ? 1 : L)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(rows > 1 ? t.sr : dense) * 2, static_cast<cuuint64_t>(heads > 1 ? t.sh : dense) * 2,
+                                   static_cast<cuuint64_t>(dims[3] > 1 ? t.sl : dense) * 2};
+    const cuuint32_t box[4] = {64, 128, 1, 1};
+    return encode_tma_16bit(map, t.ptr, type == ATT_BF16, dims, strides, box);
+}
+}  // namespace att
+
 namespace {
 
 enum Kind { CROSS = 0, PREFIX = 1, GRAD = 2 };
@@ -84,11 +98,28 @@ bool rows_aligned(const KmHeads& t, int type, int d) {
     return aligned16(t.ptr) && t.stride_l % unit == 0 && t.stride_row % unit == 0 && t.stride_head % unit == 0 && d % unit == 0;
 }
 
+// What a TMA copy of 64 x 128 boxes needs beyond that: no stride of zero but the batch's, none beyond its 40 bits.
+bool tma_rows_ok(const KmHeads& t, int rows, int n_heads, int type, int d) {
+    const long long most = 1LL << 38;
+    return type != ATT_F32 && rows_aligned(t, type, d) && (rows <= 1 || (t.stride_row > 0 && t.stride_row < most)) &&
+           (n_heads <= 1 || (t.stride_head > 0 && t.stride_head < most)) && t.stride_l < most;
+}
+
+// The kernels of the forward pass: 16 rows whose keys four warps share out, 64 rows on mma.sync, 256 on tcgen05.
+enum Form { FEW, ROWS, TENSOR };
+const char* const FORM_NAMES[] = {"few", "rows", "tensor"};
+const int FORM_ROWS[] = {ATT_FEW_ROWS, ATT_TILE_ROWS, ATT_TENSOR_ROWS};
+
 struct Plan {
-    bool few_own, few_prefix;
+    Form own, prefix;
     AttentionParams p;
     long long bytes;
 };
+
+Form choose_form(long long rows, bool tensor_ok) {
+    if (rows <= ATT_FEW_ROWS) return FEW;
+    return tensor_ok && rows > ATT_TILE_ROWS ? TENSOR : ROWS;
+}
 
 // How many pieces the keys of `blocks` blocks are split into: enough to give every SM `per_sm` blocks, no piece shorter than
 // `least` keys.
@@ -105,7 +136,8 @@ Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool scratch) {
     p.q = heads(a.q), p.k = heads(a.k), p.v = heads(a.v), p.out = heads(a.out), p.kp = heads(a.k_prefix), p.vp = heads(a.v_prefix);
     p.lengths = a.lengths, p.lengths_stride = a.lengths_stride;
     p.lse = a.lse, p.lse_sl = a.lse_stride_l, p.lse_sh = a.lse_stride_head;
-    p.scale_log2 = a.scale * 1.4426950408889634f;
+    // a scale of 0 becomes 2^-100: the same weights, and the -inf of a masked score stays -inf
+    p.scale_log2 = std::max(a.scale * 1.4426950408889634f, 0x1p-100f);
     p.causal = kind == PREFIX;
     // Keys that a whole batch shares are a prefix without own keys.
     if (kind == CROSS && a.l > 1 && a.k.stride_l == 0 && !a.lengths && a.m > 0) {
@@ -116,16 +148,25 @@ Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool scratch) {
         const KmHeads &k = kind == PREFIX ? a.k_prefix : a.k, &v = kind == PREFIX ? a.v_prefix : a.v;
         p.vec = p.vec && rows_aligned(k, a.type, a.d) && rows_aligned(v, a.type, a.d);
     }
+    const bool narrow = a.type != ATT_F32 && a.d <= 128 && p.vec;
+    const bool own_ok = narrow && tma_rows_ok(a.k, a.m, a.key_heads, a.type, a.d) && tma_rows_ok(a.v, a.m, a.key_heads, a.type, a.d);
+    const bool prefix_ok = kind == PREFIX ? narrow && tma_rows_ok(a.k_prefix, a.prefix, a.key_heads, a.type, a.d) &&
+                                                tma_rows_ok(a.v_prefix, a.prefix, a.key_heads, a.type, a.d)
+                                          : own_ok;
+    p.vec_out = rows_aligned(a.out, a.type, a.d);
     const long long own_rows = static_cast<long long>(p.N) * p.G, prefix_rows = own_rows * p.L;
-    plan.few_own    = own_rows <= ATT_FEW_ROWS;
-    plan.few_prefix = prefix_rows <= ATT_FEW_ROWS;
+    plan.own    = choose_form(own_rows, own_ok);
+    plan.prefix = choose_form(prefix_rows, prefix_ok);
+    auto split = [&](Form form, long long blocks, int keys) {
+        return scratch ? pieces(blocks, keys, form == TENSOR ? 1 : 2, form == FEW ? 256 : 512) : 1;
+    };
     if (p.M > 0 || p.P == 0) {
-        p.own_tiles  = static_cast<int>(ceil_div_ll(own_rows, plan.few_own ? ATT_FEW_ROWS : ATT_TILE_ROWS));
-        p.own_splits = scratch ? pieces(static_cast<long long>(p.own_tiles) * p.L * p.Hk, p.M, 2, plan.few_own ? 256 : 512) : 1;
+        p.own_tiles  = static_cast<int>(ceil_div_ll(own_rows, FORM_ROWS[plan.own]));
+        p.own_splits = split(plan.own, static_cast<long long>(p.own_tiles) * p.L * p.Hk, p.M);
     }
     if (p.P > 0) {
-        p.prefix_tiles  = static_cast<int>(ceil_div_ll(prefix_rows, plan.few_prefix ? ATT_FEW_ROWS : ATT_TILE_ROWS));
-        p.prefix_splits = scratch ? pieces(static_cast<long long>(p.prefix_tiles) * p.Hk, p.P, 2, plan.few_prefix ? 256 : 512) : 1;
+        p.prefix_tiles  = static_cast<int>(ceil_div_ll(prefix_rows, FORM_ROWS[plan.prefix]));
+        p.prefix_splits = split(plan.prefix, static_cast<long long>(p.prefix_tiles) * p.Hk, p.P);
     }
     p.parts = p.own_splits + p.prefix_splits;
     if (p.parts > 1) plan.bytes = static_cast<long long>(p.parts) * p.L * p.N * p.H * (p.D + 1) * 4;
@@ -162,15 +203,18 @@ int forward(const KmAttentionArgs* a, Kind kind, void* stream) {
         plan.p.part_o   = static_cast<float*>(a->scratch);
         plan.p.part_lse = plan.p.part_o + static_cast<long long>(plan.p.parts) * plan.p.L * plan.p.N * plan.p.H * plan.p.D;
     }
+    auto launch = [&](const AttentionParams& p, Form form) {
+        return form == TENSOR ? attention_tensor_launch(p, a->type, st) : attention_rows_launch(p, a->type, form == FEW, st);
+    };
     const bool own = plan.p.own_splits > 0, prefix = plan.p.prefix_splits > 0;
-    if (own && prefix && plan.few_own != plan.few_prefix) {
+    if (own && prefix && plan.own != plan.prefix) {
         AttentionParams p = plan.p;
         p.own_tiles = 0;                                   // the blocks of the prefix alone
-        rc = attention_rows_launch(p, a->type, plan.few_prefix, st);
+        rc = launch(p, plan.prefix);
         p = plan.p, p.prefix_tiles = 0;
-        if (!rc) rc = attention_rows_launch(p, a->type, plan.few_own, st);
+        if (!rc) rc = launch(p, plan.own);
     } else {
-        rc = attention_rows_launch(plan.p, a->type, own ? plan.few_own : plan.few_prefix, st);
+        rc = launch(plan.p, own ? plan.own : plan.prefix);
     }
     if (!rc && plan.p.parts > 1) rc = attention_join_launch(plan.p, a->type, st);
     return rc;
@@ -272,8 +316,8 @@ int kermac_b200_describe_attention(const KmAttentionArgs* args, int32_t kind, ch
         snprintf(buf, buf_len, "grad=rows q_slices=%d kv_slices=%d scratch=%lld", plan.p.q_slices, plan.p.kv_slices, plan.bytes());
     } else {
         const Plan plan = plan_within(*args, static_cast<Kind>(kind), MOST_SCRATCH);
-        snprintf(buf, buf_len, "own=%s tiles=%d splits=%d prefix=%s tiles=%d splits=%d scratch=%lld", plan.few_own ? "few" : "rows",
-                 plan.p.own_tiles, plan.p.own_splits, plan.few_prefix ? "few" : "rows", plan.p.prefix_tiles, plan.p.prefix_splits,
+        snprintf(buf, buf_len, "own=%s tiles=%d splits=%d prefix=%s tiles=%d splits=%d scratch=%lld", FORM_NAMES[plan.own],
+                 plan.p.own_tiles, plan.p.own_splits, FORM_NAMES[plan.prefix], plan.p.prefix_tiles, plan.p.prefix_splits,
                  plan.bytes);
     }
     return 0;

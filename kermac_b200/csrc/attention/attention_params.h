@@ -60,6 +60,10 @@ enum { ATT_F32 = KM_TYPE_FLOAT32, ATT_BF16 = KM_TYPE_BFLOAT16, ATT_F16 = KM_TYPE
 int  attention_rows_launch(const AttentionParams& p, int type, bool few, cudaStream_t st);
 constexpr int ATT_FEW_ROWS = 16, ATT_TILE_ROWS = 64;
 int  attention_join_launch(const AttentionParams& p, int type, cudaStream_t st);
+// attention_tensor.cu (tcgen05): 16-bit types, D a multiple of 8 up to 128, rows that TMA can copy.
+constexpr int ATT_TENSOR_ROWS = 256;
+int  attention_tensor_launch(const AttentionParams& p, int type, cudaStream_t st);
+int  attention_tensor_take_wait_flag();
 // attention_grad_rows.cu
 constexpr int ATT_GRAD_ROWS = 64, ATT_PEAK_ROWS = 64;
 int  attention_delta_launch(const AttentionGradParams& p, int type, cudaStream_t st);

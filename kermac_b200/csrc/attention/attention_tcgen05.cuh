@@ -1,0 +1,105 @@
+// Pieces that the tensor-core attention kernels share: operand descriptors, 16-bit tcgen05.mma, tensor-memory reads and writes,
+// and the shared-memory layout of a tile.
+//
+// A tile of 128 rows is held as slabs of 64 channels: row r of a slab is 128 bytes, its 16-byte chunk c at position c ^ (r % 8),
+// which is what a TMA copy with the 128-byte swizzle writes.  One copy of a tile serves both kinds of product: as a K-major operand
+// (contraction over channels) and, through the transpose bit of the instruction, as an MN-major one (contraction over rows).
+#pragma once
+
+#include "../km_mbar.cuh"
+#include "../km_tcgen05.cuh"
+#include "attention_work.cuh"
+
+namespace km {
+namespace att {
+
+constexpr int TC_ROWS = 128, TC_SLAB = TC_ROWS * 128;
+
+// Instruction descriptor: fp32 sums (1 in bits [4,6)), both operands float16 (0) or bfloat16 (1) in [7,10) and [10,13), B MN-major
+// in bit 16, N / 8 in [17,23), M / 16 in [24,29).
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t instr_desc(int n, bool b_rows) {
+    const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return (1u << 4) | (f << 7) | (f << 10) | (b_rows ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+// 16 channels of a tile as a K-major operand, from channel 16 * k on.
+__device__ __forceinline__ uint64_t desc_channels(uint32_t tile, int k) {
+    return tc::smem_desc_k_major_sw128(tile + (k >> 2) * TC_SLAB + (k & 3) * 32);
+}
+// 16 rows of a tile as an MN-major operand, from row 16 * k on: 64-channel blocks TC_SLAB apart (leading offset), groups of
+// eight rows 1024 bytes apart (stride offset).
+__device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int k) {
+    return static_cast<uint64_t>(((tile + k * 2048) & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(TC_SLAB >> 4) << 16) | (64ull << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+
+// D (+)= A B, A and B in shared memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+        : "memory");
+}
+// The same with A in tensor memory, two of its columns in one of 32 bits.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    tc::mma_bf16_a_tmem(d, a, b, idesc, accumulate);
+}
+
+// One row (lane) of 32 columns.  The values may be used behind wait_loaded() of the same registers.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+        "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Ties 32 registers to the wait before it, so that no use of them moves in front.
+__device__ __forceinline__ void tmem_loaded32(uint32_t* r) {
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]),
+                 "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+        "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+          "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+          "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+// Host: a 16-bit tensor [l][row][head][channel] for copies of boxes of 64 channels x 128 rows; what a box has beyond `rows` or D
+// is filled with zeros.  Needs tma_rows_ok().
+int encode_rows(CUtensorMap* map, const Heads& t, int rows, int heads, int L, int D, int type);
+
+// One box of 64 channels x 128 rows of a [l][head][row][channel] tensor; x is 0 or 64 (16-bit: a multiple of 128 bytes).
+__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, int x, int row, int head, int l, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(head), "r"(l), "r"(bar)
+        : "memory");
+}
+
+// A row of 16-bit channels into a tile by the thread that owns the row; nullptr: zeros.  D is a multiple of 8.
+template <int DP>
+__device__ __forceinline__ void fill_row(char* tile, int r, const char* row, int D) {
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (row != nullptr && c * 8 < D) x = *reinterpret_cast<const uint4*>(row + c * 16);
+        *reinterpret_cast<uint4*>(tile + (c >> 3) * TC_SLAB + r * 128 + ((c & 7) ^ (r & 7)) * 16) = x;
+    }
+}
+
+}  // namespace att
+}  // namespace km

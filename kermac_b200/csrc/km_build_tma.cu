@@ -30,6 +30,8 @@
 
 namespace km {
 
+int attention_tensor_take_wait_flag();     // attention/attention_tensor.cu
+
 __device__ int g_tma_wait_expired = 0;
 
 namespace {
@@ -260,6 +262,18 @@ int encode_tma_operand(CUtensorMap* map, const float* base, int extent, int K, i
                        int box_k) {
     return encode_operand(map, base, extent, K, L, s_k, s_l, box_k);
 }
+int encode_tma_16bit(CUtensorMap* map, const void* base, bool bfloat16, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3],
+                     const cuuint32_t (&box)[4]) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return fail(KM_ERR_INTERNAL, "cuTensorMapEncodeTiled is not available from this driver");
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, bfloat16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
+                          dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(KM_ERR_INTERNAL, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    return 0;
+}
+
 int encode_tma_box(CUtensorMap* map, const float* base, int inner, int outer, int L, long long s_outer, long long s_l,
                    int box_inner, int box_outer, bool swizzle_128b) {
     return encode_box(map, base, inner, outer, L, s_outer, s_l, box_inner, box_outer, swizzle_128b);
@@ -356,6 +370,7 @@ extern "C" int kermac_b200_device_error_flag(void) {
     const int gv = km::grad_tensor_take_wait_flag();
     const int hv = km::grad_sign_take_wait_flag();
     const int sv = km::small_take_wait_flag();
-    if (mv < 0 || gv < 0 || hv < 0 || sv < 0) return KM_ERR_INTERNAL;
-    return (v || mv || gv || hv || sv) ? 1 : 0;
+    const int av = km::attention_tensor_take_wait_flag();
+    if (mv < 0 || gv < 0 || hv < 0 || sv < 0 || av < 0) return KM_ERR_INTERNAL;
+    return (v || mv || gv || hv || sv || av) ? 1 : 0;
 }

@@ -27,6 +27,10 @@ int encode_tma_operand(CUtensorMap* map, const float* base, int extent, int K, i
 // (128 with the 128-byte swizzle, which stores 16-byte chunk c of row r at chunk position c ^ (r % 8)).
 int encode_tma_box(CUtensorMap* map, const float* base, int inner, int outer, int L, long long s_outer, long long s_l,
                    int box_inner, int box_outer, bool swizzle_128b = false);
+// Describes a rank-4 tensor of 16-bit values (extents and box innermost first, strides of the outer three in bytes), its boxes
+// stored with the 128-byte swizzle: box[0] is 64.  Base and strides are multiples of 16 bytes.
+int encode_tma_16bit(CUtensorMap* map, const void* base, bool bfloat16, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3],
+                     const cuuint32_t (&box)[4]);
 // True when an operand with these strides can be described that way.
 bool tma_operand_ok(const float* base, long long s_t, long long s_k, long long s_l, int K, int L);
 
