@@ -4,16 +4,11 @@
 //   dv = p^T dout,   ds = p * (dout v^T - delta),   dk = scale ds^T q,   dq = scale ds k.
 // Two kernels, so that every sum has one owner and a fixed order: one holds 64 keys and streams the queries (dk, dv), one holds 64
 // queries and streams the keys (dq).  The price is that s and dout v^T are computed twice, 7 products instead of 5.
-#include "attention_mma.cuh"
+#include "attention_grad.cuh"
 
 namespace km {
 namespace att {
 namespace {
-
-// float16 weights are multiplied by this before they are rounded: they are at most 1, and float16 ends at 6e-8.
-constexpr float F16_WEIGHT = 256.0f;
-
-template <typename T> constexpr bool is_f16 = std::is_same<T, __half>::value;
 
 template <typename T, int DP>
 struct GradShape {
@@ -25,51 +20,6 @@ struct GradShape {
     static constexpr int STATS  = 2 * 2 * STREAM * 4;                    // two stages of lse and delta
     static constexpr int SMEM   = 2 * HELD + 2 * 2 * MOVED + STATS;
 };
-
-// 2^-e with 2^e the power of two at or below the largest of the given peaks; 1 when they are zero, infinite or NaN.
-// Called by the whole block.
-template <typename T>
-__device__ __forceinline__ float find_factor(const AttentionGradParams& p, int l0, int l1, int h0, int h1) {
-    if constexpr (!is_f16<T>) {
-        return 1.0f;
-    } else {
-        __shared__ float of_warp[WARPS];
-        float best = 0.0f;
-        const int per_l = (h1 - h0) * p.peak_count;
-        for (int l = l0; l < l1; ++l)
-            for (int i = threadIdx.x; i < per_l; i += THREADS)
-                best = fmaxf(best, p.peaks[(static_cast<long long>(l) * p.H + h0) * p.peak_count + i]);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
-        if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = best;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < WARPS; ++i) best = fmaxf(best, of_warp[i]);
-        const uint32_t e = __float_as_uint(best) >> 23;                  // best is a float16 magnitude: 2^-24 .. 65504
-        return (best > 0.0f && e < 255) ? __uint_as_float((254u - e) << 23) : 1.0f;
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ const T* head_of(const Heads& t, int l, int h) {
-    return reinterpret_cast<const T*>(t.ptr) + l * t.sl + h * t.sh;
-}
-
-// Channels (c, c + 1) of a gradient: into the tensor, or into a slice's 32-bit sums [l][row][head][D].
-template <typename T>
-__device__ __forceinline__ void put_grad(const Heads& to, float* part, int l, int row, int h, int rows, int heads, int D, int c,
-                                         float x, float y) {
-    if (c >= D) return;
-    if (part) {
-        float* o = part + ((static_cast<long long>(l) * rows + row) * heads + h) * D + c;
-        o[0] = x;
-        if (c + 1 < D) o[1] = y;
-    } else {
-        T* o = reinterpret_cast<T*>(to.ptr) + l * to.sl + row * to.sr + h * to.sh + c;
-        o[0] = Type<T>::to(x);
-        if (c + 1 < D) o[1] = Type<T>::to(y);
-    }
-}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(THREADS) attention_grad_keys_kernel(const AttentionGradParams p) {
@@ -105,7 +55,7 @@ __global__ void __launch_bounds__(THREADS) attention_grad_keys_kernel(const Atte
             longest = n > longest ? n : longest;
         }
     const bool  idle   = key0 >= longest;
-    const float factor = find_factor<T>(p, l_first, l_first + l_count, hk * p.G, hk * p.G + p.G);
+    const float factor = find_factor<T, THREADS>(p, l_first, l_first + l_count, hk * p.G, hk * p.G + p.G);
     const float by     = is_f16<T> ? factor / F16_WEIGHT : 1.0f;
 
     float dk[CT][4], dv[CT][4];
@@ -155,7 +105,7 @@ __global__ void __launch_bounds__(THREADS) attention_grad_keys_kernel(const Atte
                 for (int e = 0; e < 4; ++e) {
                     const int   col  = j * 8 + 2 * t + (e & 1);
                     const bool  seen = key0 + warp * 16 + g + 8 * (e >> 1) < count && n0 + col < p.N;
-                    const float w    = ex2_approx(fmaf(s[j][e], p.scale_log2, (is_f16<T> ? 8.0f : 0.0f) - lse[col] * (1.0f / LN2)));
+                    const float w    = ex2_approx(fmaf(s[j][e], p.scale_log2, (is_f16<T> ? F16_WEIGHT_LOG2 : 0.0f) - lse[col] * (1.0f / LN2)));
                     ds[j][e] = seen ? w * ((ds[j][e] - delta[col]) * by) : 0.0f;
                     s[j][e]  = seen ? w : 0.0f;
                 }
@@ -199,7 +149,7 @@ __global__ void __launch_bounds__(THREADS) attention_grad_queries_kernel(const A
     const int h = block % p.H, l = block / p.H, hk = h / p.G;
     const int   count  = key_count(p.lengths, p.lengths_stride, l, p.M);
     const int   kl     = p.kv_batch == 1 ? 0 : l;
-    const float factor = find_factor<T>(p, l, l + 1, h, h + 1);
+    const float factor = find_factor<T, THREADS>(p, l, l + 1, h, h + 1);
 
     copy_rows<T, DP>(held_q, head_of<T>(p.q, l, h), p.q.sr, n0, p.N, S::ROWS, p.D, p.vec, threadIdx.x, THREADS);
     copy_rows<T, DP>(held_d, head_of<T>(p.dout, l, h), p.dout.sr, n0, p.N, S::ROWS, p.D, p.vec, threadIdx.x, THREADS);
@@ -270,18 +220,33 @@ __global__ void __launch_bounds__(THREADS) attention_delta_kernel(const Attentio
     const int h = block % p.H, l = block / p.H, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const T * out = head_of<T>(p.out, l, h), *dout = head_of<T>(p.dout, l, h);
     float     peak = 0.0f;
-    for (int r = warp; r < ATT_PEAK_ROWS; r += WARPS) {
+    // `lanes` lanes a row, a 16-byte unit each in turn, so a warp takes 32 / lanes rows at a time
+    constexpr int CHUNK = Type<T>::CHUNK;
+    const int units = (p.D + CHUNK - 1) / CHUNK, lanes = units > 16 ? 32 : units > 8 ? 16 : 8, sub = lane & (lanes - 1);
+    for (int r = (warp * 32 + lane) / lanes; r < ATT_PEAK_ROWS; r += THREADS / lanes) {     // uniform: a multiple of lanes rows
         const int n = group * ATT_PEAK_ROWS + r;
-        if (n >= p.N) break;
         float sum = 0.0f;
-        for (int c = lane; c < p.D; c += 32) {
-            const float x = Type<T>::from(dout[n * p.dout.sr + c]);
-            sum  = fmaf(x, Type<T>::from(out[n * p.out.sr + c]), sum);
-            peak = fmaxf(peak, fabsf(x));
-        }
+        for (int u = sub; u < units; u += lanes) {
+            alignas(16) T x[CHUNK], y[CHUNK];
+            if (n < p.N && p.vec_out) {
+                *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(dout + n * p.dout.sr + u * CHUNK);
+                *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(out + n * p.out.sr + u * CHUNK);
+            } else {
 #pragma unroll
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (lane == 0) p.delta[(static_cast<long long>(l) * p.H + h) * p.N + n] = sum;
+                for (int e = 0; e < CHUNK; ++e) {
+                    const bool there = n < p.N && u * CHUNK + e < p.D;
+                    x[e] = there ? dout[n * p.dout.sr + u * CHUNK + e] : Type<T>::to(0.0f);
+                    y[e] = there ? out[n * p.out.sr + u * CHUNK + e] : Type<T>::to(0.0f);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < CHUNK; ++e) {
+                sum  = fmaf(Type<T>::from(x[e]), Type<T>::from(y[e]), sum);
+                peak = fmaxf(peak, fabsf(Type<T>::from(x[e])));
+            }
+        }
+        for (int d = lanes >> 1; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (sub == 0 && n < p.N) p.delta[(static_cast<long long>(l) * p.H + h) * p.N + n] = sum;
     }
     if (p.peaks) {
 #pragma unroll

@@ -1,0 +1,565 @@
+// Gradient of the attention of 16-bit tensors on the tensor cores (tcgen05), head widths up to 128.
+//
+// Two kernels as in attention_grad_rows.cu: a block holds 128 keys and streams query tiles (dk, dv), or holds 128 queries and streams
+// key tiles (dq).  Scores and dout v^T are in tensor memory, the weights and their gradients are written back over them as
+// 16-bit operands.  The keys' kernel computes both transposed, so that its operands need no transposition either: a
+// lane is a key there and a query in the other kernel.
+//
+// Tensor memory has no room for a second set of both products beside the 128-channel sums dk and dv, and needs none: what the tensor
+// cores do is cut in two, and the weights' warps (eight, 64 columns each) work on the other half meanwhile,
+//   tensor cores:  dv(i), s(i + 1)   | dk(i), dp(i + 1)
+//   warps:         ds(i)             | p(i + 1)
+#include <algorithm>
+
+#include "attention_grad.cuh"
+#include "attention_tcgen05.cuh"
+
+namespace km {
+namespace att {
+namespace {
+
+__device__ int g_attention_grad_wait_expired = 0;
+
+template <int DP>
+struct GradTensorShape {
+    static constexpr int TILE = DP / 64 * TC_SLAB;
+    static constexpr int WARPS_ON_WEIGHTS = 8, LOAD_WARP = 8, MMA_WARP = 9, STATS_WARP = 10, BLOCK = 384;
+    static constexpr int KEYS_STAGES = 2;                                   // keys' kernel: tiles of q, and of dout, under way
+    static constexpr int K_STAGES = 3, V_STAGES = 2;                        // queries' kernel: k is needed again for dq
+    static constexpr int KEYS_SMEM    = 1024 + (2 + 2 * KEYS_STAGES) * TILE + 2 * 2 * TC_ROWS * 4;
+    static constexpr int QUERIES_SMEM = 1024 + (2 + K_STAGES + V_STAGES) * TILE;
+    // more than half of an SM's shared memory: a second block would wait inside tcgen05.alloc
+    static constexpr int at_least_half(int n) { return n > 115 * 1024 ? n : 115 * 1024; }
+};
+
+struct GradMaps { CUtensorMap q, k, v, dout; };
+
+// Bounded waits of one warp; once one has run out the warp stops waiting, and the block writes nothing.
+struct Waits {
+    int* flag;
+    bool expired = false;
+    __device__ __forceinline__ void operator()(uint32_t bar, int parity) {
+        if (!expired && !mbar_wait_bounded(bar, parity)) {
+            expired = true;
+            *reinterpret_cast<volatile int*>(flag) = 1;
+        }
+    }
+    // what is in flight at the end is waited for (with a limit) in any case
+    __device__ __forceinline__ void drain(uint32_t bar, int parity) {
+        if (!mbar_wait_bounded(bar, parity, expired ? 1 << 16 : MBAR_WAIT_TRIES)) *reinterpret_cast<volatile int*>(flag) = 1;
+    }
+};
+
+template <int DP>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int row, int head, int l, uint32_t bar) {
+#pragma unroll
+    for (int d = 0; d < DP / 64; ++d) tma_load_rows(dst + d * TC_SLAB, map, d * 64, row, head, l, bar);
+}
+
+// d (128 x 128) = A B^T over all channels of two tiles
+template <typename T, int DP>
+__device__ __forceinline__ void product_channels(uint32_t d, uint32_t a, uint32_t b) {
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) mma_ss(d, desc_channels(a, k), desc_channels(b, k), instr_desc<T>(128, false), k > 0);
+}
+// d (128 x DP) (+)= A B over the 128 rows of B; A as the two halves of columns left it: 32 columns from `a`, 32 from a + 64
+template <typename T, int DP>
+__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        mma_ts(d, a + (k >> 2) * 64 + (k & 3) * 8, desc_rows(b, k), instr_desc<T>(DP, true), accumulate || k > 0);
+}
+
+// Writes columns [first, first + 32) of a row's sums, times `by`.
+template <typename T>
+__device__ __forceinline__ void put_grad_32(const Heads& to, float* part, bool vec, int l, int row, int h, int rows, int heads, int D,
+                                            int first, const uint32_t* x, float by) {
+    if (vec && !part) {
+        char* const at = to.ptr + (l * to.sl + row * to.sr + h * to.sh + first) * 2;
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+            uint32_t y[4];
+#pragma unroll
+            for (int f = 0; f < 4; ++f) y[f] = Type<T>::pair(__uint_as_float(x[e + 2 * f]) * by, __uint_as_float(x[e + 2 * f + 1]) * by);
+            if (first + e < D) *reinterpret_cast<uint4*>(at + e * 2) = make_uint4(y[0], y[1], y[2], y[3]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
+            put_grad<T>(to, part, l, row, h, rows, heads, D, first + e, __uint_as_float(x[e]) * by, __uint_as_float(x[e + 1]) * by);
+    }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(GradTensorShape<DP>::BLOCK, 1)
+attention_grad_keys_tensor_kernel(const __grid_constant__ AttentionGradParams p, const __grid_constant__ GradMaps maps) {
+    typedef GradTensorShape<DP> S;
+    constexpr int ST = S::KEYS_STAGES;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long s_bars[6 * ST + 6];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_expired;
+    const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u, bars = smem_addr(s_bars);
+    const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto q_full  = [&](int st) { return bars + 8u * st; };
+    auto q_empty = [&](int st) { return bars + 8u * (ST + st); };
+    auto d_full  = [&](int st) { return bars + 8u * (2 * ST + st); };
+    auto d_empty = [&](int st) { return bars + 8u * (3 * ST + st); };
+    auto t_full  = [&](int st) { return bars + 8u * (4 * ST + st); };       // lse and delta of a query tile
+    auto t_empty = [&](int st) { return bars + 8u * (5 * ST + st); };
+    const uint32_t held_full = bars + 8u * (6 * ST), s_full = held_full + 8, dp_full = held_full + 16, p_ready = held_full + 24,
+                   ds_ready = held_full + 32, done = held_full + 40;
+    if (threadIdx.x == 0) {
+        for (int st = 0; st < ST; ++st) {
+            mbar_init(q_full(st), 1), mbar_init(q_empty(st), 1), mbar_init(d_full(st), 1), mbar_init(d_empty(st), 1);
+            mbar_init(t_full(st), 1), mbar_init(t_empty(st), S::WARPS_ON_WEIGHTS);
+        }
+        mbar_init(held_full, 1), mbar_init(s_full, 1), mbar_init(dp_full, 1), mbar_init(done, 1);
+        mbar_init(p_ready, S::WARPS_ON_WEIGHTS), mbar_init(ds_ready, S::WARPS_ON_WEIGHTS);
+        s_expired = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tc::fence_smem_to_async();
+    }
+    after_previous_grid();
+    if (warp == S::MMA_WARP) tc::tmem_alloc(smem_addr(&s_tmem), 512);
+
+    // (key tile, slice, key head, batch entry of k and v)
+    const int tiles = (p.M + TC_ROWS - 1) / TC_ROWS;
+    int       block = blockIdx.x;
+    const int key0 = block % tiles * TC_ROWS; block /= tiles;
+    const int slice = block % p.kv_slices;    block /= p.kv_slices;
+    const int hk = block % p.Hk, kl = block / p.Hk;
+    const int l_count = p.kv_batch == 1 ? p.L : 1, l_first = p.kv_batch == 1 ? 0 : kl;
+    const int q_tiles = (p.N + TC_ROWS - 1) / TC_ROWS;
+    const int all     = l_count * p.G * q_tiles;
+    const int from    = static_cast<int>(static_cast<long long>(all) * slice / p.kv_slices);
+    const int to      = static_cast<int>(static_cast<long long>(all) * (slice + 1) / p.kv_slices);
+    int longest = 0;                               // keys from here on are in no sum of this block: their gradient is zero
+    if (from < to)
+        for (int l = l_first + from / (p.G * q_tiles); l <= l_first + (to - 1) / (p.G * q_tiles); ++l)
+            longest = max(longest, key_count(p.lengths, p.lengths_stride, l, p.M));
+    const int   n_items = key0 < longest ? to - from : 0;
+    const float factor  = find_factor<T, S::BLOCK>(p, l_first, l_first + l_count, hk * p.G, hk * p.G + p.G);
+    const float by      = is_f16<T> ? factor / F16_WEIGHT : 1.0f;
+
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = s_tmem, s_col = tmem, dp_col = tmem + 128, dv_col = tmem + 256, dk_col = tmem + 256 + DP;
+    const uint32_t held_k = base, held_v = base + S::TILE, ring_q = base + 2 * S::TILE, ring_d = ring_q + ST * S::TILE;
+    float* const   stats = reinterpret_cast<float*>(smem_raw + (base - raw) + (2 + 2 * ST) * S::TILE);
+    Waits wait{&s_expired};
+
+    if (warp < S::WARPS_ON_WEIGHTS) {
+        // ------------------------------------------------------------------ weights: lane = key, 64 queries of a tile
+        const int      half = warp >> 2, key = key0 + (threadIdx.x & 127);
+        const uint32_t at   = (static_cast<uint32_t>((warp & 3) * 32) << 16) + half * 64;
+        const u64      c2 = pack2(p.scale_log2, p.scale_log2), by2 = pack2(by, by);
+        for (int i = 0; i < n_items; ++i) {
+            const int  st   = i % ST;
+            const bool seen = key < key_count(p.lengths, p.lengths_stride, l_first + (from + i) / (p.G * q_tiles), p.M);
+            const ulonglong2* const lse   = reinterpret_cast<const ulonglong2*>(stats + st * 2 * TC_ROWS + half * 64);
+            const ulonglong2* const delta = reinterpret_cast<const ulonglong2*>(stats + st * 2 * TC_ROWS + TC_ROWS + half * 64);
+            uint32_t w[64];
+            wait(t_full(st), (i / ST) & 1);
+            wait(s_full, i & 1);
+            tc::fence_after_sync();
+            tmem_load32(s_col + at, w);
+            tmem_load32(s_col + at + 32, w + 32);
+            tmem_wait_load();
+            tmem_loaded32(w);
+            tmem_loaded32(w + 32);
+            uint32_t y[32];
+#pragma unroll
+            for (int j = 0; j < 64; j += 4) {
+                const ulonglong2 shift = lse[j / 4];       // -lse * log2(e), -inf behind the last query
+                float x[4];
+                unpack2(fma2(pack2(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), c2, shift.x), x[0], x[1]);
+                unpack2(fma2(pack2(__uint_as_float(w[j + 2]), __uint_as_float(w[j + 3])), c2, shift.y), x[2], x[3]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = ex2_approx(x[e]), w[j + e] = __float_as_uint(x[e]);
+                y[j / 2]     = seen ? Type<T>::pair(x[0], x[1]) : 0;
+                y[j / 2 + 1] = seen ? Type<T>::pair(x[2], x[3]) : 0;
+            }
+            tmem_store32(s_col + at, y);
+            tc::wait_st();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_ready);
+
+            wait(dp_full, i & 1);
+            tc::fence_after_sync();
+#pragma unroll
+            for (int j = 0; j < 64; j += 32) {
+                uint32_t g[32];
+                tmem_load32(dp_col + at + j, g);
+                tmem_wait_load();
+                tmem_loaded32(g);
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    const ulonglong2 d = delta[(j + e) / 4];       // -delta * by
+                    float x[4];
+                    unpack2(mul2(pack2(__uint_as_float(w[j + e]), __uint_as_float(w[j + e + 1])),
+                                 fma2(pack2(__uint_as_float(g[e]), __uint_as_float(g[e + 1])), by2, d.x)), x[0], x[1]);
+                    unpack2(mul2(pack2(__uint_as_float(w[j + e + 2]), __uint_as_float(w[j + e + 3])),
+                                 fma2(pack2(__uint_as_float(g[e + 2]), __uint_as_float(g[e + 3])), by2, d.y)), x[2], x[3]);
+                    y[(j + e) / 2]     = seen ? Type<T>::pair(x[0], x[1]) : 0;
+                    y[(j + e) / 2 + 1] = seen ? Type<T>::pair(x[2], x[3]) : 0;
+                }
+            }
+            tmem_store32(dp_col + at, y);
+            tc::wait_st();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(t_empty(st)), mbar_arrive(ds_ready);
+        }
+        if (n_items > 0) {
+            wait(done, 0);
+            tc::fence_after_sync();
+        }
+        const bool good = key < p.M && *reinterpret_cast<volatile int*>(&s_expired) == 0;
+        // the first half of the warps writes dv, the second dk
+        const Heads& dst   = half == 0 ? p.dv : p.dk;
+        float* const whole = half == 0 ? p.dv_part : p.dk_part;
+        float* const part  = p.kv_slices > 1 ? whole + static_cast<long long>(slice) * p.kv_batch * p.M * p.Hk * p.D : nullptr;
+        const float  times = half == 0 ? (is_f16<T> ? 1.0f / F16_WEIGHT : 1.0f) : p.scale / factor;
+        const uint32_t sums = (half == 0 ? dv_col : dk_col) + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+#pragma unroll
+        for (int j = 0; j < DP; j += 32) {
+            uint32_t x[32];
+            if (n_items > 0) {
+                tmem_load32(sums + j, x);
+                tmem_wait_load();
+                tmem_loaded32(x);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = 0;
+            }
+            if (good) put_grad_32<T>(dst, part, p.vec_grad, kl, key, hk, p.M, p.Hk, p.D, j, x, times);
+        }
+    } else if (warp == S::LOAD_WARP) {
+        // ------------------------------------------------------------------ copies
+        if (tc::elect_one() && n_items > 0) {
+            const int l_kv = p.k.sl == 0 ? 0 : kl, l_v = p.v.sl == 0 ? 0 : kl;
+            mbar_expect_tx(held_full, 2 * S::TILE);
+            load_tile<DP>(held_k, &maps.k, key0, hk, l_kv, held_full);
+            load_tile<DP>(held_v, &maps.v, key0, hk, l_v, held_full);
+            for (int i = 0; i < n_items; ++i) {
+                const int st = i % ST, item = from + i, lg = item / q_tiles, l = l_first + lg / p.G, h = hk * p.G + lg % p.G;
+                const int n0 = item % q_tiles * TC_ROWS;
+                if (i >= ST) wait(q_empty(st), (i / ST - 1) & 1);
+                mbar_expect_tx(q_full(st), S::TILE);
+                load_tile<DP>(ring_q + st * S::TILE, &maps.q, n0, h, p.q.sl == 0 ? 0 : l, q_full(st));
+                if (i >= ST) wait(d_empty(st), (i / ST - 1) & 1);
+                mbar_expect_tx(d_full(st), S::TILE);
+                load_tile<DP>(ring_d + st * S::TILE, &maps.dout, n0, h, p.dout.sl == 0 ? 0 : l, d_full(st));
+            }
+            wait.drain(held_full, 0);
+            for (int i = max(0, n_items - ST); i < n_items; ++i) {
+                wait.drain(q_full(i % ST), (i / ST) & 1);
+                wait.drain(d_full(i % ST), (i / ST) & 1);
+            }
+        }
+        __syncwarp();
+    } else if (warp == S::STATS_WARP) {
+        // ------------------------------------------------------------------ lse and delta of the query tiles
+        for (int i = 0; i < n_items; ++i) {
+            const int st = i % ST, item = from + i, lg = item / q_tiles, l = l_first + lg / p.G, h = hk * p.G + lg % p.G;
+            const int n0 = item % q_tiles * TC_ROWS;
+            const float* const lse   = p.lse + l * p.lse_sl + h * p.lse_sh;
+            const float* const delta = p.delta + (static_cast<long long>(l) * p.H + h) * p.N;
+            float a[4], d[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int n = n0 + e * 32 + lane;
+                a[e] = n < p.N ? (is_f16<T> ? F16_WEIGHT_LOG2 : 0.0f) - lse[n] * (1.0f / LN2) : -INFINITY;
+                d[e] = n < p.N ? -delta[n] * by : 0.0f;
+            }
+            if (i >= ST) wait(t_empty(st), (i / ST - 1) & 1);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                stats[st * 2 * TC_ROWS + e * 32 + lane]           = a[e];
+                stats[st * 2 * TC_ROWS + TC_ROWS + e * 32 + lane] = d[e];
+            }
+            __threadfence_block();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(t_full(st));
+        }
+    } else if (warp == S::MMA_WARP && n_items > 0) {
+        // ------------------------------------------------------------------ products, issued by one lane
+        const bool one = tc::elect_one();
+        wait(held_full, 0);
+        wait(q_full(0), 0);
+        tc::fence_after_sync();
+        if (one) product_channels<T, DP>(s_col, held_k, ring_q), tc::commit(s_full);
+        __syncwarp();
+        wait(d_full(0), 0);
+        tc::fence_after_sync();
+        if (one) product_channels<T, DP>(dp_col, held_v, ring_d), tc::commit(dp_full);
+        __syncwarp();
+        for (int i = 0; i < n_items; ++i) {
+            const int st = i % ST, next = (i + 1) % ST;
+            wait(p_ready, i & 1);
+            tc::fence_after_sync();
+            if (one) product_rows<T, DP>(dv_col, s_col, ring_d + st * S::TILE, i > 0), tc::commit(d_empty(st));
+            __syncwarp();
+            if (i + 1 < n_items) {
+                wait(q_full(next), ((i + 1) / ST) & 1);
+                tc::fence_after_sync();
+                if (one) product_channels<T, DP>(s_col, held_k, ring_q + next * S::TILE), tc::commit(s_full);
+                __syncwarp();
+            }
+            wait(ds_ready, i & 1);
+            tc::fence_after_sync();
+            if (one) product_rows<T, DP>(dk_col, dp_col, ring_q + st * S::TILE, i > 0), tc::commit(q_empty(st));
+            __syncwarp();
+            if (i + 1 < n_items) {
+                wait(d_full(next), ((i + 1) / ST) & 1);
+                tc::fence_after_sync();
+                if (one) product_channels<T, DP>(dp_col, held_v, ring_d + next * S::TILE), tc::commit(dp_full);
+                __syncwarp();
+            }
+        }
+        if (one) tc::commit(done);
+        __syncwarp();
+        wait.drain(done, 0);
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    if (warp == S::MMA_WARP) tc::tmem_dealloc(tmem, 512);
+    if (threadIdx.x == 0 && s_expired) g_attention_grad_wait_expired = 1;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(GradTensorShape<DP>::BLOCK, 1)
+attention_grad_queries_tensor_kernel(const __grid_constant__ AttentionGradParams p, const __grid_constant__ GradMaps maps) {
+    typedef GradTensorShape<DP> S;
+    constexpr int KS = S::K_STAGES, VS = S::V_STAGES;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long s_bars[2 * KS + 2 * VS + 6];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_expired;
+    const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u, bars = smem_addr(s_bars);
+    const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto k_full  = [&](int st) { return bars + 8u * st; };
+    auto k_empty = [&](int st) { return bars + 8u * (KS + st); };
+    auto v_full  = [&](int st) { return bars + 8u * (2 * KS + st); };
+    auto v_empty = [&](int st) { return bars + 8u * (2 * KS + VS + st); };
+    const uint32_t held_full = bars + 8u * (2 * KS + 2 * VS), dp_full = held_full + 8, ds_ready = held_full + 16, done = held_full + 24;
+    auto s_full  = [&](int buf) { return held_full + 32 + 8u * buf; };
+    if (threadIdx.x == 0) {
+        for (int st = 0; st < KS; ++st) mbar_init(k_full(st), 1), mbar_init(k_empty(st), 1);
+        for (int st = 0; st < VS; ++st) mbar_init(v_full(st), 1), mbar_init(v_empty(st), 1);
+        mbar_init(held_full, 1), mbar_init(dp_full, 1), mbar_init(done, 1), mbar_init(s_full(0), 1), mbar_init(s_full(1), 1);
+        mbar_init(ds_ready, S::WARPS_ON_WEIGHTS);
+        s_expired = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tc::fence_smem_to_async();
+    }
+    after_previous_grid();
+    if (warp == S::MMA_WARP) tc::tmem_alloc(smem_addr(&s_tmem), 512);
+
+    const int tiles = (p.N + TC_ROWS - 1) / TC_ROWS;
+    int       block = blockIdx.x;
+    const int n0 = block % tiles * TC_ROWS; block /= tiles;
+    const int h = block % p.H, l = block / p.H, hk = h / p.G;
+    const int kl = p.kv_batch == 1 ? 0 : l;
+    const int count = key_count(p.lengths, p.lengths_stride, l, p.M), n_items = (count + TC_ROWS - 1) / TC_ROWS;
+    const float factor = find_factor<T, S::BLOCK>(p, l, l + 1, h, h + 1);
+
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    // two sets of scores: the next one is ready when the warps come to it
+    const uint32_t tmem = s_tmem, dp_col = tmem + 256, dq_col = tmem + 384;
+    const uint32_t held_q = base, held_d = base + S::TILE, ring_k = base + 2 * S::TILE, ring_v = ring_k + KS * S::TILE;
+    Waits wait{&s_expired};
+
+    if (warp < S::WARPS_ON_WEIGHTS) {
+        // ------------------------------------------------------------------ weights: lane = query, 64 keys of a tile
+        const int      half = warp >> 2, n = n0 + (threadIdx.x & 127);
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, at = lanes + half * 64;
+        const float    shift = n < p.N ? -p.lse[l * p.lse_sl + h * p.lse_sh + n] * (1.0f / LN2) : -INFINITY;
+        const float    delta = n < p.N ? -p.delta[(static_cast<long long>(l) * p.H + h) * p.N + n] * factor : 0.0f;
+        const u64      c2 = pack2(p.scale_log2, p.scale_log2), by2 = pack2(factor, factor), shift2 = pack2(shift, shift),
+                       delta2 = pack2(delta, delta);
+        for (int i = 0; i < n_items; ++i) {
+            uint32_t w[64];
+            wait(s_full(i & 1), (i >> 1) & 1);
+            tc::fence_after_sync();
+            tmem_load32(tmem + (i & 1) * 128 + at, w);
+            tmem_load32(tmem + (i & 1) * 128 + at + 32, w + 32);
+            tmem_wait_load();
+            tmem_loaded32(w);
+            tmem_loaded32(w + 32);
+#pragma unroll
+            for (int j = 0; j < 64; j += 2) {
+                float x, y;
+                unpack2(fma2(pack2(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), c2, shift2), x, y);
+                w[j] = __float_as_uint(ex2_approx(x)), w[j + 1] = __float_as_uint(ex2_approx(y));
+            }
+            const int  there = count - i * TC_ROWS;                    // keys of this tile
+            const bool tail  = there < TC_ROWS;
+            if (tail && count < p.M) {
+                // rows of k behind the length hold whatever the memory holds, and 0 * NaN is NaN
+                const int st = i % KS;
+                wait(k_full(st), (i / KS) & 1);
+                char* const tile = reinterpret_cast<char*>(smem_raw) + (ring_k - raw) + st * S::TILE;
+                for (int e = there * 8 + static_cast<int>(threadIdx.x); e < TC_ROWS * 8; e += 32 * S::WARPS_ON_WEIGHTS)
+#pragma unroll
+                    for (int d = 0; d < DP / 64; ++d) *reinterpret_cast<uint4*>(tile + d * TC_SLAB + e * 16) = make_uint4(0, 0, 0, 0);
+                tc::fence_smem_to_async();
+            }
+            wait(dp_full, i & 1);
+            tc::fence_after_sync();
+            uint32_t y[32];
+#pragma unroll
+            for (int j = 0; j < 64; j += 32) {
+                uint32_t g[32];
+                tmem_load32(dp_col + at + j, g);
+                tmem_wait_load();
+                tmem_loaded32(g);
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float x0, x1;
+                    unpack2(mul2(pack2(__uint_as_float(w[j + e]), __uint_as_float(w[j + e + 1])),
+                                 fma2(pack2(__uint_as_float(g[e]), __uint_as_float(g[e + 1])), by2, delta2)), x0, x1);
+                    if (tail) {
+                        x0 = half * 64 + j + e < there ? x0 : 0.0f;
+                        x1 = half * 64 + j + e + 1 < there ? x1 : 0.0f;
+                    }
+                    y[(j + e) / 2] = Type<T>::pair(x0, x1);
+                }
+            }
+            tmem_store32(dp_col + at, y);
+            tc::wait_st();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ds_ready);
+        }
+        if (n_items > 0) {
+            wait(done, 0);
+            tc::fence_after_sync();
+        }
+        const bool   good = n < p.N && *reinterpret_cast<volatile int*>(&s_expired) == 0;
+        float* const part = p.q_slices > 1 ? p.dq_part + static_cast<long long>(l) * p.N * p.H * p.D : nullptr;
+#pragma unroll
+        for (int j = 0; j < DP / 2; j += 32) {
+            const int first = half * (DP / 2) + j;
+            uint32_t  x[32];
+            if (n_items > 0) {
+                tmem_load32(dq_col + lanes + first, x);
+                tmem_wait_load();
+                tmem_loaded32(x);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = 0;
+            }
+            if (good) put_grad_32<T>(p.dq, part, p.vec_grad, part ? 0 : l, n, h, p.N, p.H, p.D, first, x, p.scale / factor);
+        }
+    } else if (warp == S::LOAD_WARP) {
+        // ------------------------------------------------------------------ copies
+        if (tc::elect_one() && n_items > 0) {
+            mbar_expect_tx(held_full, 2 * S::TILE);
+            load_tile<DP>(held_q, &maps.q, n0, h, p.q.sl == 0 ? 0 : l, held_full);
+            load_tile<DP>(held_d, &maps.dout, n0, h, p.dout.sl == 0 ? 0 : l, held_full);
+            for (int i = 0; i < n_items; ++i) {
+                const int ks = i % KS, vs = i % VS;
+                if (i >= KS) wait(k_empty(ks), (i / KS - 1) & 1);
+                mbar_expect_tx(k_full(ks), S::TILE);
+                load_tile<DP>(ring_k + ks * S::TILE, &maps.k, i * TC_ROWS, hk, p.k.sl == 0 ? 0 : kl, k_full(ks));
+                if (i >= VS) wait(v_empty(vs), (i / VS - 1) & 1);
+                mbar_expect_tx(v_full(vs), S::TILE);
+                load_tile<DP>(ring_v + vs * S::TILE, &maps.v, i * TC_ROWS, hk, p.v.sl == 0 ? 0 : kl, v_full(vs));
+            }
+            wait.drain(held_full, 0);
+            for (int i = max(0, n_items - KS); i < n_items; ++i) wait.drain(k_full(i % KS), (i / KS) & 1);
+            for (int i = max(0, n_items - VS); i < n_items; ++i) wait.drain(v_full(i % VS), (i / VS) & 1);
+        }
+        __syncwarp();
+    } else if (warp == S::MMA_WARP && n_items > 0) {
+        // ------------------------------------------------------------------ products, issued by one lane
+        const bool one = tc::elect_one();
+        auto scores = [&](int i) {
+            wait(k_full(i % KS), (i / KS) & 1);
+            tc::fence_after_sync();
+            if (one) product_channels<T, DP>(tmem + (i & 1) * 128, held_q, ring_k + i % KS * S::TILE), tc::commit(s_full(i & 1));
+            __syncwarp();
+        };
+        auto gradients = [&](int i) {
+            wait(v_full(i % VS), (i / VS) & 1);
+            tc::fence_after_sync();
+            if (one) product_channels<T, DP>(dp_col, held_d, ring_v + i % VS * S::TILE), tc::commit(dp_full), tc::commit(v_empty(i % VS));
+            __syncwarp();
+        };
+        wait(held_full, 0);
+        scores(0);
+        gradients(0);
+        if (n_items > 1) scores(1);
+        for (int i = 0; i < n_items; ++i) {
+            wait(ds_ready, i & 1);
+            tc::fence_after_sync();
+            if (one) product_rows<T, DP>(dq_col, dp_col, ring_k + i % KS * S::TILE, i > 0), tc::commit(k_empty(i % KS));
+            __syncwarp();
+            if (i + 1 < n_items) gradients(i + 1);
+            if (i + 2 < n_items) scores(i + 2);       // over the scores that ds(i) was the last to need
+        }
+        if (one) tc::commit(done);
+        __syncwarp();
+        wait.drain(done, 0);
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    if (warp == S::MMA_WARP) tc::tmem_dealloc(tmem, 512);
+    if (threadIdx.x == 0 && s_expired) g_attention_grad_wait_expired = 1;
+}
+
+template <typename T, int DP>
+int launch_grad_tensor(const AttentionGradParams& p, const GradMaps& maps, cudaStream_t st) {
+    typedef GradTensorShape<DP> S;
+    constexpr int keys_smem = S::at_least_half(S::KEYS_SMEM), queries_smem = S::at_least_half(S::QUERIES_SMEM);
+    static_assert(keys_smem <= 227 * 1024 && queries_smem <= 227 * 1024, "more shared memory than a block has");
+    auto* const keys    = &attention_grad_keys_tensor_kernel<T, DP>;
+    auto* const queries = &attention_grad_queries_tensor_kernel<T, DP>;
+    int rc = cuda_status(cudaFuncSetAttribute(keys, cudaFuncAttributeMaxDynamicSharedMemorySize, keys_smem), "cudaFuncSetAttribute");
+    if (!rc) rc = cuda_status(cudaFuncSetAttribute(queries, cudaFuncAttributeMaxDynamicSharedMemorySize, queries_smem), "cudaFuncSetAttribute");
+    const long long kb = ceil_div_ll(p.M, TC_ROWS) * p.kv_slices * p.Hk * p.kv_batch, qb = ceil_div_ll(p.N, TC_ROWS) * p.H * p.L;
+    if (!rc && std::max(kb, qb) > 0x7fffffffLL) rc = fail(KM_ERR_TOO_LARGE, "attention: more than 2^31 - 1 blocks");
+    if (!rc)
+        rc = cuda_status(launch_overlapped(keys, dim3(static_cast<unsigned>(kb)), S::BLOCK, keys_smem, st, p, maps),
+                         "attention_grad_keys_tensor_kernel");
+    if (!rc)
+        rc = cuda_status(launch_overlapped(queries, dim3(static_cast<unsigned>(qb)), S::BLOCK, queries_smem, st, p, maps),
+                         "attention_grad_queries_tensor_kernel");
+    return rc;
+}
+
+}  // namespace
+}  // namespace att
+
+int attention_grad_tensor_launch(const AttentionGradParams& p, int type, cudaStream_t st) {
+    using namespace att;
+    GradMaps maps = {};
+    int rc = encode_rows(&maps.q, p.q, p.N, p.H, p.L, p.D, type);
+    if (!rc) rc = encode_rows(&maps.dout, p.dout, p.N, p.H, p.L, p.D, type);
+    if (!rc) rc = encode_rows(&maps.k, p.k, p.M, p.Hk, p.kv_batch, p.D, type);
+    if (!rc) rc = encode_rows(&maps.v, p.v, p.M, p.Hk, p.kv_batch, p.D, type);
+    if (rc) return rc;
+    if (type == ATT_BF16)
+        return p.D <= 64 ? launch_grad_tensor<__nv_bfloat16, 64>(p, maps, st) : launch_grad_tensor<__nv_bfloat16, 128>(p, maps, st);
+    return p.D <= 64 ? launch_grad_tensor<__half, 64>(p, maps, st) : launch_grad_tensor<__half, 128>(p, maps, st);
+}
+
+int attention_grad_tensor_take_wait_flag() {
+    int flag = 0;
+    if (cudaMemcpyFromSymbol(&flag, att::g_attention_grad_wait_expired, sizeof(flag)) != cudaSuccess) return -1;
+    if (flag) {
+        const int zero = 0;
+        if (cudaMemcpyToSymbol(att::g_attention_grad_wait_expired, &zero, sizeof(zero)) != cudaSuccess) return -1;
+    }
+    return flag ? 1 : 0;
+}
+
+}  // namespace km

@@ -222,6 +222,7 @@ int forward(const KmAttentionArgs* a, Kind kind, void* stream) {
 
 struct GradPlan {
     AttentionGradParams p;
+    bool tensor;
     long long delta, peaks, dq, dkv;     // floats of scratch, each a multiple of 4
     long long bytes() const { return 4 * (delta + peaks + dq + 2 * dkv); }
 };
@@ -238,12 +239,16 @@ GradPlan plan_grad(const KmAttentionArgs& a) {
     p.scale = a.scale, p.scale_log2 = a.scale * 1.4426950408889634f;
     p.vec = rows_aligned(a.q, a.type, a.d) && rows_aligned(a.k, a.type, a.d) && rows_aligned(a.v, a.type, a.d) &&
             rows_aligned(a.grad_out, a.type, a.d);
+    p.vec_out  = rows_aligned(a.out, a.type, a.d) && rows_aligned(a.grad_out, a.type, a.d);
+    p.vec_grad = rows_aligned(a.grad_q, a.type, a.d) && rows_aligned(a.grad_k, a.type, a.d) && rows_aligned(a.grad_v, a.type, a.d);
+    plan.tensor = a.d <= 128 && tma_rows_ok(a.q, a.n, a.heads, a.type, a.d) && tma_rows_ok(a.grad_out, a.n, a.heads, a.type, a.d) &&
+                  tma_rows_ok(a.k, a.m, a.key_heads, a.type, a.d) && tma_rows_ok(a.v, a.m, a.key_heads, a.type, a.d);
     p.q_slices = a.q_batch == 1 && a.l > 1 ? a.l : 1;
     p.kv_batch = a.kv_batch;
     // The sum over queries of a key tile is split where the key tiles alone do not fill the SMs.
-    const long long tiles = ceil_div_ll(a.m, ATT_GRAD_ROWS) * a.key_heads * a.kv_batch;
+    const long long tiles = ceil_div_ll(a.m, plan.tensor ? ATT_GRAD_TENSOR_ROWS : ATT_GRAD_ROWS) * a.key_heads * a.kv_batch;
     const long long sum   = static_cast<long long>(a.kv_batch == 1 ? a.l : 1) * p.G * a.n;
-    p.kv_slices = pieces(tiles, sum, 2, 512);
+    p.kv_slices = pieces(tiles, sum, plan.tensor ? 1 : 2, 512);
     if (static_cast<long long>(p.kv_slices) * a.kv_batch * a.m * a.key_heads * a.d > (MOST_SCRATCH >> 3)) p.kv_slices = 1;
     plan.delta = round4(static_cast<long long>(a.l) * a.heads * a.n);
     if (a.type == ATT_F16) {
@@ -284,7 +289,7 @@ int gradient(const KmAttentionArgs* a, void* stream) {
     if (plan.dq) p.dq_part = at, at += plan.dq;
     if (plan.dkv) p.dk_part = at, p.dv_part = at + plan.dkv;
     rc = attention_delta_launch(p, a->type, st);
-    if (!rc) rc = attention_grad_rows_launch(p, a->type, st);
+    if (!rc) rc = plan.tensor ? attention_grad_tensor_launch(p, a->type, st) : attention_grad_rows_launch(p, a->type, st);
     if (!rc && p.q_slices > 1) rc = attention_reduce_launch(p.dq_part, p.q_slices, p.dq, 1, p.N, p.H, p.D, a->type, st);
     if (!rc && p.kv_slices > 1) rc = attention_reduce_launch(p.dk_part, p.kv_slices, p.dk, p.kv_batch, p.M, p.Hk, p.D, a->type, st);
     if (!rc && p.kv_slices > 1) rc = attention_reduce_launch(p.dv_part, p.kv_slices, p.dv, p.kv_batch, p.M, p.Hk, p.D, a->type, st);
@@ -313,7 +318,7 @@ int kermac_b200_describe_attention(const KmAttentionArgs* args, int32_t kind, ch
     if (!buf || buf_len <= 0) return fail(KM_ERR_NULL_POINTER, "buf must not be NULL");
     if (kind == GRAD) {
         const GradPlan plan = plan_grad(*args);
-        snprintf(buf, buf_len, "grad=rows q_slices=%d kv_slices=%d scratch=%lld", plan.p.q_slices, plan.p.kv_slices, plan.bytes());
+        snprintf(buf, buf_len, "grad=%s q_slices=%d kv_slices=%d scratch=%lld", plan.tensor ? "tensor" : "rows", plan.p.q_slices, plan.p.kv_slices, plan.bytes());
     } else {
         const Plan plan = plan_within(*args, static_cast<Kind>(kind), MOST_SCRATCH);
         snprintf(buf, buf_len, "own=%s tiles=%d splits=%d prefix=%s tiles=%d splits=%d scratch=%lld", FORM_NAMES[plan.own],

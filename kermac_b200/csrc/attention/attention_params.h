@@ -51,7 +51,9 @@ struct AttentionGradParams {
     int   q_slices;                      // 1, or L for a broadcast q
     int   kv_batch;                      // batch entries of k and v: 1 or L
     int   kv_slices;                     // pieces of the sum over (l of a broadcast k, head of the group, query tile)
-    int   vec;
+    int   vec;                           // rows of q, k, v and dout can be read 16 bytes at a time
+    int   vec_out;                       // rows of out and dout can
+    int   vec_grad;                      // rows of dq, dk and dv can be written so
 };
 
 enum { ATT_F32 = KM_TYPE_FLOAT32, ATT_BF16 = KM_TYPE_BFLOAT16, ATT_F16 = KM_TYPE_FLOAT16 };
@@ -68,6 +70,10 @@ int  attention_tensor_take_wait_flag();
 constexpr int ATT_GRAD_ROWS = 64, ATT_PEAK_ROWS = 64;
 int  attention_delta_launch(const AttentionGradParams& p, int type, cudaStream_t st);
 int  attention_grad_rows_launch(const AttentionGradParams& p, int type, cudaStream_t st);
+// attention_grad_tensor.cu (tcgen05): as attention_tensor_launch
+constexpr int ATT_GRAD_TENSOR_ROWS = 128;
+int  attention_grad_tensor_launch(const AttentionGradParams& p, int type, cudaStream_t st);
+int  attention_grad_tensor_take_wait_flag();
 // dst[i] = sum over slices of src[slice][i] for a [rows_l][rows][heads][D] array
 int  attention_reduce_launch(const float* src, int slices, const Heads& dst, int L, int rows, int heads, int D, int type,
                              cudaStream_t st);
