@@ -267,6 +267,7 @@ def torch_call():
                     _call = False
                     return _call
                 _bind_torch_call(_torch_call, handle)
+                _torch_call.bind_attention(tuple(C.cast(getattr(handle, name), C.c_void_p).value for name in ATTENTION_SYMBOLS[:6]))
                 _call = _torch_call
     return _call
 

@@ -12,7 +12,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _native
-from .build_a_kernel import _current_stream_for, _is_cuda
+from .build_a_kernel import _call_result, _current_stream_for, _is_cuda, _torch_call_for
 
 __all__ = ["cross_attention", "cross_attention_grad", "prefix_attention"]
 
@@ -135,6 +135,14 @@ def _launch(args, kind, q, debug):
 
 
 def _forward(kind, q, k, v, lengths, scale, out, lse, return_lse, debug, prefix=None):
+    # An ordinary call goes straight to the C-ABI (csrc/km_torch_call.cpp); what that declines (None) is checked below.
+    call = _native._call
+    if call is None:
+        call = _torch_call_for(q)
+    if call and not debug:
+        result = call.attention(kind, q, k, v, *(prefix or (None, None)), lengths, scale, out, lse, return_lse)
+        if result is not None:
+            return _call_result(result, _native.ATTENTION_SYMBOLS[kind])
     args, L = _marshal(q, k, v, lengths, scale, prefix)
     N, H, D = q.shape[-3:]
     if out is None:
@@ -229,6 +237,13 @@ def cross_attention_grad(
     Sums are 32-bit and in a fixed order: equal calls give equal bits.  Takes scratch from torch's allocator for the duration
     of the call: 4 bytes a query and head, and partial sums where an input is broadcast or few states meet many queries.
     """
+    call = _native._call
+    if call is None:
+        call = _torch_call_for(q)
+    if call and not debug and grad_q is None and grad_k is None and grad_v is None:
+        result = call.attention_grad(q, k, v, out, lse, grad_out, lengths, scale)
+        if result is not None:
+            return _call_result(result, _native.ATTENTION_SYMBOLS[_native.ATTENTION_GRAD])
     args, L = _marshal(q, k, v, lengths, scale)
     N, H, D = q.shape[-3:]
     M, Hk = k.shape[-3:-1]

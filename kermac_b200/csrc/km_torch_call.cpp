@@ -2,7 +2,7 @@
 // It reads torch's C++ objects, so it serves the one CPython its file name carries and the one torch version it was
 // compiled against; _native.torch_call() compares the latter.
 //
-// A call of cdist / run_kernel / cdist_grad / kernel_matvec on a small problem is bound by the host:
+// A call of cdist / run_kernel / cdist_grad / kernel_matvec / the attention functions on a small problem is bound by the host:
 // checking three tensors, filling an argument struct through ctypes and asking torch for an output took
 // 22 - 35 us in Python against 4 - 10 us of GPU time.  The functions here do the same work on the
 // tensors' C++ objects (5 to 7 us including the launch, by the machine; 10 to 12 us for a call that splits or packs: it
@@ -17,10 +17,11 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 
-#include "../../include/kermac_b200.h"
+#include "../../include/kermac_b200_attention.h"
 
 namespace {
 
@@ -32,6 +33,9 @@ struct Library {
     int64_t (*grad_scratch)(const KmGradArgs*)            = nullptr;
     int (*matvec)(const KmMatvecArgs*, void*)             = nullptr;
     int64_t (*matvec_scratch)(const KmMatvecArgs*)        = nullptr;
+    // cross_attention, prefix_attention, cross_attention_grad
+    int (*attention[3])(const KmAttentionArgs*, void*)        = {nullptr, nullptr, nullptr};
+    int64_t (*attention_scratch[3])(const KmAttentionArgs*) = {nullptr, nullptr, nullptr};
 } g_lib;
 
 constexpr int64_t MAX_EXTENT = 0x7fffffff;
@@ -483,6 +487,184 @@ PyObject* call_cdist_grad(PyObject*, PyObject* const* v, Py_ssize_t n) {
     return finish(rc, made, given ? v[4] : nullptr);
 }
 
+// ---------------------------------------------------------------- attention
+enum AttentionKind { CROSS = 0, PREFIX = 1, GRAD = 2 };
+
+// A (rows, heads, channels) tensor or, where `batched`, (batch, rows, heads, channels), of type `type`.
+bool read_heads(PyObject* o, at::ScalarType type, int device, bool plain, bool batched, const at::Tensor*& t, KmHeads& h) {
+    if (!THPVariable_CheckExact(o)) return false;
+    t = &THPVariable_Unpack(o);
+    if (!t->is_cuda() || t->scalar_type() != type || t->layout() != at::kStrided || t->device().index() != device) return false;
+    if (!((t->dim() == 3 && plain) || (t->dim() == 4 && batched))) return false;
+    for (int64_t s : t->sizes())
+        if (s > MAX_EXTENT) return false;
+    if (t->size(-1) > 1 && t->stride(-1) != 1) return false;
+    h = {t->data_ptr(), t->dim() == 4 && t->size(0) != 1 ? t->stride(0) : 0, t->stride(-3), t->stride(-2)};
+    return true;
+}
+bool read_lse(PyObject* o, int device, int64_t L, int64_t H, int64_t N, KmAttentionArgs& args) {
+    if (!THPVariable_CheckExact(o)) return false;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_cuda() || t.scalar_type() != at::kFloat || t.layout() != at::kStrided || t.device().index() != device) return false;
+    if (t.dim() != 3 || t.size(0) != L || t.size(1) != H || t.size(2) != N || (N > 1 && t.stride(2) != 1)) return false;
+    args.lse = static_cast<float*>(t.data_ptr()), args.lse_stride_l = t.stride(0), args.lse_stride_head = t.stride(1);
+    return true;
+}
+int64_t batch_of(const at::Tensor& t) { return t.dim() == 4 ? t.size(0) : 1; }
+bool same_shape(const at::Tensor& t, int64_t L, int64_t N, int64_t H, int64_t D) {
+    return t.dim() == 4 && t.size(0) == L && t.size(1) == N && t.size(2) == H && t.size(3) == D;
+}
+
+// q, k, v, lengths and scale, which the three operators share.
+struct AttentionInputs {
+    const at::Tensor *q, *k, *v;
+    int64_t L = 1, N, H, D;
+    int     device;
+};
+bool read_attention(PyObject* pq, PyObject* pk, PyObject* pv, PyObject* lengths, PyObject* scale, AttentionInputs& in, KmAttentionArgs& args) {
+    std::memset(&args, 0, sizeof(args));
+    in.device = call_device(pq);
+    if (in.device < 0) return false;
+    const at::ScalarType type = THPVariable_Unpack(pq).scalar_type();
+    if (type == at::kFloat) args.type = KM_TYPE_FLOAT32;
+    else if (type == at::kBFloat16) args.type = KM_TYPE_BFLOAT16;
+    else if (type == at::kHalf) args.type = KM_TYPE_FLOAT16;
+    else return false;
+    if (!read_heads(pq, type, in.device, true, true, in.q, args.q) || !read_heads(pk, type, in.device, true, true, in.k, args.k) ||
+        !read_heads(pv, type, in.device, true, true, in.v, args.v) || in.k->sizes() != in.v->sizes())
+        return false;
+    in.N = in.q->size(-3), in.H = in.q->size(-2), in.D = in.q->size(-1);
+    const int64_t M = in.k->size(-3), Hk = in.k->size(-2);
+    if (in.k->size(-1) != in.D || in.D < 1 || in.D > 256 || Hk < 1 || in.H % Hk != 0) return false;
+    if (batch_of(*in.q) == 0 || batch_of(*in.k) == 0) return false;
+    if (!merge_batch(in.L, batch_of(*in.q)) || !merge_batch(in.L, batch_of(*in.k))) return false;
+    if (in.L > 1 && M > 0 && (args.k.stride_l == 0) != (args.v.stride_l == 0)) return false;
+    if (lengths != Py_None) {
+        if (!THPVariable_CheckExact(lengths)) return false;
+        const at::Tensor& t = THPVariable_Unpack(lengths);
+        if (!t.is_cuda() || t.scalar_type() != at::kInt || t.layout() != at::kStrided || t.device().index() != in.device || t.dim() != 1 ||
+            (t.size(0) != in.L && in.L != 1))
+            return false;
+        in.L = t.size(0);
+        args.lengths = static_cast<const int32_t*>(t.data_ptr()), args.lengths_stride = in.L > 1 ? t.stride(0) : 0;
+    }
+    if (scale == Py_None) {
+        args.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(in.D)));
+    } else {
+        if (!PyFloat_CheckExact(scale)) return false;
+        args.scale = static_cast<float>(PyFloat_AS_DOUBLE(scale));
+        if (!(args.scale >= 0.0f) || std::isinf(args.scale)) return false;
+    }
+    args.l = static_cast<int32_t>(in.L), args.n = static_cast<int32_t>(in.N), args.m = static_cast<int32_t>(M);
+    args.heads = static_cast<int32_t>(in.H), args.key_heads = static_cast<int32_t>(Hk), args.d = static_cast<int32_t>(in.D);
+    return true;
+}
+
+at::Tensor new_heads(int64_t L, int64_t rows, int64_t heads, int64_t D, const at::Tensor& like, int device) {
+    return at::Tensor(at::detail::empty_cuda({L, rows, heads, D}, like.scalar_type(),
+                                             c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(device)), std::nullopt));
+}
+KmHeads heads_of(const at::Tensor& t) { return {t.data_ptr(), t.size(0) != 1 ? t.stride(0) : 0, t.stride(1), t.stride(2)}; }
+
+int launch_attention(KmAttentionArgs& args, AttentionKind kind, int device) {
+    at::Tensor scratch;
+    const int64_t need = g_lib.attention_scratch[kind](&args);
+    if (need > 0) {
+        scratch            = new_float({need / 4}, device);
+        args.scratch       = scratch.data_ptr();
+        args.scratch_bytes = need;
+    }
+    return g_lib.attention[kind](&args, c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream());
+}
+
+// attention(kind, q, k, v, k_prefix, v_prefix, lengths, scale, out, lse, return_lse)
+PyObject* call_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    int32_t kind;
+    if (n != 11 || !g_lib.attention[0] || !read_int32(v[0], kind) || (kind != CROSS && kind != PREFIX) || !PyBool_Check(v[10])) return decline();
+    AttentionInputs in;
+    KmAttentionArgs args;
+    if (!read_attention(v[1], v[2], v[3], v[6], v[7], in, args)) return decline();
+    if (kind == PREFIX) {
+        const at::Tensor *kp, *vp;
+        if (!read_heads(v[4], in.q->scalar_type(), in.device, true, false, kp, args.k_prefix) ||
+            !read_heads(v[5], in.q->scalar_type(), in.device, true, false, vp, args.v_prefix) || kp->sizes() != vp->sizes() ||
+            kp->size(1) != args.key_heads || kp->size(2) != in.D)
+            return decline();
+        args.prefix = static_cast<int32_t>(kp->size(0));
+    }
+    const at::Tensor* out = nullptr;
+    if (v[8] != Py_None) {
+        if (!read_heads(v[8], in.q->scalar_type(), in.device, false, true, out, args.out) || !same_shape(*out, in.L, in.N, in.H, in.D))
+            return decline();
+    }
+    if (v[9] != Py_None && !read_lse(v[9], in.device, in.L, in.H, in.N, args)) return decline();
+    const bool return_lse = v[10] == Py_True;
+    at::Tensor made, made_lse;
+    int rc;
+    {
+        Unlocked unlocked;
+        if (!out) {
+            made     = new_heads(in.L, in.N, in.H, in.D, *in.q, in.device);
+            args.out = heads_of(made);
+        }
+        if (return_lse && !args.lse && v[9] == Py_None) {
+            made_lse = new_float({in.L, in.H, in.N}, in.device);
+            args.lse = static_cast<float*>(made_lse.data_ptr()), args.lse_stride_l = made_lse.stride(0), args.lse_stride_head = made_lse.stride(1);
+        }
+        rc = launch_attention(args, static_cast<AttentionKind>(kind), in.device);
+    }
+    PyObject* result = finish(rc, made, out ? v[8] : nullptr);
+    if (rc != 0 || !return_lse || !result) return result;
+    PyObject* lse  = finish(0, made_lse, v[9] != Py_None ? v[9] : nullptr);
+    PyObject* both = lse ? PyTuple_Pack(2, result, lse) : nullptr;
+    Py_DECREF(result);
+    Py_XDECREF(lse);
+    return both;
+}
+
+// attention_grad(q, k, v, out, lse, grad_out, lengths, scale), with the gradients allocated here
+PyObject* call_attention_grad(PyObject*, PyObject* const* v, Py_ssize_t n) {
+    if (n != 8 || !g_lib.attention[GRAD]) return decline();
+    AttentionInputs in;
+    KmAttentionArgs args;
+    const at::Tensor *out, *grad_out;
+    if (!read_attention(v[0], v[1], v[2], v[6], v[7], in, args)) return decline();
+    if (!read_heads(v[3], in.q->scalar_type(), in.device, false, true, out, args.out) || !same_shape(*out, in.L, in.N, in.H, in.D) ||
+        !read_heads(v[5], in.q->scalar_type(), in.device, false, true, grad_out, args.grad_out) ||
+        !same_shape(*grad_out, in.L, in.N, in.H, in.D) || !read_lse(v[4], in.device, in.L, in.H, in.N, args))
+        return decline();
+    args.q_batch = static_cast<int32_t>(batch_of(*in.q)), args.kv_batch = static_cast<int32_t>(batch_of(*in.k));
+    at::Tensor made[3];
+    int rc;
+    {
+        Unlocked unlocked;
+        made[0] = new_heads(args.q_batch, in.N, in.H, in.D, *in.q, in.device);
+        made[1] = new_heads(args.kv_batch, args.m, args.key_heads, in.D, *in.q, in.device);
+        made[2] = new_heads(args.kv_batch, args.m, args.key_heads, in.D, *in.q, in.device);
+        args.grad_q = heads_of(made[0]), args.grad_k = heads_of(made[1]), args.grad_v = heads_of(made[2]);
+        rc = launch_attention(args, GRAD, in.device);
+    }
+    if (rc != 0) return PyLong_FromLong(rc);
+    PyObject* grads = PyTuple_New(3);
+    for (int i = 0; grads && i < 3; ++i) {
+        PyObject* wrapped = THPVariable_Wrap(made[i]);
+        if (!wrapped) Py_CLEAR(grads);
+        else PyTuple_SET_ITEM(grads, i, wrapped);
+    }
+    return grads;
+}
+
+// bind_attention((addresses of the three entry points and of their three scratch functions))
+PyObject* call_bind_attention(PyObject*, PyObject* args) {
+    unsigned long long fn[6];
+    if (!PyArg_ParseTuple(args, "(KKKKKK)", &fn[0], &fn[1], &fn[2], &fn[3], &fn[4], &fn[5])) return nullptr;
+    for (int i = 0; i < 3; ++i) {
+        g_lib.attention[i]         = reinterpret_cast<int (*)(const KmAttentionArgs*, void*)>(fn[i]);
+        g_lib.attention_scratch[i] = reinterpret_cast<int64_t (*)(const KmAttentionArgs*)>(fn[3 + i]);
+    }
+    Py_RETURN_NONE;
+}
+
 // bind((addresses of the six entry points), (InnerOperator, PowerType, KernelType))
 PyObject* call_bind(PyObject*, PyObject* args) {
     unsigned long long build_fn, build_scratch_fn, grad_fn, grad_scratch_fn, matvec_fn, matvec_scratch_fn;
@@ -516,6 +698,9 @@ PyObject* guarded(PyObject* self, PyObject* const* v, Py_ssize_t n) {
 
 #define FAST(fn) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&guarded<fn>)), METH_FASTCALL
 PyMethodDef g_methods[] = {
+    {"bind_attention", call_bind_attention, METH_VARARGS, "bind_attention(entry point addresses)"},
+    {"attention", FAST(call_attention), "attention(kind, q, k, v, k_prefix, v_prefix, lengths, scale, out, lse, return_lse)"},
+    {"attention_grad", FAST(call_attention_grad), "attention_grad(q, k, v, out, lse, grad_out, lengths, scale)"},
     {"bind", call_bind, METH_VARARGS, "bind(entry point addresses, enum classes)"},
     {"cdist", FAST(call_cdist), "cdist(a, b, out, p, skip_epilogue) -> tensor, None (not an ordinary call) or an error code"},
     {"run_kernel", FAST(call_run_kernel), "run_kernel(descriptor, a, b, out, p, inner_p, outer_p, bandwidth, epsilon, regularization, offset_x, offset_y)"},

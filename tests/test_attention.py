@@ -222,6 +222,17 @@ def test_the_reference_name_serves_them():
         assert getattr(served, name) is getattr(kermac, name)
 
 
+def test_the_extension_declines_what_is_not_an_ordinary_call():
+    call = _native.torch_call()
+    q, k = _t(*Q), _t(*K)
+    assert call.attention(0, q, k, k, None, None, None, None, None, None, False) is None      # not on a CUDA device
+    assert call.attention(2, q, k, k, None, None, None, None, None, None, False) is None
+    assert call.attention(0, q.numpy(), k, k, None, None, None, None, None, None, False) is None
+    assert call.attention(0, q, k) is None
+    assert call.attention_grad(q, k, k, q, _t(2, 4, 3), q, None, None) is None
+    assert call.attention_grad(None) is None
+
+
 def _attention_kernels():
     """(name, parameters, body) of the kernels under csrc/attention."""
     for path in sorted(glob.glob(os.path.join(ROOT, "kermac_b200", "csrc", "attention", "*.cu*"))):

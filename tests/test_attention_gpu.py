@@ -395,3 +395,30 @@ def test_a_run_of_them_together():
     many = kermac.prefix_attention(new_q, kp, vp, new_k, new_v)
     want, _, bound, _ = ao.attention(new_q, new_k, new_v, prefix=(kp, vp))
     assert_within(many, want, bound, "all tokens at once")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("N", [1, 100])
+def test_same_bits_as_the_ctypes_marshalling(dtype, N, capsys):
+    L, M, H, Hk, D, P = 2, 300, 4, 2, 64, 130
+    q, g = make(1, L, N, H, D, dtype=dtype), make(9, L, N, H, D, dtype=dtype)
+    k, v = make(2, L, M, Hk, D, dtype=dtype), make(3, L, M, Hk, D, dtype=dtype)
+    kp, vp = make(4, P, Hk, D, dtype=dtype), make(5, P, Hk, D, dtype=dtype)
+    lengths = torch.tensor([300, 120], dtype=torch.int32, device="cuda")
+    assert _native.torch_call()
+    for options in (dict(), dict(lengths=lengths), dict(lengths=lengths, scale=0.3)):
+        out, lse = kermac.cross_attention(q, k, v, return_lse=True, **options)
+        slow, slow_lse = kermac.cross_attention(q, k, v, return_lse=True, debug=True, **options)
+        assert torch.equal(out, slow) and torch.equal(lse, slow_lse)
+        into, into_lse = torch.empty_like(out), torch.empty_like(lse)
+        got = kermac.cross_attention(q, k, v, out=into, lse=into_lse, **options)
+        assert got is into and torch.equal(into, out) and torch.equal(into_lse, lse)
+        for a, b in zip(kermac.cross_attention_grad(q, k, v, out, lse, g, **options),
+                        kermac.cross_attention_grad(q, k, v, out, lse, g, debug=True, **options)):
+            assert torch.equal(a, b)
+        assert torch.equal(kermac.prefix_attention(q, kp, vp, k, v, **options), kermac.prefix_attention(q, kp, vp, k, v, debug=True, **options))
+    assert "Launching kernel" in capsys.readouterr().out
+    # declined by the extension, refused by the Python layer
+    for bad in (dict(k=k.cpu()), dict(scale=-1.0), dict(lengths=lengths.long())):
+        with pytest.raises((TypeError, ValueError)):
+            kermac.cross_attention(**dict(dict(q=q, k=k, v=v), **bad))
