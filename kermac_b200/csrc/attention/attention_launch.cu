@@ -3,21 +3,42 @@
 #include <cmath>
 
 #include "../km_build_tma.cuh"
-#include "attention_params.h"
+#include "attention_tcgen05.cuh"
 
 namespace km {
 namespace att {
-int encode_rows(CUtensorMap* map, const Heads& t, int rows, int heads, int L, int D, int type) {
+int encode_rows(CUtensorMap* map, const Heads& t, int rows, int heads, int L, int D, int type, int box_rows) {
     // an extent of one may come with any stride; a broadcast batch is one entry
     const long long dense = (D + 7) & ~7;
     const cuuint64_t dims[4]    = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(heads),
                                    static_cast<cuuint64_t>(t.sl == 0 ? 1 : L)};
     const cuuint64_t strides[3] = {static_cast<cuuint64_t>(rows > 1 ? t.sr : dense) * 2, static_cast<cuuint64_t>(heads > 1 ? t.sh : dense) * 2,
                                    static_cast<cuuint64_t>(dims[3] > 1 ? t.sl : dense) * 2};
-    const cuuint32_t box[4] = {64, 128, 1, 1};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
     return encode_tma_16bit(map, t.ptr, type == ATT_BF16, dims, strides, box);
 }
+
+int encode_forward(TensorMaps* maps, const AttentionParams& p, int type, int box_rows) {
+    int rc = 0;
+    if (p.own_tiles > 0 && p.M > 0) {
+        rc = encode_rows(&maps->k, p.k, p.M, p.Hk, p.L, p.D, type, box_rows);
+        if (!rc) rc = encode_rows(&maps->v, p.v, p.M, p.Hk, p.L, p.D, type, box_rows);
+    }
+    if (!rc && p.prefix_tiles > 0) {
+        rc = encode_rows(&maps->kp, p.kp, p.P, p.Hk, 1, p.D, type, box_rows);
+        if (!rc) rc = encode_rows(&maps->vp, p.vp, p.P, p.Hk, 1, p.D, type, box_rows);
+    }
+    return rc;
+}
 }  // namespace att
+
+int count_blocks(const AttentionParams& p, unsigned* blocks) {
+    const long long n = static_cast<long long>(p.Hk) * p.prefix_tiles * p.prefix_splits +
+                        static_cast<long long>(p.L) * p.Hk * p.own_tiles * p.own_splits;
+    if (n > 0x7fffffffLL) return fail(KM_ERR_TOO_LARGE, "attention: more than 2^31 - 1 blocks");
+    *blocks = static_cast<unsigned>(n);
+    return 0;
+}
 
 namespace {
 
@@ -105,10 +126,16 @@ bool tma_rows_ok(const KmHeads& t, int rows, int n_heads, int type, int d) {
            (n_heads <= 1 || (t.stride_head > 0 && t.stride_head < most)) && t.stride_l < most;
 }
 
-// The kernels of the forward pass: 16 rows whose keys four warps share out, 64 rows on mma.sync, 256 on tcgen05.
-enum Form { FEW, ROWS, TENSOR };
-const char* const FORM_NAMES[] = {"few", "rows", "tensor"};
-const int FORM_ROWS[] = {ATT_FEW_ROWS, ATT_TILE_ROWS, ATT_TENSOR_ROWS};
+// The kernels of the forward pass.  TENSOR: 256 rows on tcgen05.  FEW: 8, 16 or 32 rows whose keys four warps share out, fed by TMA.
+// For what these two do not take: SCALAR_FEW, 16 rows in the manner of FEW, and ROWS, 64 rows that share key tiles.
+enum Kernel { TENSOR, FEW, SCALAR_FEW, ROWS };
+struct Form {
+    Kernel kernel;
+    int    rows;            // of a block
+    int    per_sm, least;   // blocks that an SM holds; keys below which a piece does not pay
+    bool operator!=(const Form& f) const { return kernel != f.kernel || rows != f.rows; }
+    const char* name() const { return kernel == TENSOR ? "tensor" : kernel == FEW ? "few" : kernel == ROWS ? "rows" : "scalar few"; }
+};
 
 struct Plan {
     Form own, prefix;
@@ -116,17 +143,18 @@ struct Plan {
     long long bytes;
 };
 
-Form choose_form(long long rows, bool tensor_ok) {
-    if (rows <= ATT_FEW_ROWS) return FEW;
-    return tensor_ok && rows > ATT_TILE_ROWS ? TENSOR : ROWS;
+Form choose_form(long long rows, bool tma_ok, int d) {
+    if (tma_ok && rows > 64) return {TENSOR, ATT_TENSOR_ROWS, 1, 512};
+    if (tma_ok) return {FEW, rows <= 8 ? 8 : rows <= 16 ? 16 : ATT_FEW_MOST, d <= 64 ? 2 : 1, 256};
+    if (rows <= ATT_FEW_ROWS) return {SCALAR_FEW, ATT_FEW_ROWS, 1, 256};
+    return {ROWS, ATT_TILE_ROWS, 2, 512};
 }
 
-// How many pieces the keys of `blocks` blocks are split into: enough to give every SM `per_sm` blocks, no piece shorter than
-// `least` keys.
+// How many pieces the keys of `blocks` blocks are split into: as many as the SMs hold at once, no piece shorter than `least` keys.
 int pieces(long long blocks, long long keys, int per_sm, int least) {
     if (blocks <= 0 || keys <= 0) return 1;
-    const long long wanted = ceil_div_ll(static_cast<long long>(sm_count()) * per_sm, blocks);
-    return static_cast<int>(std::max(1LL, std::min({wanted, keys / least, 256LL})));
+    const long long fit = static_cast<long long>(sm_count()) * per_sm / blocks;
+    return static_cast<int>(std::max(1LL, std::min({fit, keys / least, 256LL})));
 }
 
 Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool scratch) {
@@ -155,18 +183,15 @@ Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool scratch) {
                                           : own_ok;
     p.vec_out = rows_aligned(a.out, a.type, a.d);
     const long long own_rows = static_cast<long long>(p.N) * p.G, prefix_rows = own_rows * p.L;
-    plan.own    = choose_form(own_rows, own_ok);
-    plan.prefix = choose_form(prefix_rows, prefix_ok);
-    auto split = [&](Form form, long long blocks, int keys) {
-        return scratch ? pieces(blocks, keys, form == TENSOR ? 1 : 2, form == FEW ? 256 : 512) : 1;
-    };
+    plan.own    = choose_form(own_rows, own_ok, p.D);
+    plan.prefix = choose_form(prefix_rows, prefix_ok, p.D);
     if (p.M > 0 || p.P == 0) {
-        p.own_tiles  = static_cast<int>(ceil_div_ll(own_rows, FORM_ROWS[plan.own]));
-        p.own_splits = split(plan.own, static_cast<long long>(p.own_tiles) * p.L * p.Hk, p.M);
+        p.own_tiles  = static_cast<int>(ceil_div_ll(own_rows, plan.own.rows));
+        p.own_splits = scratch ? pieces(static_cast<long long>(p.own_tiles) * p.L * p.Hk, p.M, plan.own.per_sm, plan.own.least) : 1;
     }
     if (p.P > 0) {
-        p.prefix_tiles  = static_cast<int>(ceil_div_ll(prefix_rows, FORM_ROWS[plan.prefix]));
-        p.prefix_splits = split(plan.prefix, static_cast<long long>(p.prefix_tiles) * p.Hk, p.P);
+        p.prefix_tiles  = static_cast<int>(ceil_div_ll(prefix_rows, plan.prefix.rows));
+        p.prefix_splits = scratch ? pieces(static_cast<long long>(p.prefix_tiles) * p.Hk, p.P, plan.prefix.per_sm, plan.prefix.least) : 1;
     }
     p.parts = p.own_splits + p.prefix_splits;
     if (p.parts > 1) plan.bytes = static_cast<long long>(p.parts) * p.L * p.N * p.H * (p.D + 1) * 4;
@@ -203,8 +228,10 @@ int forward(const KmAttentionArgs* a, Kind kind, void* stream) {
         plan.p.part_o   = static_cast<float*>(a->scratch);
         plan.p.part_lse = plan.p.part_o + static_cast<long long>(plan.p.parts) * plan.p.L * plan.p.N * plan.p.H * plan.p.D;
     }
-    auto launch = [&](const AttentionParams& p, Form form) {
-        return form == TENSOR ? attention_tensor_launch(p, a->type, st) : attention_rows_launch(p, a->type, form == FEW, st);
+    auto launch = [&](const AttentionParams& p, const Form& form) {
+        if (form.kernel == TENSOR) return attention_tensor_launch(p, a->type, st);
+        if (form.kernel == FEW) return attention_few_launch(p, a->type, form.rows, st);
+        return attention_rows_launch(p, a->type, form.kernel == SCALAR_FEW, st);
     };
     const bool own = plan.p.own_splits > 0, prefix = plan.p.prefix_splits > 0;
     if (own && prefix && plan.own != plan.prefix) {
@@ -321,8 +348,8 @@ int kermac_b200_describe_attention(const KmAttentionArgs* args, int32_t kind, ch
         snprintf(buf, buf_len, "grad=%s q_slices=%d kv_slices=%d scratch=%lld", plan.tensor ? "tensor" : "rows", plan.p.q_slices, plan.p.kv_slices, plan.bytes());
     } else {
         const Plan plan = plan_within(*args, static_cast<Kind>(kind), MOST_SCRATCH);
-        snprintf(buf, buf_len, "own=%s tiles=%d splits=%d prefix=%s tiles=%d splits=%d scratch=%lld", FORM_NAMES[plan.own],
-                 plan.p.own_tiles, plan.p.own_splits, FORM_NAMES[plan.prefix], plan.p.prefix_tiles, plan.p.prefix_splits,
+        snprintf(buf, buf_len, "own=%s rows=%d tiles=%d splits=%d prefix=%s rows=%d tiles=%d splits=%d scratch=%lld", plan.own.name(),
+                 plan.own.rows, plan.p.own_tiles, plan.p.own_splits, plan.prefix.name(), plan.prefix.rows, plan.p.prefix_tiles, plan.p.prefix_splits,
                  plan.bytes);
     }
     return 0;

@@ -62,6 +62,12 @@ enum { ATT_F32 = KM_TYPE_FLOAT32, ATT_BF16 = KM_TYPE_BFLOAT16, ATT_F16 = KM_TYPE
 int  attention_rows_launch(const AttentionParams& p, int type, bool few, cudaStream_t st);
 constexpr int ATT_FEW_ROWS = 16, ATT_TILE_ROWS = 64;
 int  attention_join_launch(const AttentionParams& p, int type, cudaStream_t st);
+// attention_few.cu: 16-bit types, D a multiple of 8 up to 128, rows that TMA can copy; up to ATT_FEW_MOST rows a block (8, 16 or 32).
+constexpr int ATT_FEW_MOST = 32;
+int  attention_few_launch(const AttentionParams& p, int type, int rows, cudaStream_t st);
+int  attention_few_take_wait_flag();
+// Blocks of a forward launch: every (key head, row tile, piece) of both sets of keys.
+int  count_blocks(const AttentionParams& p, unsigned* blocks);
 // attention_tensor.cu (tcgen05): 16-bit types, D a multiple of 8 up to 128, rows that TMA can copy.
 constexpr int ATT_TENSOR_ROWS = 256;
 int  attention_tensor_launch(const AttentionParams& p, int type, cudaStream_t st);

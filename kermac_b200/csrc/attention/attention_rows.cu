@@ -219,10 +219,9 @@ int launch_rows(const AttentionParams& p, cudaStream_t st) {
     auto* const kernel = &attention_rows_kernel<T, DP, FEW>;
     int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute");
     if (rc) return rc;
-    const long long blocks = static_cast<long long>(p.Hk) * p.prefix_tiles * p.prefix_splits +
-                             static_cast<long long>(p.L) * p.Hk * p.own_tiles * p.own_splits;
-    if (blocks > 0x7fffffffLL) return fail(KM_ERR_TOO_LARGE, "attention: more than 2^31 - 1 blocks");
-    return cuda_status(launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks)), THREADS, smem, st, p), "attention_rows_kernel");
+    unsigned blocks;
+    if ((rc = count_blocks(p, &blocks))) return rc;
+    return cuda_status(launch_overlapped(kernel, dim3(blocks), THREADS, smem, st, p), "attention_rows_kernel");
 }
 template <typename T>
 int launch_type(const AttentionParams& p, bool few, cudaStream_t st) {

@@ -78,11 +78,14 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
         : "memory");
 }
 
-// Host: a 16-bit tensor [l][row][head][channel] for copies of boxes of 64 channels x 128 rows; what a box has beyond `rows` or D
+// Host: a 16-bit tensor [l][row][head][channel] for copies of boxes of 64 channels; what a box has beyond `rows` or D
 // is filled with zeros.  Needs tma_rows_ok().
-int encode_rows(CUtensorMap* map, const Heads& t, int rows, int heads, int L, int D, int type);
+int encode_rows(CUtensorMap* map, const Heads& t, int rows, int heads, int L, int D, int type, int box_rows = TC_ROWS);
+// The keys and values of a forward pass, those that it has.
+struct TensorMaps { CUtensorMap k, v, kp, vp; };
+int encode_forward(TensorMaps* maps, const AttentionParams& p, int type, int box_rows);
 
-// One box of 64 channels x 128 rows of a [l][head][row][channel] tensor; x is 0 or 64 (16-bit: a multiple of 128 bytes).
+// One box of 64 channels of a [l][head][row][channel] tensor; x is 0 or 64 (16-bit: a multiple of 128 bytes).
 __device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, int x, int row, int head, int l, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"

@@ -29,8 +29,6 @@ struct TensorShape {
     static constexpr int S_COL = 0, O_COL = GROUPS * 128;
 };
 
-struct TensorMaps { CUtensorMap k, v, kp, vp; };
-
 template <typename T, int DP>
 __global__ void __launch_bounds__(TensorShape<DP>::THREADS, 1)
 attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ TensorMaps maps) {
@@ -304,10 +302,9 @@ int launch_tensor(const AttentionParams& p, const TensorMaps& maps, cudaStream_t
     auto* const kernel = &attention_tensor_kernel<T, DP>;
     int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "cudaFuncSetAttribute");
     if (rc) return rc;
-    const long long blocks = static_cast<long long>(p.Hk) * p.prefix_tiles * p.prefix_splits +
-                             static_cast<long long>(p.L) * p.Hk * p.own_tiles * p.own_splits;
-    if (blocks > 0x7fffffffLL) return fail(KM_ERR_TOO_LARGE, "attention: more than 2^31 - 1 blocks");
-    return cuda_status(launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks)), S::THREADS, S::SMEM, st, p, maps),
+    unsigned blocks;
+    if ((rc = count_blocks(p, &blocks))) return rc;
+    return cuda_status(launch_overlapped(kernel, dim3(blocks), S::THREADS, S::SMEM, st, p, maps),
                        "attention_tensor_kernel");
 }
 
@@ -317,16 +314,7 @@ int launch_tensor(const AttentionParams& p, const TensorMaps& maps, cudaStream_t
 int attention_tensor_launch(const AttentionParams& p, int type, cudaStream_t st) {
     using namespace att;
     TensorMaps maps = {};
-    int rc = 0;
-    if (p.own_tiles > 0 && p.M > 0) {
-        rc = encode_rows(&maps.k, p.k, p.M, p.Hk, p.L, p.D, type);
-        if (!rc) rc = encode_rows(&maps.v, p.v, p.M, p.Hk, p.L, p.D, type);
-    }
-    if (!rc && p.prefix_tiles > 0) {
-        rc = encode_rows(&maps.kp, p.kp, p.P, p.Hk, 1, p.D, type);
-        if (!rc) rc = encode_rows(&maps.vp, p.vp, p.P, p.Hk, 1, p.D, type);
-    }
-    if (rc) return rc;
+    if (int rc = encode_forward(&maps, p, type, TC_ROWS)) return rc;
     if (type == ATT_BF16) return p.D <= 64 ? launch_tensor<__nv_bfloat16, 64>(p, maps, st) : launch_tensor<__nv_bfloat16, 128>(p, maps, st);
     return p.D <= 64 ? launch_tensor<__half, 64>(p, maps, st) : launch_tensor<__half, 128>(p, maps, st);
 }

@@ -70,12 +70,22 @@ __device__ __forceinline__ void put_pair(const AttentionParams& p, const Work& w
     if (c >= p.D) return;
     if (p.parts == 1) {
         T* o = reinterpret_cast<T*>(p.out.ptr) + row.l * p.out.sl + row.n * p.out.sr + row.h * p.out.sh + c;
+        if constexpr (sizeof(T) == 2) {
+            if (p.vec_out) {
+                *reinterpret_cast<uint32_t*>(o) = Type<T>::pair(x, y);
+                return;
+            }
+        }
         o[0] = Type<T>::to(x);
         if (c + 1 < p.D) o[1] = Type<T>::to(y);
     } else {
         float* o = p.part_o + ((((static_cast<long long>(w.part) * p.L + row.l) * p.N + row.n) * p.H) + row.h) * p.D + c;
-        o[0] = x;
-        if (c + 1 < p.D) o[1] = y;
+        if (p.D % 2 == 0) {
+            *reinterpret_cast<float2*>(o) = make_float2(x, y);
+        } else {
+            o[0] = x;
+            if (c + 1 < p.D) o[1] = y;
+        }
     }
 }
 // lse2: log2 of the sum of exp2; -inf for a row without keys.
