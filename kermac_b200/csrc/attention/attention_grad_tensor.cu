@@ -56,20 +56,6 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
     for (int d = 0; d < DP / 64; ++d) tma_load_rows(dst + d * TC_SLAB, map, d * 64, row, head, l, bar);
 }
 
-// d (128 x 128) = A B^T over all channels of two tiles
-template <typename T, int DP>
-__device__ __forceinline__ void product_channels(uint32_t d, uint32_t a, uint32_t b) {
-#pragma unroll
-    for (int k = 0; k < DP / 16; ++k) mma_ss(d, desc_channels(a, k), desc_channels(b, k), instr_desc<T>(128, false), k > 0);
-}
-// d (128 x DP) (+)= A B over the 128 rows of B; A as the two halves of columns left it: 32 columns from `a`, 32 from a + 64
-template <typename T, int DP>
-__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-        mma_ts(d, a + (k >> 2) * 64 + (k & 3) * 8, desc_rows(b, k), instr_desc<T>(DP, true), accumulate || k > 0);
-}
-
 // Writes columns [first, first + 32) of a row's sums, times `by`.
 template <typename T>
 __device__ __forceinline__ void put_grad_32(const Heads& to, float* part, bool vec, int l, int row, int h, int rows, int heads, int D,
@@ -286,42 +272,36 @@ attention_grad_keys_tensor_kernel(const __grid_constant__ AttentionGradParams p,
             if (lane == 0) mbar_arrive(t_full(st));
         }
     } else if (warp == S::MMA_WARP && n_items > 0) {
-        // ------------------------------------------------------------------ products, issued by one lane
-        const bool one = tc::elect_one();
+        // ------------------------------------------------------------------ products
         wait(held_full, 0);
         wait(q_full(0), 0);
         tc::fence_after_sync();
-        if (one) product_channels<T, DP>(s_col, held_k, ring_q), tc::commit(s_full);
-        __syncwarp();
+        issue_channels<T, DP>(p.D, s_col, desc_channels(held_k), desc_channels(ring_q), s_full);
         wait(d_full(0), 0);
         tc::fence_after_sync();
-        if (one) product_channels<T, DP>(dp_col, held_v, ring_d), tc::commit(dp_full);
-        __syncwarp();
+        issue_channels<T, DP>(p.D, dp_col, desc_channels(held_v), desc_channels(ring_d), dp_full);
         for (int i = 0; i < n_items; ++i) {
             const int st = i % ST, next = (i + 1) % ST;
             wait(p_ready, i & 1);
             tc::fence_after_sync();
-            if (one) product_rows<T, DP>(dv_col, s_col, ring_d + st * S::TILE, i > 0), tc::commit(d_empty(st));
-            __syncwarp();
+            issue_rows<T, DP>(p.D, dv_col, s_col, desc_rows(ring_d + st * S::TILE), i > 0);
+            issue_commit(d_empty(st));
             if (i + 1 < n_items) {
                 wait(q_full(next), ((i + 1) / ST) & 1);
                 tc::fence_after_sync();
-                if (one) product_channels<T, DP>(s_col, held_k, ring_q + next * S::TILE), tc::commit(s_full);
-                __syncwarp();
+                issue_channels<T, DP>(p.D, s_col, desc_channels(held_k), desc_channels(ring_q + next * S::TILE), s_full);
             }
             wait(ds_ready, i & 1);
             tc::fence_after_sync();
-            if (one) product_rows<T, DP>(dk_col, dp_col, ring_q + st * S::TILE, i > 0), tc::commit(q_empty(st));
-            __syncwarp();
+            issue_rows<T, DP>(p.D, dk_col, dp_col, desc_rows(ring_q + st * S::TILE), i > 0);
+            issue_commit(q_empty(st));
             if (i + 1 < n_items) {
                 wait(d_full(next), ((i + 1) / ST) & 1);
                 tc::fence_after_sync();
-                if (one) product_channels<T, DP>(dp_col, held_v, ring_d + next * S::TILE), tc::commit(dp_full);
-                __syncwarp();
+                issue_channels<T, DP>(p.D, dp_col, desc_channels(held_v), desc_channels(ring_d + next * S::TILE), dp_full);
             }
         }
-        if (one) tc::commit(done);
-        __syncwarp();
+        issue_commit(done);
         wait.drain(done, 0);
     }
     tc::fence_before_sync();
@@ -479,19 +459,17 @@ attention_grad_queries_tensor_kernel(const __grid_constant__ AttentionGradParams
         }
         __syncwarp();
     } else if (warp == S::MMA_WARP && n_items > 0) {
-        // ------------------------------------------------------------------ products, issued by one lane
-        const bool one = tc::elect_one();
+        // ------------------------------------------------------------------ products
         auto scores = [&](int i) {
             wait(k_full(i % KS), (i / KS) & 1);
             tc::fence_after_sync();
-            if (one) product_channels<T, DP>(tmem + (i & 1) * 128, held_q, ring_k + i % KS * S::TILE), tc::commit(s_full(i & 1));
-            __syncwarp();
+            issue_channels<T, DP>(p.D, tmem + (i & 1) * 128, desc_channels(held_q), desc_channels(ring_k + i % KS * S::TILE), s_full(i & 1));
         };
         auto gradients = [&](int i) {
             wait(v_full(i % VS), (i / VS) & 1);
             tc::fence_after_sync();
-            if (one) product_channels<T, DP>(dp_col, held_d, ring_v + i % VS * S::TILE), tc::commit(dp_full), tc::commit(v_empty(i % VS));
-            __syncwarp();
+            issue_channels<T, DP>(p.D, dp_col, desc_channels(held_d), desc_channels(ring_v + i % VS * S::TILE), dp_full);
+            issue_commit(v_empty(i % VS));
         };
         wait(held_full, 0);
         scores(0);
@@ -500,13 +478,12 @@ attention_grad_queries_tensor_kernel(const __grid_constant__ AttentionGradParams
         for (int i = 0; i < n_items; ++i) {
             wait(ds_ready, i & 1);
             tc::fence_after_sync();
-            if (one) product_rows<T, DP>(dq_col, dp_col, ring_k + i % KS * S::TILE, i > 0), tc::commit(k_empty(i % KS));
-            __syncwarp();
+            issue_rows<T, DP>(p.D, dq_col, dp_col, desc_rows(ring_k + i % KS * S::TILE), i > 0);
+            issue_commit(k_empty(i % KS));
             if (i + 1 < n_items) gradients(i + 1);
             if (i + 2 < n_items) scores(i + 2);       // over the scores that ds(i) was the last to need
         }
-        if (one) tc::commit(done);
-        __syncwarp();
+        issue_commit(done);
         wait.drain(done, 0);
     }
     tc::fence_before_sync();

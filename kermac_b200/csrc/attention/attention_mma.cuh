@@ -227,6 +227,33 @@ __device__ __forceinline__ int key_count(const int* lengths, long long stride, i
     return n < 0 ? 0 : n > M ? M : n;
 }
 
+// 2^x of a pair on the FP32 pipe, for x below 128: MUFU has 16 lanes per SM and is what a softmax waits for.  As ex2_poly2, x is rounded
+// to an integer n whose biased exponent stands in the low bits of t, and 2^(x - n) is a polynomial, here of degree 4: minimax on
+// [-1/2, 1/2], relative error 2.7e-6.  -infinity (and all below -127) gives exactly 0, NaN stays NaN.
+__device__ __forceinline__ u64 exp2_pair(u64 v) {
+    float x, y;
+    unpack2(v, x, y);
+    v = pack2(max_nan(x, -127.0f), max_nan(y, -127.0f));
+    const u64 magic = pack2(12583039.0f, 12583039.0f), t = add2(v, magic), f = sub2(v, sub2(t, magic));
+    u64 q = fma2(f, pack2(0x1.3997d6p-7f, 0x1.3997d6p-7f), pack2(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+    q     = fma2(q, f, pack2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    q     = fma2(q, f, pack2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    q     = fma2(q, f, pack2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    float a, b;
+    unpack2(t, a, b);
+    return mul2(q, pack2(__int_as_float(__float_as_int(a) << 23), __int_as_float(__float_as_int(b) << 23)));
+}
+// The same for pair `i` of a row: pairs that MUFU takes and pairs that the FP32 pipe takes, POLY of every 8.
+template <int POLY>
+__device__ __forceinline__ void exp2_shared(int i, u64 v, float& x, float& y) {
+    if ((i * POLY) % 8 < POLY) {
+        unpack2(exp2_pair(v), x, y);
+    } else {
+        unpack2(v, x, y);
+        x = ex2_approx(x), y = ex2_approx(y);
+    }
+}
+
 // Sum and maximum over the four lanes that hold one row.
 __device__ __forceinline__ float quad_max(float v) {
     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));

@@ -191,16 +191,23 @@ __global__ void __launch_bounds__(THREADS) attention_join_kernel(const Attention
     float total = 0.0f, x[8];
 #pragma unroll
     for (int c = 0; c < 8; ++c) x[c] = 0.0f;
-    for (int i = 0; i < p.parts; ++i) {
-        const float lse = p.part_lse[i * rows + row];
-        if (lse == -INFINITY) continue;      // a part without keys has written no sum
-        const float  weight = ex2_approx(lse - base);
-        const float* from   = p.part_o + (i * rows + row) * p.D;
-        total += weight;
+    for (int i0 = 0; i0 < p.parts; i0 += 32) {
+        // a lane's part; one without keys has weight 0 and has written no sum
+        const float mine = i0 + lane < p.parts ? ex2_approx(p.part_lse[(i0 + lane) * rows + row] - base) : 0.0f;
+        total += mine;
+        const int   many = min(32, p.parts - i0);
+        const float* from = p.part_o + (i0 * rows + row) * p.D + lane;
+#pragma unroll 4
+        for (int i = 0; i < many; ++i, from += rows * p.D) {
+            const float weight = __shfl_sync(0xffffffffu, mine, i);
+            if (weight == 0.0f) continue;
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-            if (c * 32 + lane < p.D) x[c] += weight * from[c * 32 + lane];
+            for (int c = 0; c < 8; ++c)
+                if (c * 32 + lane < p.D) x[c] += weight * from[c * 32];
+        }
     }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
     const int       h = static_cast<int>(row % p.H);
     const long long ln = row / p.H;
     const int       l = static_cast<int>(ln / p.N), n = static_cast<int>(ln - static_cast<long long>(l) * p.N);

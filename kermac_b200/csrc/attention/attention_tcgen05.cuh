@@ -22,15 +22,12 @@ __device__ __forceinline__ constexpr uint32_t instr_desc(int n, bool b_rows) {
     const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     return (1u << 4) | (f << 7) | (f << 10) | (b_rows ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
-// 16 channels of a tile as a K-major operand, from channel 16 * k on.
-__device__ __forceinline__ uint64_t desc_channels(uint32_t tile, int k) {
-    return tc::smem_desc_k_major_sw128(tile + (k >> 2) * TC_SLAB + (k & 3) * 32);
-}
-// 16 rows of a tile as an MN-major operand, from row 16 * k on: 64-channel blocks TC_SLAB apart (leading offset), groups of
-// eight rows 1024 bytes apart (stride offset).
-__device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int k) {
-    return static_cast<uint64_t>(((tile + k * 2048) & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(TC_SLAB >> 4) << 16) | (64ull << 32) |
-           (1ull << 46) | (2ull << 61);
+// A tile as a K-major operand (contraction over channels).
+__device__ __forceinline__ uint64_t desc_channels(uint32_t tile) { return tc::smem_desc_k_major_sw128(tile); }
+// A tile as an MN-major operand (contraction over rows): 64-channel blocks TC_SLAB apart (leading offset), groups of eight rows
+// 1024 bytes apart (stride offset).
+__device__ __forceinline__ uint64_t desc_rows(uint32_t tile) {
+    return static_cast<uint64_t>((tile & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(TC_SLAB >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
 // D (+)= A B, A and B in shared memory.
@@ -45,6 +42,57 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
 // The same with A in tensor memory, two of its columns in one of 32 bits.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
     tc::mma_bf16_a_tmem(d, a, b, idesc, accumulate);
+}
+
+// The products of two tiles, issued by one lane: called by a converged warp.  Descriptors are formed by the whole warp and the guard
+// is elect_one() itself, so that they stay in uniform registers.
+//
+// d (128 x 128) = A B^T over the D channels (those up to the next multiple of 16 are zeros in both).  The full width has code of its
+// own: with the test at every instruction train steps of 128 channels took 3 % longer.
+template <typename T, int DP>
+__device__ __forceinline__ void issue_channels(int D, uint32_t d, uint64_t a, uint64_t b, uint32_t done) {
+    if (D > DP - 16) {
+        if (tc::elect_one()) {
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                const uint64_t at = (k >> 2) * (TC_SLAB >> 4) + (k & 3) * 2;
+                mma_ss(d, a + at, b + at, instr_desc<T>(128, false), k > 0);
+            }
+            tc::commit(done);
+        }
+    } else {
+        if (tc::elect_one()) {
+#pragma unroll
+            for (int k = 0; k < DP / 16 - 1; ++k) {
+                const uint64_t at = (k >> 2) * (TC_SLAB >> 4) + (k & 3) * 2;
+                if (k * 16 < D) mma_ss(d, a + at, b + at, instr_desc<T>(128, false), k > 0);
+            }
+            tc::commit(done);
+        }
+    }
+    __syncwarp();
+}
+// d (128 x D, rounded up to 16) (+)= A B over the 128 rows of B; A in tensor memory, 32 columns from `a` on and 32 from a + 64
+template <typename T, int DP>
+__device__ __forceinline__ void issue_rows(int D, uint32_t d, uint32_t a, uint64_t b, bool accumulate) {
+    if (D > DP - 16) {
+        if (tc::elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                mma_ts(d, a + (k >> 2) * 64 + (k & 3) * 8, b + k * 128, instr_desc<T>(DP, true), accumulate || k > 0);
+        }
+    } else {
+        const uint32_t idesc = instr_desc<T>((D + 15) & ~15, true);
+        if (tc::elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mma_ts(d, a + (k >> 2) * 64 + (k & 3) * 8, b + k * 128, idesc, accumulate || k > 0);
+        }
+    }
+    __syncwarp();
+}
+__device__ __forceinline__ void issue_commit(uint32_t bar) {
+    if (tc::elect_one()) tc::commit(bar);
+    __syncwarp();
 }
 
 // One row (lane) of 32 columns.  The values may be used behind wait_loaded() of the same registers.
@@ -101,6 +149,32 @@ __device__ __forceinline__ void fill_row(char* tile, int r, const char* row, int
         uint4 x = make_uint4(0, 0, 0, 0);
         if (row != nullptr && c * 8 < D) x = *reinterpret_cast<const uint4*>(row + c * 16);
         *reinterpret_cast<uint4*>(tile + (c >> 3) * TC_SLAB + r * 128 + ((c & 7) ^ (r & 7)) * 16) = x;
+    }
+}
+
+// 32 columns of a finished row from column `first` on, times `by`: into out, or into its part.
+template <typename T>
+__device__ __forceinline__ void put_row_32(const AttentionParams& p, const Work& w, const Row& row, int first, const uint32_t* o, float by) {
+    if (p.parts > 1) {                       // D is a multiple of 8: 16-byte units
+        float* const to = p.part_o + ((((static_cast<long long>(w.part) * p.L + row.l) * p.N + row.n) * p.H) + row.h) * p.D + first;
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+            if (first + e < p.D)
+                *reinterpret_cast<float4*>(to + e) = make_float4(__uint_as_float(o[e]) * by, __uint_as_float(o[e + 1]) * by,
+                                                                 __uint_as_float(o[e + 2]) * by, __uint_as_float(o[e + 3]) * by);
+    } else if (p.vec_out) {
+        char* const to = p.out.ptr + (row.l * p.out.sl + row.n * p.out.sr + row.h * p.out.sh + first) * 2;
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+            uint32_t y[4];
+#pragma unroll
+            for (int f = 0; f < 4; ++f) y[f] = Type<T>::pair(__uint_as_float(o[e + 2 * f]) * by, __uint_as_float(o[e + 2 * f + 1]) * by);
+            if (first + e < p.D) *reinterpret_cast<uint4*>(to + e * 2) = make_uint4(y[0], y[1], y[2], y[3]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
+            put_pair<T>(p, w, row, first + e, __uint_as_float(o[e]) * by, __uint_as_float(o[e + 1]) * by);
     }
 }
 

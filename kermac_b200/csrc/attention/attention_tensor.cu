@@ -6,6 +6,10 @@
 //
 // The running maximum that weights are taken against may lag: it is raised, and O scaled, only where a row's maximum has grown by more
 // than 2^8, so that weights are at most 256 (the first tile sets it; after that it seldom happens).
+//
+// 4 x 4096 x 8192, 16 heads of 128, bf16: 887 us, 1.24 PFLOP/s at the 1.65 GHz that the power limit leaves; the products alone, without
+// a softmax, take 783.  A step (two tiles of rows, 128 keys) is 3440 cycles for products of 2048.  Tried: two threads a row (eight
+// warps a tile, 960 us), 2 to 5 of 8 pairs of exponentials on the FP32 pipe (952 to 1023), polling waits, K and V in one slot (no gain).
 #include <algorithm>
 
 #include "attention_tcgen05.cuh"
@@ -19,7 +23,7 @@ __device__ int g_attention_wait_expired = 0;
 template <int DP>
 struct TensorShape {
     static constexpr int TILE   = DP / 64 * TC_SLAB;
-    static constexpr int STAGES = DP == 128 ? 4 : 6;       // tiles of K and V under way
+    static constexpr int STAGES = DP == 128 ? 4 : 6;       // tiles of K and V under way (3 and 5: the same time)
     static constexpr int SMEM   = 1024 + (2 + STAGES) * TILE;
     static constexpr int GROUPS = 2;                       // row tiles, a warpgroup each
     static constexpr int LOAD_WARP = 4 * GROUPS, MMA_WARP = LOAD_WARP + 1, THREADS = 128 * (GROUPS + 1);
@@ -160,7 +164,7 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
                         total[e & 1] = add2(total[e & 1], pack2(lo, hi));
                         y[e] = Type<T>::pair(lo, hi);
                     }
-                    tmem_store32(s_col + j, y);
+                    tmem_store32(s_col + (j ? 64 : 0), y);
                 }
                 float a0, a1, a2, a3;
                 unpack2(total[0], a0, a1);
@@ -195,21 +199,7 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
                 tmem_wait_load();
                 tmem_loaded32(o);
                 if (!good) continue;
-                if (p.parts == 1 && p.vec_out) {
-                    char* const to = p.out.ptr + (row.l * p.out.sl + row.n * p.out.sr + row.h * p.out.sh + j) * 2;
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        uint32_t y[4];
-#pragma unroll
-                        for (int f = 0; f < 4; ++f)
-                            y[f] = Type<T>::pair(__uint_as_float(o[e + 2 * f]) * by, __uint_as_float(o[e + 2 * f + 1]) * by);
-                        if (j + e < p.D) *reinterpret_cast<uint4*>(to + e * 2) = make_uint4(y[0], y[1], y[2], y[3]);
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2)
-                        put_pair<T>(p, w, row, j + e, __uint_as_float(o[e]) * by, __uint_as_float(o[e + 1]) * by);
-                }
+                put_row_32<T>(p, w, row, j, o, by);
             }
         } else if (t < groups && at < w.rows) {          // no keys
             const Row row = find_row(p, w, at);
@@ -238,17 +228,9 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
         }
         __syncwarp();
     } else if (warp == S::MMA_WARP) {
-        // ------------------------------------------------------------------ products, issued by one lane
-        constexpr uint32_t qk = instr_desc<T>(128, false), pv = instr_desc<T>(DP, true);
-        const bool one = tc::elect_one();
+        // ------------------------------------------------------------------ products
         auto scores = [&](int t, int st) {
-            if (one) {
-#pragma unroll
-                for (int k = 0; k < DP / 16; ++k)
-                    mma_ss(tmem + S::S_COL + t * 128, desc_channels(base + t * S::TILE, k), desc_channels(ring + st * S::TILE, k), qk, k > 0);
-                tc::commit(s_full(t));
-            }
-            __syncwarp();
+            issue_channels<T, DP>(p.D, tmem + S::S_COL + t * 128, desc_channels(base + t * S::TILE), desc_channels(ring + st * S::TILE), s_full(t));
         };
         if (n_tiles > 0) {
             wait(full(0), 0);
@@ -257,31 +239,22 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
                 tc::fence_after_sync();
                 scores(t, 0);
             }
-            if (one) tc::commit(empty(0));
+            issue_commit(empty(0));
             for (int i = 0; i < n_tiles; ++i) {
-                const int jv = 2 * i + 1, jk = 2 * i + 2;
-                wait(full(jv % S::STAGES), (jv / S::STAGES) & 1);
+                const int jv = 2 * i + 1, jk = 2 * i + 2, sv = jv % S::STAGES, sk = jk % S::STAGES;
+                wait(full(sv), (jv / S::STAGES) & 1);
                 for (int t = 0; t < groups; ++t) {
                     wait(p_full(t), i & 1);
                     tc::fence_after_sync();
-                    if (one) {
-#pragma unroll
-                        for (int k = 0; k < TC_ROWS / 16; ++k)
-                            mma_ts(tmem + S::O_COL + t * DP, tmem + S::S_COL + t * 128 + k * 8, desc_rows(ring + jv % S::STAGES * S::TILE, k), pv,
-                                   i > 0 || k > 0);
-                        if (i == n_tiles - 1) tc::commit(o_full(t));
-                    }
-                    __syncwarp();
+                    issue_rows<T, DP>(p.D, tmem + S::O_COL + t * DP, tmem + S::S_COL + t * 128, desc_rows(ring + sv * S::TILE), i > 0);
+                    if (t == groups - 1) issue_commit(empty(sv));
+                    if (i == n_tiles - 1) issue_commit(o_full(t));
                     if (i + 1 < n_tiles) {
-                        if (t == 0) wait(full(jk % S::STAGES), (jk / S::STAGES) & 1);
-                        scores(t, jk % S::STAGES);
+                        if (t == 0) wait(full(sk), (jk / S::STAGES) & 1);
+                        scores(t, sk);
+                        if (t == groups - 1) issue_commit(empty(sk));
                     }
                 }
-                if (one) {
-                    tc::commit(empty(jv % S::STAGES));
-                    if (i + 1 < n_tiles) tc::commit(empty(jk % S::STAGES));
-                }
-                __syncwarp();
             }
             // every product has ended before tensor memory is given back
             for (int t = 0; t < groups; ++t) drain(o_full(t), 0);
