@@ -1,6 +1,6 @@
 // Attention of few 16-bit queries (decoding steps): bound by reading the keys and values once.
 //
-// Up to 32 rows share a block; its four warps take tiles of 32 keys in turn, each with a ring of its own that TMA fills, so that no
+// Up to 16 rows share a block; its warps take tiles of 32 keys in turn, each with a ring of its own that TMA fills, so that no
 // warp waits for another, and add up at the end.  Products are transposed, S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16): the rows
 // are the narrow side of an instruction, eight at a time, where the other way round 16 rows would be computed for one
 // token.  Q stays in registers; P^T passes from accumulator to operand layout by movmatrix.
@@ -17,11 +17,14 @@ namespace {
 
 __device__ int g_attention_few_wait_expired = 0;
 
+#ifndef FEW_WARPS
+#define FEW_WARPS 4
+#endif
 constexpr int FEW_KEYS = 32;
 
 template <int DP, int NR>
 struct FewShape {
-    static constexpr int ROWS   = 8 * NR, STAGES = 3;
+    static constexpr int ROWS   = 8 * NR, STAGES = 3, WARPS = FEW_WARPS, THREADS = 32 * WARPS;
     static constexpr int SLAB   = FEW_KEYS * 128, TILE = DP / 64 * SLAB;      // one tile of K or V
     static constexpr int RING   = STAGES * 2 * TILE;                          // of one warp
     static constexpr int W      = DP + 2;                                     // channels, maximum and sum of a row
@@ -46,8 +49,9 @@ __device__ __forceinline__ float column_sum(float v) {
 }
 
 template <typename T, int DP, int NR>
-__global__ void __launch_bounds__(THREADS) attention_few_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ TensorMaps maps) {
+__global__ void __launch_bounds__(32 * FEW_WARPS) attention_few_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ TensorMaps maps) {
     typedef FewShape<DP, NR> S;
+    constexpr int WARPS = S::WARPS, THREADS = S::THREADS;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long s_bars[WARPS * S::STAGES];
     __shared__ int s_expired;
@@ -254,16 +258,12 @@ int launch_few(const AttentionParams& p, const TensorMaps& maps, cudaStream_t st
     if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute")) return rc;
     unsigned blocks;
     if (int rc = count_blocks(p, &blocks)) return rc;
-    return cuda_status(launch_overlapped(kernel, dim3(blocks), THREADS, smem, st, p, maps), "attention_few_kernel");
+    return cuda_status(launch_overlapped(kernel, dim3(blocks), FewShape<DP, NR>::THREADS, smem, st, p, maps), "attention_few_kernel");
 }
 template <typename T>
 int launch_few_type(const AttentionParams& p, const TensorMaps& maps, int rows, cudaStream_t st) {
-    if (p.D <= 64) {
-        if (rows <= 8) return launch_few<T, 64, 1>(p, maps, st);
-        return rows <= 16 ? launch_few<T, 64, 2>(p, maps, st) : launch_few<T, 64, 4>(p, maps, st);
-    }
-    if (rows <= 8) return launch_few<T, 128, 1>(p, maps, st);
-    return rows <= 16 ? launch_few<T, 128, 2>(p, maps, st) : launch_few<T, 128, 4>(p, maps, st);
+    if (p.D <= 64) return rows <= 8 ? launch_few<T, 64, 1>(p, maps, st) : launch_few<T, 64, 2>(p, maps, st);
+    return rows <= 8 ? launch_few<T, 128, 1>(p, maps, st) : launch_few<T, 128, 2>(p, maps, st);
 }
 
 }  // namespace

@@ -146,6 +146,7 @@ __global__ void __launch_bounds__(THREADS) attention_grad_queries_kernel(const A
     const int tiles = (p.N + S::ROWS - 1) / S::ROWS;
     int       block = blockIdx.x;
     const int n0 = block % tiles * S::ROWS; block /= tiles;
+    const int split = block % p.q_splits;   block /= p.q_splits;
     const int h = block % p.H, l = block / p.H, hk = h / p.G;
     const int   count  = key_count(p.lengths, p.lengths_stride, l, p.M);
     const int   kl     = p.kv_batch == 1 ? 0 : l;
@@ -153,9 +154,13 @@ __global__ void __launch_bounds__(THREADS) attention_grad_queries_kernel(const A
 
     copy_rows<T, DP>(held_q, head_of<T>(p.q, l, h), p.q.sr, n0, p.N, S::ROWS, p.D, p.vec, threadIdx.x, THREADS);
     copy_rows<T, DP>(held_d, head_of<T>(p.dout, l, h), p.dout.sr, n0, p.N, S::ROWS, p.D, p.vec, threadIdx.x, THREADS);
+    // this block's piece of the keys
+    const int key_tiles = (count + S::STREAM - 1) / S::STREAM;
+    const int i_first = static_cast<int>(static_cast<long long>(key_tiles) * split / p.q_splits);
+    const int i_end   = static_cast<int>(static_cast<long long>(key_tiles) * (split + 1) / p.q_splits);
     auto load = [&](int i) {
         const int first = i * S::STREAM;
-        if (first < count) {
+        if (i < i_end) {
             T* const dst = reinterpret_cast<T*>(ring + (i & 1) * 2 * S::MOVED);
             copy_rows<T, DP>(dst, head_of<T>(p.k, kl, hk), p.k.sr, first, count, S::STREAM, p.D, p.vec, threadIdx.x, THREADS);
             copy_rows<T, DP>(dst + S::STREAM * TL::LD, head_of<T>(p.v, kl, hk), p.v.sr, first, count, S::STREAM, p.D, p.vec, threadIdx.x,
@@ -173,8 +178,8 @@ __global__ void __launch_bounds__(THREADS) attention_grad_queries_kernel(const A
 #pragma unroll
     for (int c = 0; c < CT; ++c) dq[c][0] = dq[c][1] = dq[c][2] = dq[c][3] = 0.0f;
 
-    load(0);
-    for (int i = 0; i * S::STREAM < count; ++i) {
+    load(i_first);
+    for (int i = i_first; i < i_end; ++i) {
         load(i + 1);
         copy_wait<1>();
         __syncthreads();
@@ -196,8 +201,9 @@ __global__ void __launch_bounds__(THREADS) attention_grad_queries_kernel(const A
         __syncthreads();
     }
     copy_wait<0>();
-    // slice l of a broadcast q's partial sums
-    float* const part = p.q_slices > 1 ? p.dq_part + static_cast<long long>(l) * p.N * p.H * p.D : nullptr;
+    // partial sums [slice][entry of q][n][h][D]: a broadcast q has one entry and a slice for each l and piece
+    const bool   one_q = p.q_slices > p.q_splits;
+    float* const part = p.q_slices > 1 ? p.dq_part + static_cast<long long>(one_q ? l * p.q_splits + split : split * p.L) * p.N * p.H * p.D : nullptr;
     const float  by = p.scale / factor;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -205,7 +211,7 @@ __global__ void __launch_bounds__(THREADS) attention_grad_queries_kernel(const A
         if (n >= p.N) continue;
 #pragma unroll
         for (int c = 0; c < CT; ++c)
-            put_grad<T>(p.dq, part, part ? 0 : l, n, h, p.N, p.H, p.D, c * 8 + 2 * t, dq[c][2 * r] * by, dq[c][2 * r + 1] * by);
+            put_grad<T>(p.dq, part, one_q ? 0 : l, n, h, p.N, p.H, p.D, c * 8 + 2 * t, dq[c][2 * r] * by, dq[c][2 * r + 1] * by);
     }
 }
 
@@ -223,6 +229,7 @@ __global__ void __launch_bounds__(THREADS) attention_delta_kernel(const Attentio
     // `lanes` lanes a row, a 16-byte unit each in turn, so a warp takes 32 / lanes rows at a time
     constexpr int CHUNK = Type<T>::CHUNK;
     const int units = (p.D + CHUNK - 1) / CHUNK, lanes = units > 16 ? 32 : units > 8 ? 16 : 8, sub = lane & (lanes - 1);
+#pragma unroll 4
     for (int r = (warp * 32 + lane) / lanes; r < ATT_PEAK_ROWS; r += THREADS / lanes) {     // uniform: a multiple of lanes rows
         const int n = group * ATT_PEAK_ROWS + r;
         float sum = 0.0f;
@@ -288,7 +295,7 @@ int launch_grad(const AttentionGradParams& p, cudaStream_t st) {
     int rc = cuda_status(cudaFuncSetAttribute(keys, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "cudaFuncSetAttribute");
     if (!rc) rc = cuda_status(cudaFuncSetAttribute(queries, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "cudaFuncSetAttribute");
     const long long kb = ceil_div_ll(p.M, S::ROWS) * p.kv_slices * p.Hk * p.kv_batch;
-    const long long qb = ceil_div_ll(p.N, S::ROWS) * p.H * p.L;
+    const long long qb = ceil_div_ll(p.N, S::ROWS) * p.q_splits * p.H * p.L;
     if (!rc) rc = check_blocks(kb > qb ? kb : qb);
     if (!rc && kb)
         rc = cuda_status(launch_overlapped(keys, dim3(static_cast<unsigned>(kb), DP / (S::CT * 8)), THREADS, S::SMEM, st, p),

@@ -1,7 +1,8 @@
 // Gradient of the attention of 16-bit tensors on the tensor cores (tcgen05), head widths up to 128.
 //
-// Two kernels as in attention_grad_rows.cu: a block holds 128 keys and streams query tiles (dk, dv), or holds 128 queries and streams
-// key tiles (dq).  Scores and dout v^T are in tensor memory, the weights and their gradients are written back over them as
+// Two kinds of blocks, like the two kernels of attention_grad_rows.cu: one holds 128 keys and streams query tiles (dk, dv), one holds 128 queries and streams
+// key tiles (dq).  One launch has both, the longer ones (of keys) first, so that the SMs that have finished those go on with the others
+// (two launches: a training step of 8 x 512 x 1030 waited twice for its last blocks, 140 of 195 us).  Scores and dout v^T are in tensor memory, the weights and their gradients are written back over them as
 // 16-bit operands.  The keys' kernel computes both transposed, so that its operands need no transposition either: a
 // lane is a key there and a query in the other kernel.
 //
@@ -76,9 +77,9 @@ __device__ __forceinline__ void put_grad_32(const Heads& to, float* part, bool v
     }
 }
 
+// dk and dv of 128 keys.
 template <typename T, int DP>
-__global__ void __launch_bounds__(GradTensorShape<DP>::BLOCK, 1)
-attention_grad_keys_tensor_kernel(const __grid_constant__ AttentionGradParams p, const __grid_constant__ GradMaps maps) {
+__device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, const GradMaps& maps, int block) {
     typedef GradTensorShape<DP> S;
     constexpr int ST = S::KEYS_STAGES;
     extern __shared__ unsigned char smem_raw[];
@@ -106,12 +107,10 @@ attention_grad_keys_tensor_kernel(const __grid_constant__ AttentionGradParams p,
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tc::fence_smem_to_async();
     }
-    after_previous_grid();
     if (warp == S::MMA_WARP) tc::tmem_alloc(smem_addr(&s_tmem), 512);
 
     // (key tile, slice, key head, batch entry of k and v)
     const int tiles = (p.M + TC_ROWS - 1) / TC_ROWS;
-    int       block = blockIdx.x;
     const int key0 = block % tiles * TC_ROWS; block /= tiles;
     const int slice = block % p.kv_slices;    block /= p.kv_slices;
     const int hk = block % p.Hk, kl = block / p.Hk;
@@ -311,9 +310,9 @@ attention_grad_keys_tensor_kernel(const __grid_constant__ AttentionGradParams p,
     if (threadIdx.x == 0 && s_expired) g_attention_grad_wait_expired = 1;
 }
 
+// dq of 128 queries of a head.
 template <typename T, int DP>
-__global__ void __launch_bounds__(GradTensorShape<DP>::BLOCK, 1)
-attention_grad_queries_tensor_kernel(const __grid_constant__ AttentionGradParams p, const __grid_constant__ GradMaps maps) {
+__device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p, const GradMaps& maps, int block) {
     typedef GradTensorShape<DP> S;
     constexpr int KS = S::K_STAGES, VS = S::V_STAGES;
     extern __shared__ unsigned char smem_raw[];
@@ -337,11 +336,9 @@ attention_grad_queries_tensor_kernel(const __grid_constant__ AttentionGradParams
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tc::fence_smem_to_async();
     }
-    after_previous_grid();
     if (warp == S::MMA_WARP) tc::tmem_alloc(smem_addr(&s_tmem), 512);
 
     const int tiles = (p.N + TC_ROWS - 1) / TC_ROWS;
-    int       block = blockIdx.x;
     const int n0 = block % tiles * TC_ROWS; block /= tiles;
     const int h = block % p.H, l = block / p.H, hk = h / p.G;
     const int kl = p.kv_batch == 1 ? 0 : l;
@@ -423,7 +420,7 @@ attention_grad_queries_tensor_kernel(const __grid_constant__ AttentionGradParams
             tc::fence_after_sync();
         }
         const bool   good = n < p.N && *reinterpret_cast<volatile int*>(&s_expired) == 0;
-        float* const part = p.q_slices > 1 ? p.dq_part + static_cast<long long>(l) * p.N * p.H * p.D : nullptr;
+        float* const part = p.q_slices > 1 ? p.dq_part + static_cast<long long>(l) * p.N * p.H * p.D : nullptr;    // q_splits is 1
 #pragma unroll
         for (int j = 0; j < DP / 2; j += 32) {
             const int first = half * (DP / 2) + j;
@@ -494,23 +491,26 @@ attention_grad_queries_tensor_kernel(const __grid_constant__ AttentionGradParams
 }
 
 template <typename T, int DP>
+__global__ void __launch_bounds__(GradTensorShape<DP>::BLOCK, 1)
+attention_grad_tensor_kernel(const __grid_constant__ AttentionGradParams p, const __grid_constant__ GradMaps maps, const int key_blocks) {
+    after_previous_grid();
+    if (static_cast<int>(blockIdx.x) < key_blocks)
+        gradient_of_keys<T, DP>(p, maps, blockIdx.x);
+    else
+        gradient_of_queries<T, DP>(p, maps, blockIdx.x - key_blocks);
+}
+
+template <typename T, int DP>
 int launch_grad_tensor(const AttentionGradParams& p, const GradMaps& maps, cudaStream_t st) {
     typedef GradTensorShape<DP> S;
-    constexpr int keys_smem = S::at_least_half(S::KEYS_SMEM), queries_smem = S::at_least_half(S::QUERIES_SMEM);
-    static_assert(keys_smem <= 227 * 1024 && queries_smem <= 227 * 1024, "more shared memory than a block has");
-    auto* const keys    = &attention_grad_keys_tensor_kernel<T, DP>;
-    auto* const queries = &attention_grad_queries_tensor_kernel<T, DP>;
-    int rc = cuda_status(cudaFuncSetAttribute(keys, cudaFuncAttributeMaxDynamicSharedMemorySize, keys_smem), "cudaFuncSetAttribute");
-    if (!rc) rc = cuda_status(cudaFuncSetAttribute(queries, cudaFuncAttributeMaxDynamicSharedMemorySize, queries_smem), "cudaFuncSetAttribute");
+    constexpr int smem = S::at_least_half(S::KEYS_SMEM > S::QUERIES_SMEM ? S::KEYS_SMEM : S::QUERIES_SMEM);
+    static_assert(smem <= 227 * 1024, "more shared memory than a block has");
+    auto* const kernel = &attention_grad_tensor_kernel<T, DP>;
+    if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute")) return rc;
     const long long kb = ceil_div_ll(p.M, TC_ROWS) * p.kv_slices * p.Hk * p.kv_batch, qb = ceil_div_ll(p.N, TC_ROWS) * p.H * p.L;
-    if (!rc && std::max(kb, qb) > 0x7fffffffLL) rc = fail(KM_ERR_TOO_LARGE, "attention: more than 2^31 - 1 blocks");
-    if (!rc)
-        rc = cuda_status(launch_overlapped(keys, dim3(static_cast<unsigned>(kb)), S::BLOCK, keys_smem, st, p, maps),
-                         "attention_grad_keys_tensor_kernel");
-    if (!rc)
-        rc = cuda_status(launch_overlapped(queries, dim3(static_cast<unsigned>(qb)), S::BLOCK, queries_smem, st, p, maps),
-                         "attention_grad_queries_tensor_kernel");
-    return rc;
+    if (kb + qb > 0x7fffffffLL) return fail(KM_ERR_TOO_LARGE, "attention: more than 2^31 - 1 blocks");
+    return cuda_status(launch_overlapped(kernel, dim3(static_cast<unsigned>(kb + qb)), S::BLOCK, smem, st, p, maps, static_cast<int>(kb)),
+                       "attention_grad_tensor_kernel");
 }
 
 }  // namespace

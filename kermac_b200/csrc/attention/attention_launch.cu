@@ -126,7 +126,7 @@ bool tma_rows_ok(const KmHeads& t, int rows, int n_heads, int type, int d) {
            (n_heads <= 1 || (t.stride_head > 0 && t.stride_head < most)) && t.stride_l < most;
 }
 
-// The kernels of the forward pass.  TENSOR: 256 rows on tcgen05.  FEW: 8, 16 or 32 rows whose keys four warps share out, fed by TMA.
+// The kernels of the forward pass.  TENSOR: 256 rows on tcgen05.  FEW: 8 or 16 rows whose keys a few warps share out, fed by TMA.
 // For what these two do not take: SCALAR_FEW, 16 rows in the manner of FEW, and ROWS, 64 rows that share key tiles.
 enum Kernel { TENSOR, FEW, SCALAR_FEW, ROWS };
 struct Form {
@@ -143,11 +143,11 @@ struct Plan {
     long long bytes;
 };
 
-Form choose_form(long long rows, bool tma_ok, int d) {
-    if (tma_ok && rows > 64) return {TENSOR, ATT_TENSOR_ROWS, 1, 512};
-    if (tma_ok) return {FEW, rows <= 8 ? 8 : rows <= 16 ? 16 : ATT_FEW_MOST, d <= 64 ? 2 : 1, 256};
+Form choose_form(long long rows, bool tma_ok, int type, int d) {
+    if (tma_ok && rows > 16) return {TENSOR, ATT_TENSOR_ROWS, 1, 256};
+    if (tma_ok) return {FEW, rows <= 8 ? 8 : 16, d <= 64 ? 2 : 1, 256};
     if (rows <= ATT_FEW_ROWS) return {SCALAR_FEW, ATT_FEW_ROWS, 1, 256};
-    return {ROWS, ATT_TILE_ROWS, 2, 512};
+    return {ROWS, ATT_TILE_ROWS, type == ATT_F32 ? 4 : 2, 256};
 }
 
 // How many pieces the keys of `blocks` blocks are split into: as many as the SMs hold at once, no piece shorter than `least` keys.
@@ -183,8 +183,8 @@ Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool scratch) {
                                           : own_ok;
     p.vec_out = rows_aligned(a.out, a.type, a.d);
     const long long own_rows = static_cast<long long>(p.N) * p.G, prefix_rows = own_rows * p.L;
-    plan.own    = choose_form(own_rows, own_ok, p.D);
-    plan.prefix = choose_form(prefix_rows, prefix_ok, p.D);
+    plan.own    = choose_form(own_rows, own_ok, a.type, p.D);
+    plan.prefix = choose_form(prefix_rows, prefix_ok, a.type, p.D);
     if (p.M > 0 || p.P == 0) {
         p.own_tiles  = static_cast<int>(ceil_div_ll(own_rows, plan.own.rows));
         p.own_splits = scratch ? pieces(static_cast<long long>(p.own_tiles) * p.L * p.Hk, p.M, plan.own.per_sm, plan.own.least) : 1;
@@ -270,19 +270,23 @@ GradPlan plan_grad(const KmAttentionArgs& a) {
     p.vec_grad = rows_aligned(a.grad_q, a.type, a.d) && rows_aligned(a.grad_k, a.type, a.d) && rows_aligned(a.grad_v, a.type, a.d);
     plan.tensor = a.d <= 128 && tma_rows_ok(a.q, a.n, a.heads, a.type, a.d) && tma_rows_ok(a.grad_out, a.n, a.heads, a.type, a.d) &&
                   tma_rows_ok(a.k, a.m, a.key_heads, a.type, a.d) && tma_rows_ok(a.v, a.m, a.key_heads, a.type, a.d);
-    p.q_slices = a.q_batch == 1 && a.l > 1 ? a.l : 1;
+    // The sum over keys of a query tile is split where the query tiles alone do not fill the SMs (not on the tensor cores, where
+    // the blocks of both sums run side by side and a piece would be a few tiles).
+    p.q_splits = plan.tensor ? 1 : pieces(ceil_div_ll(a.n, ATT_GRAD_ROWS) * a.heads * a.l, a.m, 2, 128);
+    if (static_cast<long long>(p.q_splits) * a.l * a.n * a.heads * a.d > (MOST_SCRATCH >> 3)) p.q_splits = 1;
+    p.q_slices = (a.q_batch == 1 && a.l > 1 ? a.l : 1) * p.q_splits;
     p.kv_batch = a.kv_batch;
     // The sum over queries of a key tile is split where the key tiles alone do not fill the SMs.
     const long long tiles = ceil_div_ll(a.m, plan.tensor ? ATT_GRAD_TENSOR_ROWS : ATT_GRAD_ROWS) * a.key_heads * a.kv_batch;
     const long long sum   = static_cast<long long>(a.kv_batch == 1 ? a.l : 1) * p.G * a.n;
-    p.kv_slices = pieces(tiles, sum, plan.tensor ? 1 : 2, 512);
+    p.kv_slices = plan.tensor ? pieces(tiles, sum, 1, 512) : pieces(tiles, sum, 2, 128);
     if (static_cast<long long>(p.kv_slices) * a.kv_batch * a.m * a.key_heads * a.d > (MOST_SCRATCH >> 3)) p.kv_slices = 1;
     plan.delta = round4(static_cast<long long>(a.l) * a.heads * a.n);
     if (a.type == ATT_F16) {
         p.peak_count = static_cast<int>(ceil_div_ll(a.n, ATT_PEAK_ROWS));
         plan.peaks   = round4(static_cast<long long>(a.l) * a.heads * p.peak_count);
     }
-    if (p.q_slices > 1) plan.dq = round4(static_cast<long long>(p.q_slices) * a.n * a.heads * a.d);
+    if (p.q_slices > 1) plan.dq = round4(static_cast<long long>(p.q_slices) * a.q_batch * a.n * a.heads * a.d);
     if (p.kv_slices > 1) plan.dkv = round4(static_cast<long long>(p.kv_slices) * a.kv_batch * a.m * a.key_heads * a.d);
     return plan;
 }
@@ -317,7 +321,7 @@ int gradient(const KmAttentionArgs* a, void* stream) {
     if (plan.dkv) p.dk_part = at, p.dv_part = at + plan.dkv;
     rc = attention_delta_launch(p, a->type, st);
     if (!rc) rc = plan.tensor ? attention_grad_tensor_launch(p, a->type, st) : attention_grad_rows_launch(p, a->type, st);
-    if (!rc && p.q_slices > 1) rc = attention_reduce_launch(p.dq_part, p.q_slices, p.dq, 1, p.N, p.H, p.D, a->type, st);
+    if (!rc && p.q_slices > 1) rc = attention_reduce_launch(p.dq_part, p.q_slices, p.dq, a->q_batch, p.N, p.H, p.D, a->type, st);
     if (!rc && p.kv_slices > 1) rc = attention_reduce_launch(p.dk_part, p.kv_slices, p.dk, p.kv_batch, p.M, p.Hk, p.D, a->type, st);
     if (!rc && p.kv_slices > 1) rc = attention_reduce_launch(p.dv_part, p.kv_slices, p.dv, p.kv_batch, p.M, p.Hk, p.D, a->type, st);
     return rc;

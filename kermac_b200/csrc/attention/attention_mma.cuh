@@ -2,7 +2,9 @@
 //
 // 16-bit inputs: m16n8k16 with fp32 sums.  float32 inputs: every value is split into a tf32 head and a tf32 remainder and
 // each product is three m16n8k8 (head x head and the two mixed ones): what is dropped is below 2^-22 of a product.  The tensor
-// cores add into their accumulator with the low bits cut off, so a float32 sum is kept in chains of one tile, added up in fp32.
+// cores add into their accumulator with the low bits cut off, so the heads' products are summed in chains of 16 terms that are
+// added up in fp32, and the mixed products, which are 2^-11 of them, in an accumulator of their own (one chain for all of
+// both: gradients 1.3e-6 off where fp32 products give 0.6e-6).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -111,23 +113,39 @@ __device__ __forceinline__ void product_nt(float (&s)[NT][4], const T* a, const 
         const int g = lane >> 2, t = lane & 3;
         const float* pa = a + g * LD + t;
         const float* pb = b + g * LD + t;
-#pragma unroll 4
-        for (int k = 0; k < DP / 8; ++k) {
-            uint32_t head[4], rest[4];
-            split_tf32(pa[k * 8], head[0], rest[0]);
-            split_tf32(pa[k * 8 + 8 * LD], head[1], rest[1]);
-            split_tf32(pa[k * 8 + 4], head[2], rest[2]);
-            split_tf32(pa[k * 8 + 8 * LD + 4], head[3], rest[3]);
+        float mixed[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mixed[j][0] = mixed[j][1] = mixed[j][2] = mixed[j][3] = 0.0f;
+#pragma unroll 2
+        for (int k = 0; k < DP / 8; k += 2) {
+            uint32_t head[2][4], rest[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                split_tf32(pa[(k + i) * 8], head[i][0], rest[i][0]);
+                split_tf32(pa[(k + i) * 8 + 8 * LD], head[i][1], rest[i][1]);
+                split_tf32(pa[(k + i) * 8 + 4], head[i][2], rest[i][2]);
+                split_tf32(pa[(k + i) * 8 + 8 * LD + 4], head[i][3], rest[i][3]);
+            }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                uint32_t bh[2], br[2];
-                split_tf32(pb[j * 8 * LD + k * 8], bh[0], br[0]);
-                split_tf32(pb[j * 8 * LD + k * 8 + 4], bh[1], br[1]);
-                mma_tf32(s[j], rest, bh);
-                mma_tf32(s[j], head, br);
-                mma_tf32(s[j], head, bh);
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t bh[2], br[2];
+                    split_tf32(pb[j * 8 * LD + (k + i) * 8], bh[0], br[0]);
+                    split_tf32(pb[j * 8 * LD + (k + i) * 8 + 4], bh[1], br[1]);
+                    mma_tf32(mixed[j], rest[i], bh);
+                    mma_tf32(mixed[j], head[i], br);
+                    mma_tf32(sum, head[i], bh);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[j][e] += sum[e];
             }
         }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][e] += mixed[j][e];
     }
 }
 
@@ -167,18 +185,24 @@ __device__ __forceinline__ void product_nn(float (&o)[CT][4], const float (&p)[N
         const float* pb = b + 2 * t * LD + g;
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float mixed[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                uint32_t bh[2], br[2];
-                split_tf32(pb[j * 8 * LD + c * 8], bh[0], br[0]);
-                split_tf32(pb[j * 8 * LD + LD + c * 8], bh[1], br[1]);
-                mma_tf32(sum, rest[j], bh);
-                mma_tf32(sum, head[j], br);
-                mma_tf32(sum, head[j], bh);
+            for (int j = 0; j < NT; j += 2) {
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = j; i < j + 2 && i < NT; ++i) {
+                    uint32_t bh[2], br[2];
+                    split_tf32(pb[i * 8 * LD + c * 8], bh[0], br[0]);
+                    split_tf32(pb[i * 8 * LD + LD + c * 8], bh[1], br[1]);
+                    mma_tf32(mixed, rest[i], bh);
+                    mma_tf32(mixed, head[i], br);
+                    mma_tf32(sum, head[i], bh);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[c][e] += sum[e];
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[c][i] += sum[i];
+            for (int e = 0; e < 4; ++e) o[c][e] += mixed[e];
         }
     }
 }
@@ -225,33 +249,6 @@ __device__ __forceinline__ int key_count(const int* lengths, long long stride, i
     if (!lengths) return M;
     const int n = lengths[l * stride];
     return n < 0 ? 0 : n > M ? M : n;
-}
-
-// 2^x of a pair on the FP32 pipe, for x below 128: MUFU has 16 lanes per SM and is what a softmax waits for.  As ex2_poly2, x is rounded
-// to an integer n whose biased exponent stands in the low bits of t, and 2^(x - n) is a polynomial, here of degree 4: minimax on
-// [-1/2, 1/2], relative error 2.7e-6.  -infinity (and all below -127) gives exactly 0, NaN stays NaN.
-__device__ __forceinline__ u64 exp2_pair(u64 v) {
-    float x, y;
-    unpack2(v, x, y);
-    v = pack2(max_nan(x, -127.0f), max_nan(y, -127.0f));
-    const u64 magic = pack2(12583039.0f, 12583039.0f), t = add2(v, magic), f = sub2(v, sub2(t, magic));
-    u64 q = fma2(f, pack2(0x1.3997d6p-7f, 0x1.3997d6p-7f), pack2(0x1.ca1440p-5f, 0x1.ca1440p-5f));
-    q     = fma2(q, f, pack2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-    q     = fma2(q, f, pack2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-    q     = fma2(q, f, pack2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-    float a, b;
-    unpack2(t, a, b);
-    return mul2(q, pack2(__int_as_float(__float_as_int(a) << 23), __int_as_float(__float_as_int(b) << 23)));
-}
-// The same for pair `i` of a row: pairs that MUFU takes and pairs that the FP32 pipe takes, POLY of every 8.
-template <int POLY>
-__device__ __forceinline__ void exp2_shared(int i, u64 v, float& x, float& y) {
-    if ((i * POLY) % 8 < POLY) {
-        unpack2(exp2_pair(v), x, y);
-    } else {
-        unpack2(v, x, y);
-        x = ex2_approx(x), y = ex2_approx(y);
-    }
 }
 
 // Sum and maximum over the four lanes that hold one row.

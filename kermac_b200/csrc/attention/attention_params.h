@@ -48,7 +48,8 @@ struct AttentionGradParams {
     // grad_reduce adds up, where a broadcast input's gradient is a sum over the batch or the sum is split.
     Heads dq, dk, dv;
     float *dq_part, *dk_part, *dv_part;
-    int   q_slices;                      // 1, or L for a broadcast q
+    int   q_slices;                      // partial sums of dq: q_splits, times L for a broadcast q
+    int   q_splits;                      // pieces of the sum over keys
     int   kv_batch;                      // batch entries of k and v: 1 or L
     int   kv_slices;                     // pieces of the sum over (l of a broadcast k, head of the group, query tile)
     int   vec;                           // rows of q, k, v and dout can be read 16 bytes at a time
@@ -62,8 +63,7 @@ enum { ATT_F32 = KM_TYPE_FLOAT32, ATT_BF16 = KM_TYPE_BFLOAT16, ATT_F16 = KM_TYPE
 int  attention_rows_launch(const AttentionParams& p, int type, bool few, cudaStream_t st);
 constexpr int ATT_FEW_ROWS = 16, ATT_TILE_ROWS = 64;
 int  attention_join_launch(const AttentionParams& p, int type, cudaStream_t st);
-// attention_few.cu: 16-bit types, D a multiple of 8 up to 128, rows that TMA can copy; up to ATT_FEW_MOST rows a block (8, 16 or 32).
-constexpr int ATT_FEW_MOST = 32;
+// attention_few.cu: 16-bit types, D a multiple of 8 up to 128, rows that TMA can copy; 8 or 16 rows a block.
 int  attention_few_launch(const AttentionParams& p, int type, int rows, cudaStream_t st);
 int  attention_few_take_wait_flag();
 // Blocks of a forward launch: every (key head, row tile, piece) of both sets of keys.
