@@ -57,23 +57,43 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
     for (int d = 0; d < DP / 64; ++d) tma_load_rows(dst + d * TC_SLAB, map, d * 64, row, head, l, bar);
 }
 
-// Writes columns [first, first + 32) of a row's sums, times `by`.
-template <typename T>
-__device__ __forceinline__ void put_grad_32(const Heads& to, float* part, bool vec, int l, int row, int h, int rows, int heads, int D,
-                                            int first, const uint32_t* x, float by) {
-    if (vec && !part) {
-        char* const at = to.ptr + (l * to.sl + row * to.sr + h * to.sh + first) * 2;
-#pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-            uint32_t y[4];
-#pragma unroll
-            for (int f = 0; f < 4; ++f) y[f] = Type<T>::pair(__uint_as_float(x[e + 2 * f]) * by, __uint_as_float(x[e + 2 * f + 1]) * by);
-            if (first + e < D) *reinterpret_cast<uint4*>(at + e * 2) = make_uint4(y[0], y[1], y[2], y[3]);
-        }
+// Columns [0, DP) of a warp's rows of sums, times `by`, into a gradient or a slice's 32-bit sums (part).  `stage`: 4 KB.
+template <typename T, int DP>
+__device__ __forceinline__ void put_sums(uint32_t columns, char* stage, const Heads& to, float* part, bool vec, bool good, int l, int row, int h,
+                                         int rows, int heads, int D, float by) {
+    if (part || vec) {
+        char* const at   = to.ptr + (l * to.sl + row * to.sr + h * to.sh) * 2;
+        char* const sums = reinterpret_cast<char*>(part + ((static_cast<long long>(l) * rows + row) * heads + h) * D);
+        store_sums<T, DP>(columns, stage, good && !part ? at : nullptr, good && part ? sums : nullptr, part != nullptr, D, by);
     } else {
 #pragma unroll
-        for (int e = 0; e < 32; e += 2)
-            put_grad<T>(to, part, l, row, h, rows, heads, D, first + e, __uint_as_float(x[e]) * by, __uint_as_float(x[e + 1]) * by);
+        for (int j = 0; j < DP; j += 32) {
+            uint32_t x[32];
+            tmem_load32(columns + j, x);
+            tmem_wait_load();
+            tmem_loaded32(x);
+            if (!good) continue;
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+                put_grad<T>(to, part, l, row, h, rows, heads, D, j + e, __uint_as_float(x[e]) * by, __uint_as_float(x[e + 1]) * by);
+        }
+    }
+}
+// Zeros instead.
+template <typename T>
+__device__ __forceinline__ void put_zeros(const Heads& to, float* part, bool vec, bool good, int l, int row, int h, int rows, int heads, int D) {
+    if (part || vec) {
+        char* const at   = to.ptr + (l * to.sl + row * to.sr + h * to.sh) * 2;
+        char* const sums = reinterpret_cast<char*>(part + ((static_cast<long long>(l) * rows + row) * heads + h) * D);
+        const u64   mine = good ? reinterpret_cast<u64>(part ? sums : at) : 0;
+        const int   lane = threadIdx.x & 31, chunks = part ? D / 4 : D / 8;
+        for (int i = 0; i < 32; ++i) {
+            char* const row_at = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, mine, i));
+            if (row_at != nullptr)
+                for (int c = lane; c < chunks; c += 32) *reinterpret_cast<uint4*>(row_at + c * 16) = make_uint4(0, 0, 0, 0);
+        }
+    } else if (good) {
+        for (int c = 0; c < D; c += 2) put_grad<T>(to, part, l, row, h, rows, heads, D, c, 0.0f, 0.0f);
     }
 }
 
@@ -209,18 +229,12 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
         float* const part  = p.kv_slices > 1 ? whole + static_cast<long long>(slice) * p.kv_batch * p.M * p.Hk * p.D : nullptr;
         const float  times = half == 0 ? (is_f16<T> ? 1.0f / F16_WEIGHT : 1.0f) : p.scale / factor;
         const uint32_t sums = (half == 0 ? dv_col : dk_col) + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-#pragma unroll
-        for (int j = 0; j < DP; j += 32) {
-            uint32_t x[32];
-            if (n_items > 0) {
-                tmem_load32(sums + j, x);
-                tmem_wait_load();
-                tmem_loaded32(x);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) x[e] = 0;
-            }
-            if (good) put_grad_32<T>(dst, part, p.vec_grad, kl, key, hk, p.M, p.Hk, p.D, j, x, times);
+        if (n_items > 0) {
+            // q and dout tiles have been used for the last time
+            char* const stage = reinterpret_cast<char*>(smem_raw) + (ring_q - raw) + warp * 4096;
+            put_sums<T, DP>(sums, stage, dst, part, p.vec_grad, good, kl, key, hk, p.M, p.Hk, p.D, times);
+        } else {
+            put_zeros<T>(dst, part, p.vec_grad, good, kl, key, hk, p.M, p.Hk, p.D);
         }
     } else if (warp == S::LOAD_WARP) {
         // ------------------------------------------------------------------ copies
@@ -421,19 +435,13 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
         }
         const bool   good = n < p.N && *reinterpret_cast<volatile int*>(&s_expired) == 0;
         float* const part = p.q_slices > 1 ? p.dq_part + static_cast<long long>(l) * p.N * p.H * p.D : nullptr;    // q_splits is 1
-#pragma unroll
-        for (int j = 0; j < DP / 2; j += 32) {
-            const int first = half * (DP / 2) + j;
-            uint32_t  x[32];
-            if (n_items > 0) {
-                tmem_load32(dq_col + lanes + first, x);
-                tmem_wait_load();
-                tmem_loaded32(x);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) x[e] = 0;
+        if (n_items > 0) {
+            if (half == 0) {                 // the warps of the first half write whole rows, where q was held
+                char* const stage = reinterpret_cast<char*>(smem_raw) + (held_q - raw) + warp * 4096;
+                put_sums<T, DP>(dq_col + lanes, stage, p.dq, part, p.vec_grad, good, part ? 0 : l, n, h, p.N, p.H, p.D, p.scale / factor);
             }
-            if (good) put_grad_32<T>(p.dq, part, p.vec_grad, part ? 0 : l, n, h, p.N, p.H, p.D, first, x, p.scale / factor);
+        } else if (half == 0) {
+            put_zeros<T>(p.dq, part, p.vec_grad, good, part ? 0 : l, n, h, p.N, p.H, p.D);
         }
     } else if (warp == S::LOAD_WARP) {
         // ------------------------------------------------------------------ copies

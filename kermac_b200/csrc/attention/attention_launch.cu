@@ -30,6 +30,33 @@ int encode_forward(TensorMaps* maps, const AttentionParams& p, int type, int box
     }
     return rc;
 }
+
+int encode_queries(QueryMaps* maps, int* which, const AttentionParams& p, int type) {
+    *which = 0;
+    const long long most = 1LL << 38;
+    if (128 % p.G != 0 || p.q.sh >= most || p.q.sr >= most || p.q.sl >= most || (p.H > 1 && p.q.sh == 0)) return 0;
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(p.G), static_cast<cuuint32_t>(128 / p.G), 1};
+    const long long  dense = (p.D + 7) & ~7;
+    auto encode = [&](CUtensorMap* map, long long rows, long long sr, int batch, long long sl) {
+        const cuuint64_t dims[4]    = {static_cast<cuuint64_t>(p.D), static_cast<cuuint64_t>(p.H), static_cast<cuuint64_t>(rows),
+                                       static_cast<cuuint64_t>(batch)};
+        const cuuint64_t strides[3] = {static_cast<cuuint64_t>(p.H > 1 ? p.q.sh : dense) * 2, static_cast<cuuint64_t>(rows > 1 ? sr : dense) * 2,
+                                       static_cast<cuuint64_t>(batch > 1 ? sl : dense) * 2};
+        return encode_tma_16bit(map, p.q.ptr, type == ATT_BF16, dims, strides, box);
+    };
+    if (p.own_tiles > 0 && (p.N == 1 || p.q.sr > 0)) {
+        if (int rc = encode(&maps->own, p.N, p.q.sr, p.q.sl == 0 ? 1 : p.L, p.q.sl)) return rc;
+        *which |= QUERIES_OWN;
+    }
+    // one distance between all the queries of the batch
+    const bool even = p.L == 1 || p.N == 1 || p.q.sl == p.N * p.q.sr;
+    const long long apart = p.N == 1 ? p.q.sl : p.q.sr;
+    if (p.prefix_tiles > 0 && even && (static_cast<long long>(p.L) * p.N == 1 || apart > 0)) {
+        if (int rc = encode(&maps->prefix, static_cast<long long>(p.L) * p.N, apart, 1, 0)) return rc;
+        *which |= QUERIES_PREFIX;
+    }
+    return 0;
+}
 }  // namespace att
 
 int count_blocks(const AttentionParams& p, unsigned* blocks) {

@@ -35,7 +35,8 @@ struct TensorShape {
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(TensorShape<DP>::THREADS, 1)
-attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ TensorMaps maps) {
+attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ TensorMaps maps,
+                        const __grid_constant__ QueryMaps queries, const int query_boxes) {
     typedef TensorShape<DP> S;
     extern __shared__ unsigned char smem_raw[];
     constexpr int BARS = 2 * S::STAGES + 4 * S::GROUPS;
@@ -55,7 +56,8 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
     auto o_full = [&](int t) { return bars + 8u * (2 * S::STAGES + 3 * S::GROUPS + t); };
     if (threadIdx.x == 0) {
         for (int st = 0; st < S::STAGES; ++st) mbar_init(full(st), 1), mbar_init(empty(st), 1);
-        for (int t = 0; t < S::GROUPS; ++t) mbar_init(q_full(t), 4), mbar_init(s_full(t), 1), mbar_init(p_full(t), 4), mbar_init(o_full(t), 1);
+        const bool boxes = query_boxes & (static_cast<int>(blockIdx.x) < p.Hk * p.prefix_tiles * p.prefix_splits ? QUERIES_PREFIX : QUERIES_OWN);
+        for (int t = 0; t < S::GROUPS; ++t) mbar_init(q_full(t), boxes ? 1 : 4), mbar_init(s_full(t), 1), mbar_init(p_full(t), 4), mbar_init(o_full(t), 1);
         s_expired = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tc::fence_smem_to_async();
@@ -80,10 +82,11 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
         if (!mbar_wait_bounded(bar, parity, expired ? 1 << 16 : MBAR_WAIT_TRIES)) *reinterpret_cast<volatile int*>(&s_expired) = 1;
     };
 
-    const Work w       = find_work<T>(p, blockIdx.x, S::GROUPS * TC_ROWS, TC_ROWS);
+    const Work w       = find_work<T, S::THREADS>(p, blockIdx.x, S::GROUPS * TC_ROWS, TC_ROWS);
     const int  n_tiles = (w.end - w.first + TC_ROWS - 1) / TC_ROWS;
     const int  groups  = w.row0 + TC_ROWS < w.rows ? 2 : 1;
     const bool prefix  = w.l < 0;
+    const bool boxes   = query_boxes & (prefix ? QUERIES_PREFIX : QUERIES_OWN);      // Q comes by TMA
     const uint32_t ring = base + S::GROUPS * S::TILE;
 
     if (warp < S::LOAD_WARP) {
@@ -93,15 +96,14 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
         const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t s_col = lane_base + S::S_COL + t * 128, o_col = lane_base + S::O_COL + t * DP;
         if (t < groups && n_tiles > 0) {
-            const char* q = nullptr;
-            if (at < w.rows) {
-                const Row row = find_row(p, w, at);
-                q = p.q.ptr + (row.l * p.q.sl + row.n * p.q.sr + row.h * p.q.sh) * 2;
+            const Row row = find_row(p, w, min(at, w.rows - 1));
+            if (!boxes) {
+                const char* q = at < w.rows ? p.q.ptr + (row.l * p.q.sl + row.n * p.q.sr + row.h * p.q.sh) * 2 : nullptr;
+                fill_row<DP>(tiles + t * S::TILE, r, q, p.D);
+                tc::fence_smem_to_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full(t));
             }
-            fill_row<DP>(tiles + t * S::TILE, r, q, p.D);
-            tc::fence_smem_to_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full(t));
 
             // -inf times the scale of 0 would be NaN; the launcher passes at least 2^-100
             const float c = p.scale_log2;
@@ -189,17 +191,27 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
             wait(o_full(t), 0);
             tc::fence_after_sync();
             const bool  good = *reinterpret_cast<volatile int*>(&s_expired) == 0 && at < w.rows;
-            const Row   row = find_row(p, w, at < w.rows ? at : w.rows - 1);
             const float by  = sum == 0.0f ? 0.0f : 1.0f / sum;
             if (good) put_lse(p, w, row, top * c + lg2_approx(sum));
+            if (p.parts > 1 || p.vec_out) {
+                // the warp's rows of Q have been used for the last time
+                char* const stage = tiles + t * S::TILE + (warp & 3) * 4096;
+                char* const to    = p.out.ptr + (row.l * p.out.sl + row.n * p.out.sr + row.h * p.out.sh) * 2;
+                float* const part = p.part_o + ((((static_cast<long long>(w.part) * p.L + row.l) * p.N + row.n) * p.H) + row.h) * p.D;
+                store_sums<T, DP>(o_col, stage, good && p.parts == 1 ? to : nullptr, good && p.parts > 1 ? reinterpret_cast<char*>(part) : nullptr,
+                                  p.parts > 1, p.D, by);
+            } else {
 #pragma unroll
-            for (int j = 0; j < DP; j += 32) {
-                uint32_t o[32];
-                tmem_load32(o_col + j, o);
-                tmem_wait_load();
-                tmem_loaded32(o);
-                if (!good) continue;
-                put_row_32<T>(p, w, row, j, o, by);
+                for (int j = 0; j < DP; j += 32) {
+                    uint32_t o[32];
+                    tmem_load32(o_col + j, o);
+                    tmem_wait_load();
+                    tmem_loaded32(o);
+                    if (!good) continue;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2)
+                        put_pair<T>(p, w, row, j + e, __uint_as_float(o[e]) * by, __uint_as_float(o[e + 1]) * by);
+                }
             }
         } else if (t < groups && at < w.rows) {          // no keys
             const Row row = find_row(p, w, at);
@@ -214,6 +226,15 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
         if (tc::elect_one()) {
             const CUtensorMap *mk = prefix ? &maps.kp : &maps.k, *mv = prefix ? &maps.vp : &maps.v;
             const int lk = prefix || p.k.sl == 0 ? 0 : w.l, lv = prefix || p.v.sl == 0 ? 0 : w.l;
+            if (n_tiles > 0 && boxes)
+                for (int t = 0; t < groups; ++t) {
+                    const CUtensorMap* const mq = prefix ? &queries.prefix : &queries.own;
+                    mbar_expect_tx(q_full(t), S::TILE);
+#pragma unroll
+                    for (int d = 0; d < DP / 64; ++d)
+                        tma_load_box(base + t * S::TILE + d * TC_SLAB, mq, d * 64, w.hk * p.G, (w.row0 + t * TC_ROWS) / p.G,
+                                     prefix || p.q.sl == 0 ? 0 : w.l, q_full(t));
+                }
             for (int j = 0; j < 2 * n_tiles; ++j) {
                 const int st = j % S::STAGES;
                 if (j >= S::STAGES) wait(empty(st), (j / S::STAGES - 1) & 1);
@@ -223,6 +244,7 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
                     tma_load_rows(ring + st * S::TILE + d * TC_SLAB, (j & 1) ? mv : mk, d * 64, w.first + (j >> 1) * TC_ROWS, w.hk,
                                   (j & 1) ? lv : lk, full(st));
             }
+            for (int t = 0; t < groups && n_tiles > 0 && boxes; ++t) drain(q_full(t), 0);
             // copies still in flight must land before the block's shared memory goes to another
             for (int j = max(0, 2 * n_tiles - S::STAGES); j < 2 * n_tiles; ++j) drain(full(j % S::STAGES), (j / S::STAGES) & 1);
         }
@@ -269,7 +291,7 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
 }
 
 template <typename T, int DP>
-int launch_tensor(const AttentionParams& p, const TensorMaps& maps, cudaStream_t st) {
+int launch_tensor(const AttentionParams& p, const TensorMaps& maps, const QueryMaps& queries, int boxes, cudaStream_t st) {
     typedef TensorShape<DP> S;
     static_assert(S::SMEM <= 227 * 1024 && S::SMEM > 114 * 1024, "one block an SM: a second would wait for its tensor memory");
     auto* const kernel = &attention_tensor_kernel<T, DP>;
@@ -277,7 +299,7 @@ int launch_tensor(const AttentionParams& p, const TensorMaps& maps, cudaStream_t
     if (rc) return rc;
     unsigned blocks;
     if ((rc = count_blocks(p, &blocks))) return rc;
-    return cuda_status(launch_overlapped(kernel, dim3(blocks), S::THREADS, S::SMEM, st, p, maps),
+    return cuda_status(launch_overlapped(kernel, dim3(blocks), S::THREADS, S::SMEM, st, p, maps, queries, boxes),
                        "attention_tensor_kernel");
 }
 
@@ -288,8 +310,11 @@ int attention_tensor_launch(const AttentionParams& p, int type, cudaStream_t st)
     using namespace att;
     TensorMaps maps = {};
     if (int rc = encode_forward(&maps, p, type, TC_ROWS)) return rc;
-    if (type == ATT_BF16) return p.D <= 64 ? launch_tensor<__nv_bfloat16, 64>(p, maps, st) : launch_tensor<__nv_bfloat16, 128>(p, maps, st);
-    return p.D <= 64 ? launch_tensor<__half, 64>(p, maps, st) : launch_tensor<__half, 128>(p, maps, st);
+    QueryMaps queries = {};
+    int boxes = 0;
+    if (int rc = encode_queries(&queries, &boxes, p, type)) return rc;
+    if (type == ATT_BF16) return p.D <= 64 ? launch_tensor<__nv_bfloat16, 64>(p, maps, queries, boxes, st) : launch_tensor<__nv_bfloat16, 128>(p, maps, queries, boxes, st);
+    return p.D <= 64 ? launch_tensor<__half, 64>(p, maps, queries, boxes, st) : launch_tensor<__half, 128>(p, maps, queries, boxes, st);
 }
 
 int attention_tensor_take_wait_flag() {

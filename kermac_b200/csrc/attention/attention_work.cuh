@@ -17,7 +17,28 @@ struct Work {
     bool        causal;
 };
 
-template <typename T>
+// The batch entry with the rank-th longest sequence, so that blocks that start first have the most to do (a tail of long ones costs a
+// third of a launch of two rounds).  Called by a whole block of BLOCK threads; more than LPT_MOST entries stay in their order.
+constexpr int LPT_MOST = 256;
+template <int BLOCK>
+__device__ __forceinline__ int longest_first(const int* lengths, long long stride, int L, int M, int rank) {
+    if (!lengths || L == 1 || L > LPT_MOST) return rank;
+    __shared__ int s_length[LPT_MOST], s_entry;
+    for (int i = threadIdx.x; i < L; i += BLOCK) s_length[i] = key_count(lengths, stride, i, M);
+    __syncthreads();
+    for (int i = threadIdx.x; i < L; i += BLOCK) {
+        const int mine = s_length[i];
+        int       longer = 0;
+#pragma unroll 8
+        for (int j = 0; j < L; ++j) longer += s_length[j] > mine || (s_length[j] == mine && j < i);
+        if (longer == rank) s_entry = i;
+    }
+    __syncthreads();
+    return s_entry;
+}
+
+// ORDERED > 0: entries of the batch longest first, called by a whole block of that many threads.
+template <typename T, int ORDERED = 0>
 __device__ __forceinline__ Work find_work(const AttentionParams& p, int block, int rows_per_block, int keys_per_tile) {
     Work w;
     const int prefix_blocks = p.Hk * p.prefix_tiles * p.prefix_splits;
@@ -34,6 +55,7 @@ __device__ __forceinline__ Work find_work(const AttentionParams& p, int block, i
         split = block % p.own_splits, block /= p.own_splits;
         tile  = block % p.own_tiles, block /= p.own_tiles;
         w.hk = block % p.Hk, w.l = block / p.Hk;
+        if constexpr (ORDERED > 0) w.l = longest_first<ORDERED>(p.lengths, p.lengths_stride, p.L, p.M, w.l);
         splits = p.own_splits;
         w.rows = p.N * p.G, w.length = key_count(p.lengths, p.lengths_stride, w.l, p.M), w.part = p.prefix_splits + split;
         w.causal = p.causal;
