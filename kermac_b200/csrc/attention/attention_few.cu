@@ -1,12 +1,17 @@
 // Attention of few 16-bit queries (decoding steps): bound by reading the keys and values once.
 //
-// Up to 16 rows share a block; its warps take tiles of 32 keys in turn, each with a ring of its own that TMA fills, so that no
+// Up to 16 rows share a block; its four warps take tiles of 32 keys in turn, each with a ring of its own that TMA fills, so that no
 // warp waits for another, and add up at the end.  Products are transposed, S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16): the rows
 // are the narrow side of an instruction, eight at a time, where the other way round 16 rows would be computed for one
 // token.  Q stays in registers; P^T passes from accumulator to operand layout by movmatrix.
 //
 // Measured at 64 sequences x 1 x 4096 keys (ragged), 32 heads of 128, 8 key heads, float16, 674 MB: copies by the lanes
-// (cp.async, 480 of some 700 instructions a tile) with 16 rows an instruction took 294 us.
+// (cp.async, 480 of some 700 instructions a tile) with 16 rows an instruction took 294 us, this takes 105: 6.4 TB/s, 99 % of a plain
+// copy.  Two warps a block and two blocks an SM: 118.
+//
+// Two blocks an SM hide what a block does before its first and behind its last tile.  Up to 64 channels they fit; above, tiles of 16
+// keys make room for them and pay where a block has few keys: 128 sequences with 100 to 1024 keys below a prefix of 32768 143.9 -> 138.4 us
+// a pass, but the 64 x 4096 keys above 110.4 -> 113.9.
 #include <algorithm>
 
 #include "attention_tcgen05.cuh"
@@ -17,15 +22,12 @@ namespace {
 
 __device__ int g_attention_few_wait_expired = 0;
 
-#ifndef FEW_WARPS
-#define FEW_WARPS 4
-#endif
-constexpr int FEW_KEYS = 32;
 
-template <int DP, int NR>
+// KEYS: 32 or 16 keys a tile.
+template <int DP, int NR, int KEYS>
 struct FewShape {
-    static constexpr int ROWS   = 8 * NR, STAGES = 3, WARPS = FEW_WARPS, THREADS = 32 * WARPS;
-    static constexpr int SLAB   = FEW_KEYS * 128, TILE = DP / 64 * SLAB;      // one tile of K or V
+    static constexpr int ROWS   = 8 * NR, STAGES = 3;
+    static constexpr int SLAB   = KEYS * 128, TILE = DP / 64 * SLAB;      // one tile of K or V
     static constexpr int RING   = STAGES * 2 * TILE;                          // of one warp
     static constexpr int W      = DP + 2;                                     // channels, maximum and sum of a row
     static constexpr int MERGE  = WARPS * ROWS * W * 4;
@@ -48,10 +50,10 @@ __device__ __forceinline__ float column_sum(float v) {
     return v + __shfl_xor_sync(0xffffffffu, v, 16);
 }
 
-template <typename T, int DP, int NR>
-__global__ void __launch_bounds__(32 * FEW_WARPS) attention_few_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ TensorMaps maps) {
-    typedef FewShape<DP, NR> S;
-    constexpr int WARPS = S::WARPS, THREADS = S::THREADS;
+template <typename T, int DP, int NR, int KEYS>
+__global__ void __launch_bounds__(THREADS) attention_few_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ TensorMaps maps) {
+    typedef FewShape<DP, NR, KEYS> S;
+    constexpr int BLOCKS = KEYS / 16;              // operands of 16 keys in a tile
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long s_bars[WARPS * S::STAGES];
     __shared__ int s_expired;
@@ -67,13 +69,13 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) attention_few_kernel(const __g
     __syncthreads();
     after_previous_grid();
 
-    const Work w      = find_work<T>(p, blockIdx.x, S::ROWS, FEW_KEYS);
+    const Work w      = find_work<T>(p, blockIdx.x, S::ROWS, KEYS);
     const bool prefix = w.l < 0;
-    const int  tiles = (w.end - w.first + FEW_KEYS - 1) / FEW_KEYS, mine = (tiles - warp + WARPS - 1) / WARPS;
+    const int  tiles = (w.end - w.first + KEYS - 1) / KEYS, mine = (tiles - warp + WARPS - 1) / WARPS;
     const CUtensorMap *mk = prefix ? &maps.kp : &maps.k, *mv = prefix ? &maps.vp : &maps.v;
     const int lk = prefix || p.k.sl == 0 ? 0 : w.l, lv = prefix || p.v.sl == 0 ? 0 : w.l;
     auto load = [&](int i) {                                  // by lane 0
-        const int      st = i % S::STAGES, first = w.first + (i * WARPS + warp) * FEW_KEYS;
+        const int      st = i % S::STAGES, first = w.first + (i * WARPS + warp) * KEYS;
         const uint32_t to = ring + st * 2 * S::TILE, bar = bars + 8 * st;
         mbar_expect_tx(bar, 2 * S::TILE);
 #pragma unroll
@@ -118,36 +120,36 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) attention_few_kernel(const __g
     }
     bool expired = false;
     for (int i = 0; i < mine; ++i) {
-        const int      st = i % S::STAGES, first = w.first + (i * WARPS + warp) * FEW_KEYS;
+        const int      st = i % S::STAGES, first = w.first + (i * WARPS + warp) * KEYS;
         const uint32_t tile_k = ring + st * 2 * S::TILE, tile_v = tile_k + S::TILE;
         // every copy is waited for, with a short limit once a wait has run out
         if (!mbar_wait_bounded(bars + 8 * st, (i / S::STAGES) & 1, expired ? 1 << 16 : MBAR_WAIT_TRIES)) expired = true;
-        float s[2][NR][4];
+        float s[BLOCKS][NR][4];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < BLOCKS; ++m)
 #pragma unroll
             for (int r = 0; r < NR; ++r) s[m][r][0] = s[m][r][1] = s[m][r][2] = s[m][r][3] = 0.0f;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
+            for (int m = 0; m < BLOCKS; ++m) {
                 const int row = m * 16 + (lane & 15), chunk = k * 2 + (lane >> 4);
                 uint32_t  a[4];
                 ldmatrix4(a, tile_k + (chunk >> 3) * S::SLAB + row * 128 + ((chunk ^ row) & 7) * 16);
 #pragma unroll
                 for (int r = 0; r < NR; ++r) mma_16(s[m][r], a, q[r][k][0], q[r][k][1], static_cast<const T*>(nullptr));
             }
-        if (first + FEW_KEYS > all_see) {
+        if (first + KEYS > all_see) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int m = 0; m < BLOCKS; ++m)
 #pragma unroll
                 for (int r = 0; r < NR; ++r)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (first + m * 16 + g + 8 * (e >> 1) >= limit[r][e & 1]) s[m][r][e] = -INFINITY;
-            if (first + FEW_KEYS > w.end && w.end < held) {
+            if (first + KEYS > w.end && w.end < held) {
                 // rows of V behind the length hold whatever the memory holds, and 0 * NaN is NaN
-                if (first + lane >= w.end) {
+                if (lane < KEYS && first + lane >= w.end) {
 #pragma unroll
                     for (int c = 0; c < DP / 8; ++c)
                         asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile_v + (c >> 3) * S::SLAB + lane * 128 + (c & 7) * 16), "r"(0) : "memory");
@@ -161,8 +163,9 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) attention_few_kernel(const __g
         for (int r = 0; r < NR; ++r)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float best = fmaxf(fmaxf(s[0][r][e], s[0][r][e + 2]), fmaxf(s[1][r][e], s[1][r][e + 2]));
-                best       = column_max(best);
+                float best = fmaxf(s[0][r][e], s[0][r][e + 2]);
+                if (BLOCKS > 1) best = fmaxf(best, fmaxf(s[BLOCKS - 1][r][e], s[BLOCKS - 1][r][e + 2]));
+                best = column_max(best);
                 grown      = grown || best > top[r][e];
                 base_m[r][e] = fmaxf(best, top[r][e]);
             }
@@ -182,14 +185,14 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) attention_few_kernel(const __g
                     o[d][r][0] *= shrink[0], o[d][r][1] *= shrink[1], o[d][r][2] *= shrink[0], o[d][r][3] *= shrink[1];
             }
         }
-        uint32_t weights[2][NR][2];
+        uint32_t weights[BLOCKS][NR][2];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             float minus[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) minus[e] = top[r][e] == -INFINITY ? 0.0f : -top[r][e] * p.scale_log2;
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
+            for (int m = 0; m < BLOCKS; ++m) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     s[m][r][e] = ex2_approx(fmaf(s[m][r][e], p.scale_log2, minus[e & 1]));
@@ -200,7 +203,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) attention_few_kernel(const __g
             }
         }
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < BLOCKS; ++m)
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) {
                 const int row = m * 16 + (lane & 7) + ((lane >> 4) << 3), chunk = d * 2 + ((lane >> 3) & 1);
@@ -250,20 +253,21 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) attention_few_kernel(const __g
     }
 }
 
-template <typename T, int DP, int NR>
+template <typename T, int DP, int NR, int KEYS>
 int launch_few(const AttentionParams& p, const TensorMaps& maps, cudaStream_t st) {
-    constexpr int smem = FewShape<DP, NR>::SMEM;
+    constexpr int smem = FewShape<DP, NR, KEYS>::SMEM;
     static_assert(smem <= 227 * 1024, "more shared memory than a block has");
-    auto* const kernel = &attention_few_kernel<T, DP, NR>;
+    auto* const kernel = &attention_few_kernel<T, DP, NR, KEYS>;
     if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute")) return rc;
     unsigned blocks;
     if (int rc = count_blocks(p, &blocks)) return rc;
-    return cuda_status(launch_overlapped(kernel, dim3(blocks), FewShape<DP, NR>::THREADS, smem, st, p, maps), "attention_few_kernel");
+    return cuda_status(launch_overlapped(kernel, dim3(blocks), THREADS, smem, st, p, maps), "attention_few_kernel");
 }
 template <typename T>
-int launch_few_type(const AttentionParams& p, const TensorMaps& maps, int rows, cudaStream_t st) {
-    if (p.D <= 64) return rows <= 8 ? launch_few<T, 64, 1>(p, maps, st) : launch_few<T, 64, 2>(p, maps, st);
-    return rows <= 8 ? launch_few<T, 128, 1>(p, maps, st) : launch_few<T, 128, 2>(p, maps, st);
+int launch_few_type(const AttentionParams& p, const TensorMaps& maps, int rows, int keys, cudaStream_t st) {
+    if (p.D <= 64) return rows <= 8 ? launch_few<T, 64, 1, 32>(p, maps, st) : launch_few<T, 64, 2, 32>(p, maps, st);
+    if (keys == 16) return rows <= 8 ? launch_few<T, 128, 1, 16>(p, maps, st) : launch_few<T, 128, 2, 16>(p, maps, st);
+    return rows <= 8 ? launch_few<T, 128, 1, 32>(p, maps, st) : launch_few<T, 128, 2, 32>(p, maps, st);
 }
 
 }  // namespace
@@ -272,8 +276,9 @@ int launch_few_type(const AttentionParams& p, const TensorMaps& maps, int rows, 
 int attention_few_launch(const AttentionParams& p, int type, int rows, cudaStream_t st) {
     using namespace att;
     TensorMaps maps = {};
-    if (int rc = encode_forward(&maps, p, type, FEW_KEYS)) return rc;
-    return type == ATT_BF16 ? launch_few_type<__nv_bfloat16>(p, maps, rows, st) : launch_few_type<__half>(p, maps, rows, st);
+    const int  keys = attention_few_tile(p.D, p.own_tiles > 0 ? p.M : 0, p.prefix_tiles > 0 ? p.P : 0);
+    if (int rc = encode_forward(&maps, p, type, keys)) return rc;
+    return type == ATT_BF16 ? launch_few_type<__nv_bfloat16>(p, maps, rows, keys, st) : launch_few_type<__half>(p, maps, rows, keys, st);
 }
 
 int attention_few_take_wait_flag() {

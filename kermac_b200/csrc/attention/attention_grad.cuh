@@ -11,25 +11,20 @@ constexpr float F16_WEIGHT = 256.0f, F16_WEIGHT_LOG2 = 8.0f;
 
 template <typename T> constexpr bool is_f16 = std::is_same<T, __half>::value;
 
-// 2^-e with 2^e the power of two at or below the largest of the given peaks; 1 when they are zero, infinite or NaN.
-// Called by the whole block of BLOCK threads.
-template <typename T, int BLOCK>
+// 2^-e with 2^e the power of two at or below the largest of the peaks of entries [l0, l1) and heads [h0, h1); 1 when they are zero,
+// infinite or NaN, and for the types that have the range.  Called by whole warps, each for itself.
+template <typename T>
 __device__ __forceinline__ float find_factor(const AttentionGradParams& p, int l0, int l1, int h0, int h1) {
     if constexpr (!is_f16<T>) {
         return 1.0f;
     } else {
-        __shared__ float of_warp[BLOCK / 32];
-        float best = 0.0f;
+        float     best  = 0.0f;
         const int per_l = (h1 - h0) * p.peak_count;
         for (int l = l0; l < l1; ++l)
-            for (int i = threadIdx.x; i < per_l; i += BLOCK)
+            for (int i = threadIdx.x & 31; i < per_l; i += 32)
                 best = fmaxf(best, p.peaks[(static_cast<long long>(l) * p.H + h0) * p.peak_count + i]);
 #pragma unroll
         for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
-        if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = best;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < BLOCK / 32; ++i) best = fmaxf(best, of_warp[i]);
         const uint32_t e = __float_as_uint(best) >> 23;                  // best is a float16 magnitude: 2^-24 .. 65504
         return (best > 0.0f && e < 255) ? __uint_as_float((254u - e) << 23) : 1.0f;
     }

@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(THREADS) attention_grad_keys_kernel(const Atte
             longest = n > longest ? n : longest;
         }
     const bool  idle   = key0 >= longest;
-    const float factor = find_factor<T, THREADS>(p, l_first, l_first + l_count, hk * p.G, hk * p.G + p.G);
+    const float factor = find_factor<T>(p, l_first, l_first + l_count, hk * p.G, hk * p.G + p.G);
     const float by     = is_f16<T> ? factor / F16_WEIGHT : 1.0f;
 
     float dk[CT][4], dv[CT][4];
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(THREADS) attention_grad_queries_kernel(const A
     const int h = block % p.H, l = block / p.H, hk = h / p.G;
     const int   count  = key_count(p.lengths, p.lengths_stride, l, p.M);
     const int   kl     = p.kv_batch == 1 ? 0 : l;
-    const float factor = find_factor<T, THREADS>(p, l, l + 1, h, h + 1);
+    const float factor = find_factor<T>(p, l, l + 1, h, h + 1);
 
     copy_rows<T, DP>(held_q, head_of<T>(p.q, l, h), p.q.sr, n0, p.N, S::ROWS, p.D, p.vec, threadIdx.x, THREADS);
     copy_rows<T, DP>(held_d, head_of<T>(p.dout, l, h), p.dout.sr, n0, p.N, S::ROWS, p.D, p.vec, threadIdx.x, THREADS);

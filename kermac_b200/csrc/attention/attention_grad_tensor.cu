@@ -87,6 +87,7 @@ __device__ __forceinline__ void put_zeros(const Heads& to, float* part, bool vec
         char* const sums = reinterpret_cast<char*>(part + ((static_cast<long long>(l) * rows + row) * heads + h) * D);
         const u64   mine = good ? reinterpret_cast<u64>(part ? sums : at) : 0;
         const int   lane = threadIdx.x & 31, chunks = part ? D / 4 : D / 8;
+#pragma unroll 8
         for (int i = 0; i < 32; ++i) {
             char* const row_at = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, mine, i));
             if (row_at != nullptr)
@@ -143,9 +144,9 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
     if (from < to)
         for (int l = l_first + from / (p.G * q_tiles); l <= l_first + (to - 1) / (p.G * q_tiles); ++l)
             longest = max(longest, key_count(p.lengths, p.lengths_stride, l, p.M));
-    const int   n_items = key0 < longest ? to - from : 0;
-    const float factor  = find_factor<T, S::BLOCK>(p, l_first, l_first + l_count, hk * p.G, hk * p.G + p.G);
-    const float by      = is_f16<T> ? factor / F16_WEIGHT : 1.0f;
+    const int n_items = key0 < longest ? to - from : 0;
+    // asked for by the warps that need it, while the copies are under way
+    auto find_this_factor = [&] { return n_items > 0 ? find_factor<T>(p, l_first, l_first + l_count, hk * p.G, hk * p.G + p.G) : 1.0f; };
 
     tc::fence_before_sync();
     __syncthreads();
@@ -157,6 +158,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
 
     if (warp < S::WARPS_ON_WEIGHTS) {
         // ------------------------------------------------------------------ weights: lane = key, 64 queries of a tile
+        const float    factor = find_this_factor(), by = is_f16<T> ? factor / F16_WEIGHT : 1.0f;
         const int      half = warp >> 2, key = key0 + (threadIdx.x & 127);
         const uint32_t at   = (static_cast<uint32_t>((warp & 3) * 32) << 16) + half * 64;
         const u64      c2 = pack2(p.scale_log2, p.scale_log2), by2 = pack2(by, by);
@@ -262,6 +264,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
         __syncwarp();
     } else if (warp == S::STATS_WARP) {
         // ------------------------------------------------------------------ lse and delta of the query tiles
+        const float by = is_f16<T> ? find_this_factor() / F16_WEIGHT : 1.0f;
         for (int i = 0; i < n_items; ++i) {
             const int st = i % ST, item = from + i, lg = item / q_tiles, l = l_first + lg / p.G, h = hk * p.G + lg % p.G;
             const int n0 = item % q_tiles * TC_ROWS;
@@ -357,7 +360,6 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
     const int h = block % p.H, l = block / p.H, hk = h / p.G;
     const int kl = p.kv_batch == 1 ? 0 : l;
     const int count = key_count(p.lengths, p.lengths_stride, l, p.M), n_items = (count + TC_ROWS - 1) / TC_ROWS;
-    const float factor = find_factor<T, S::BLOCK>(p, l, l + 1, h, h + 1);
 
     tc::fence_before_sync();
     __syncthreads();
@@ -369,6 +371,7 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
 
     if (warp < S::WARPS_ON_WEIGHTS) {
         // ------------------------------------------------------------------ weights: lane = query, 64 keys of a tile
+        const float    factor = n_items > 0 ? find_factor<T>(p, l, l + 1, h, h + 1) : 1.0f;
         const int      half = warp >> 2, n = n0 + (threadIdx.x & 127);
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, at = lanes + half * 64;
         const float    shift = n < p.N ? -p.lse[l * p.lse_sl + h * p.lse_sh + n] * (1.0f / LN2) : -INFINITY;

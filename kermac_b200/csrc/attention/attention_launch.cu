@@ -170,9 +170,9 @@ struct Plan {
     long long bytes;
 };
 
-Form choose_form(long long rows, bool tma_ok, int type, int d) {
+Form choose_form(long long rows, bool tma_ok, int type, int d, int keys) {
     if (tma_ok && rows > 16) return {TENSOR, ATT_TENSOR_ROWS, 1, 256};
-    if (tma_ok) return {FEW, rows <= 8 ? 8 : 16, d <= 64 ? 2 : 1, 256};
+    if (tma_ok) return {FEW, rows <= 8 ? 8 : 16, d <= 64 || attention_few_tile(d, keys, 0) == 16 ? 2 : 1, 256};
     if (rows <= ATT_FEW_ROWS) return {SCALAR_FEW, ATT_FEW_ROWS, 1, 256};
     return {ROWS, ATT_TILE_ROWS, type == ATT_F32 ? 4 : 2, 256};
 }
@@ -210,8 +210,8 @@ Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool scratch) {
                                           : own_ok;
     p.vec_out = rows_aligned(a.out, a.type, a.d);
     const long long own_rows = static_cast<long long>(p.N) * p.G, prefix_rows = own_rows * p.L;
-    plan.own    = choose_form(own_rows, own_ok, a.type, p.D);
-    plan.prefix = choose_form(prefix_rows, prefix_ok, a.type, p.D);
+    plan.own    = choose_form(own_rows, own_ok, a.type, p.D, p.M);
+    plan.prefix = choose_form(prefix_rows, prefix_ok, a.type, p.D, p.P);
     if (p.M > 0 || p.P == 0) {
         p.own_tiles  = static_cast<int>(ceil_div_ll(own_rows, plan.own.rows));
         p.own_splits = scratch ? pieces(static_cast<long long>(p.own_tiles) * p.L * p.Hk, p.M, plan.own.per_sm, plan.own.least) : 1;

@@ -64,6 +64,8 @@ int  attention_rows_launch(const AttentionParams& p, int type, bool few, cudaStr
 constexpr int ATT_FEW_ROWS = 16, ATT_TILE_ROWS = 64;
 int  attention_join_launch(const AttentionParams& p, int type, cudaStream_t st);
 // attention_few.cu: 16-bit types, D a multiple of 8 up to 128, rows that TMA can copy; 8 or 16 rows a block.
+// Keys of a tile, from the channels and the keys of the launch's two sets (0: none): see attention_few.cu.
+inline int attention_few_tile(int d, int keys, int prefix) { return d > 64 && keys <= 2048 && prefix <= 2048 ? 16 : 32; }
 int  attention_few_launch(const AttentionParams& p, int type, int rows, cudaStream_t st);
 int  attention_few_take_wait_flag();
 // Blocks of a forward launch: every (key head, row tile, piece) of both sets of keys.
