@@ -56,8 +56,9 @@ int kermac_b200_prefix_attention(const KmAttentionArgs* args, void* stream);
 /* grad_q, grad_k and grad_v from grad_out and the forward pass's out and lse.  Every row is written, those of keys behind
  * lengths[l] with zeros.  The sums have a fixed order: equal calls give equal bits. */
 int kermac_b200_cross_attention_grad(const KmAttentionArgs* args, void* stream);
-/* Bytes of scratch that the three calls use (0: none).  The two forward calls run without it, slower where few blocks have to
- * read long keys, unless there are both a prefix and own keys; the gradient needs it. */
+/* Bytes of scratch that the three calls use (0: none): partial sums, 512 MB at most, and copies of float32 inputs of up to 64
+ * channels, 1 GiB at most.  The two forward calls take less or none, and are slower then, unless there are both a prefix and own
+ * keys, whose partial sums they need; the gradient needs all of it. */
 int64_t kermac_b200_cross_attention_scratch_bytes(const KmAttentionArgs* args);
 int64_t kermac_b200_prefix_attention_scratch_bytes(const KmAttentionArgs* args);
 int64_t kermac_b200_cross_attention_grad_scratch_bytes(const KmAttentionArgs* args);

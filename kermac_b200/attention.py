@@ -127,8 +127,12 @@ def _launch(args, kind, q, debug):
     need = _native.attention_scratch_bytes(args, kind)
     scratch = None
     if need > 0:
-        scratch = torch.empty(need // 4, dtype=torch.float32, device=q.device)
-        args.scratch, args.scratch_bytes = scratch.data_ptr(), need
+        try:
+            scratch = torch.empty(need // 4, dtype=torch.float32, device=q.device)
+            args.scratch, args.scratch_bytes = scratch.data_ptr(), need
+        except torch.cuda.OutOfMemoryError:      # there it only makes the call faster
+            if kind != _native.ATTENTION_CROSS:
+                raise
     if debug:
         print(f'(Kermac Debug) Launching kernel: {_native.describe_attention(args, kind)}')
     _native.launch_attention(args, kind, stream_ptr)
@@ -184,9 +188,13 @@ def cross_attention(
     `cross_attention_grad` needs; with `return_lse` the call returns (out, lse).  `scale` is 1 / sqrt(D) when None.
 
     Scores, softmax and sums are 32-bit; with 16-bit types the weights are rounded to that type for the product with v.  Equal
-    calls give equal bits.  Partial sums, where few queries look at many states, take at most 512 MB from torch's allocator for
-    the duration of the call.  Launches on torch's current stream and returns without synchronising; like every
-    allocation by torch that has to be captured through torch.cuda.graph.
+    calls give equal bits.  Partial sums, where few queries look at many states (at most 512 MB), and copies of float32 inputs
+    of up to 64 channels (1.5 times their size, at most 1 GiB) are taken from torch's allocator for the duration of the call.
+    Launches on torch's current stream and returns without synchronising; like every allocation by torch that has to be
+    captured through torch.cuda.graph.
+
+    Bounded waits as in `kernel_matvec`: one that runs out leaves rows unwritten and raises the flag that
+    `kermac_b200._native.device_error_flag()` reads.
     """
     return _forward(_native.ATTENTION_CROSS, q, k, v, lengths, scale, out, lse, return_lse, debug)
 

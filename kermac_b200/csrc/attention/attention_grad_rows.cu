@@ -266,19 +266,22 @@ __global__ void __launch_bounds__(THREADS) attention_delta_kernel(const Attentio
     }
 }
 
-// dst[l][row][head][c] = sum over the slices, in their order.
 template <typename T>
-__global__ void __launch_bounds__(THREADS) attention_reduce_kernel(const float* src, int slices, const Heads dst, int L, int rows,
-                                                                  int heads, int D) {
+__global__ void __launch_bounds__(THREADS) attention_reduce_kernel(const SliceSums sums) {
     after_previous_grid();
-    const long long total = static_cast<long long>(L) * rows * heads * D;
-    for (long long i = static_cast<long long>(blockIdx.x) * THREADS + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * THREADS) {
+    const long long all = sums.first[sums.count];
+    for (long long at = static_cast<long long>(blockIdx.x) * THREADS + threadIdx.x; at < all; at += static_cast<long long>(gridDim.x) * THREADS) {
+        int which = 0;
+        while (which + 1 < sums.count && at >= sums.first[which + 1]) ++which;
+        const SliceSum& j = sums.job[which];
+        const long long i = at - sums.first[which], total = sums.first[which + 1] - sums.first[which];
         float sum = 0.0f;
-        for (int s = 0; s < slices; ++s) sum += src[s * total + i];
-        const int       c = static_cast<int>(i % D);
-        const long long at = i / D;
-        const int       h = static_cast<int>(at % heads), row = static_cast<int>(at / heads % rows), l = static_cast<int>(at / heads / rows);
-        reinterpret_cast<T*>(dst.ptr)[l * dst.sl + row * dst.sr + h * dst.sh + c] = Type<T>::to(sum);
+#pragma unroll 4
+        for (int s = 0; s < j.slices; ++s) sum += j.src[s * total + i];
+        const int       c = static_cast<int>(i % j.D);
+        const long long rest = i / j.D;
+        const int       h = static_cast<int>(rest % j.heads), row = static_cast<int>(rest / j.heads % j.rows), l = static_cast<int>(rest / j.heads / j.rows);
+        reinterpret_cast<T*>(j.dst.ptr)[l * j.dst.sl + row * j.dst.sr + h * j.dst.sh + c] = Type<T>::to(sum);
     }
 }
 
@@ -333,16 +336,15 @@ int attention_delta_launch(const AttentionGradParams& p, int type, cudaStream_t 
     return cuda_status(e, "attention_delta_kernel");
 }
 
-int attention_reduce_launch(const float* src, int slices, const Heads& dst, int L, int rows, int heads, int D, int type,
-                            cudaStream_t st) {
+int attention_reduce_launch(const SliceSums& sums, int type, cudaStream_t st) {
     using namespace att;
-    long long blocks = ceil_div_ll(static_cast<long long>(L) * rows * heads * D, THREADS);
+    long long blocks = ceil_div_ll(sums.first[sums.count], THREADS);
+    if (blocks == 0) return 0;
     if (blocks > 65536) blocks = 65536;                     // the kernel strides over the rest
     const dim3 grid(static_cast<unsigned>(blocks));
-    const cudaError_t e =
-        type == ATT_F32    ? launch_overlapped(&attention_reduce_kernel<float>, grid, THREADS, 0, st, src, slices, dst, L, rows, heads, D)
-        : type == ATT_BF16 ? launch_overlapped(&attention_reduce_kernel<__nv_bfloat16>, grid, THREADS, 0, st, src, slices, dst, L, rows, heads, D)
-                           : launch_overlapped(&attention_reduce_kernel<__half>, grid, THREADS, 0, st, src, slices, dst, L, rows, heads, D);
+    const cudaError_t e = type == ATT_F32    ? launch_overlapped(&attention_reduce_kernel<float>, grid, THREADS, 0, st, sums)
+                          : type == ATT_BF16 ? launch_overlapped(&attention_reduce_kernel<__nv_bfloat16>, grid, THREADS, 0, st, sums)
+                                             : launch_overlapped(&attention_reduce_kernel<__half>, grid, THREADS, 0, st, sums);
     return cuda_status(e, "attention_reduce_kernel");
 }
 

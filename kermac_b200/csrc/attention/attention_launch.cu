@@ -106,7 +106,8 @@ int check(const KmAttentionArgs* a, Kind kind) {
     if (kind != PREFIX && a->prefix != 0) return fail(KM_ERR_BAD_SHAPE, "only prefix_attention has a prefix");
     if (a->m > (1 << 30) || a->prefix > (1 << 30)) return fail(KM_ERR_TOO_LARGE, "more than 2^30 keys");
     const long long rows = static_cast<long long>(a->l) * a->n * a->heads;
-    if (static_cast<long long>(a->l) * a->n > 0x7fffffffLL || rows > 0x7fffffffLL) return fail(KM_ERR_TOO_LARGE, "batch * queries * heads must be below 2^31");
+    const long long most_rows = (1LL << 31) - 1024;           // row numbers of the last tile stay below 2^31
+    if (static_cast<long long>(a->l) * a->n > most_rows || rows > most_rows) return fail(KM_ERR_TOO_LARGE, "batch * queries * heads must be below 2^31");
     if ((a->k.stride_l == 0) != (a->v.stride_l == 0) && a->l > 1 && a->m > 0)
         return fail(KM_ERR_BAD_STRIDE, "k and v must both be broadcast over the batch, or neither");
     const bool any = rows > 0;
@@ -154,26 +155,30 @@ bool tma_rows_ok(const KmHeads& t, int rows, int n_heads, int type, int d) {
 }
 
 // The kernels of the forward pass.  TENSOR: 256 rows on tcgen05.  FEW: 8 or 16 rows whose keys a few warps share out, fed by TMA.
-// For what these two do not take: SCALAR_FEW, 16 rows in the manner of FEW, and ROWS, 64 rows that share key tiles.
-enum Kernel { TENSOR, FEW, SCALAR_FEW, ROWS };
+// TENSOR32: 256 rows of float32 on tcgen05, from copies in three bf16 planes.  For what these do not take: SCALAR_FEW, 16 rows in the manner of FEW, and ROWS, 64 rows that share key tiles.
+enum Kernel { TENSOR, FEW, TENSOR32, SCALAR_FEW, ROWS };
 struct Form {
     Kernel kernel;
     int    rows;            // of a block
     int    per_sm, least;   // blocks that an SM holds; keys below which a piece does not pay
     bool operator!=(const Form& f) const { return kernel != f.kernel || rows != f.rows; }
-    const char* name() const { return kernel == TENSOR ? "tensor" : kernel == FEW ? "few" : kernel == ROWS ? "rows" : "scalar few"; }
+    const char* name() const { return kernel == TENSOR ? "tensor" : kernel == FEW ? "few" : kernel == TENSOR32 ? "tensor32" : kernel == ROWS ? "rows" : "scalar few"; }
 };
 
 struct Plan {
     Form own, prefix;
     AttentionParams p;
-    long long bytes;
+    long long parts;         // bytes of partial sums, and of the planes behind them
+    long long planes;
+    long long bytes() const { return parts + planes; }
 };
 
-Form choose_form(long long rows, bool tma_ok, int type, int d, int keys) {
+// keys: of the set; all_keys: of both.
+Form choose_form(long long rows, bool tma_ok, int type, int d, int keys, int all_keys, bool planes) {
     if (tma_ok && rows > 16) return {TENSOR, ATT_TENSOR_ROWS, 1, 256};
     if (tma_ok) return {FEW, rows <= 8 ? 8 : 16, d <= 64 || attention_few_tile(d, keys, 0) == 16 ? 2 : 1, 256};
     if (rows <= ATT_FEW_ROWS) return {SCALAR_FEW, ATT_FEW_ROWS, 1, 256};
+    if (planes && all_keys > 64) return {TENSOR32, ATT_TENSOR_ROWS, 1, 256};      // measured in attention_tensor32.cu
     return {ROWS, ATT_TILE_ROWS, type == ATT_F32 ? 4 : 2, 256};
 }
 
@@ -184,7 +189,8 @@ int pieces(long long blocks, long long keys, int per_sm, int least) {
     return static_cast<int>(std::max(1LL, std::min({fit, keys / least, 256LL})));
 }
 
-Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool scratch) {
+// `split`: keys may be divided; `planes`: copies of the inputs may be made.
+Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool split, bool planes) {
     Plan plan = {};
     AttentionParams& p = plan.p;
     p.L = a.l, p.N = a.n, p.H = a.heads, p.Hk = a.key_heads, p.G = a.heads / a.key_heads, p.D = a.d, p.M = a.m, p.P = a.prefix;
@@ -210,35 +216,49 @@ Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool scratch) {
                                           : own_ok;
     p.vec_out = rows_aligned(a.out, a.type, a.d);
     const long long own_rows = static_cast<long long>(p.N) * p.G, prefix_rows = own_rows * p.L;
-    plan.own    = choose_form(own_rows, own_ok, a.type, p.D, p.M);
-    plan.prefix = choose_form(prefix_rows, prefix_ok, a.type, p.D, p.P);
+    plan.own    = choose_form(own_rows, own_ok, a.type, p.D, p.M, p.M + p.P, planes);
+    plan.prefix = choose_form(prefix_rows, prefix_ok, a.type, p.D, p.P, p.M + p.P, planes);
+    // one launch for both sets where the same kernel takes them
+    if (p.M > 0 && p.P > 0 && plan.own.kernel == FEW && plan.prefix.kernel == FEW)
+        plan.own.rows = plan.prefix.rows = std::max(plan.own.rows, plan.prefix.rows);
     if (p.M > 0 || p.P == 0) {
         p.own_tiles  = static_cast<int>(ceil_div_ll(own_rows, plan.own.rows));
-        p.own_splits = scratch ? pieces(static_cast<long long>(p.own_tiles) * p.L * p.Hk, p.M, plan.own.per_sm, plan.own.least) : 1;
+        p.own_splits = split ? pieces(static_cast<long long>(p.own_tiles) * p.L * p.Hk, p.M, plan.own.per_sm, plan.own.least) : 1;
     }
     if (p.P > 0) {
         p.prefix_tiles  = static_cast<int>(ceil_div_ll(prefix_rows, plan.prefix.rows));
-        p.prefix_splits = scratch ? pieces(static_cast<long long>(p.prefix_tiles) * p.Hk, p.P, plan.prefix.per_sm, plan.prefix.least) : 1;
+        p.prefix_splits = split ? pieces(static_cast<long long>(p.prefix_tiles) * p.Hk, p.P, plan.prefix.per_sm, plan.prefix.least) : 1;
     }
     p.parts = p.own_splits + p.prefix_splits;
-    if (p.parts > 1) plan.bytes = static_cast<long long>(p.parts) * p.L * p.N * p.H * (p.D + 1) * 4;
+    auto round16 = [](long long n) { return (n + 15) & ~15LL; };
+    if (p.parts > 1) plan.parts = round16(static_cast<long long>(p.parts) * p.L * p.N * p.H * (p.D + 1) * 4);
+    if ((p.own_splits > 0 && plan.own.kernel == TENSOR32) || (p.prefix_splits > 0 && plan.prefix.kernel == TENSOR32))
+        plan.planes = round16(attention_planes_bytes(p));
     return plan;
 }
 
 bool empty(const KmAttentionArgs& a) { return a.l == 0 || a.n == 0 || a.heads == 0; }
 
-// The largest scratch that a call asks for: a plan that wants more takes a single piece for each set of keys.
-constexpr long long MOST_SCRATCH = 512LL << 20;
+// The most scratch that a call asks for: partial sums, and planes of float32 inputs.
+constexpr long long MOST_SCRATCH = 512LL << 20, MOST_PLANES = 1LL << 30;
 
+// The plan that a scratch of `most` bytes allows: first without planes, then with a single piece for each set of keys.
 Plan plan_within(const KmAttentionArgs& a, Kind kind, long long most) {
-    Plan plan = plan_forward(a, kind, true);
-    if (plan.bytes > most) plan = plan_forward(a, kind, false);
+    Plan plan = {};
+    const bool one_set = a.l > 1 && a.k.stride_l == 0 && a.lengths;      // see attention_tensor32_launch
+    if (a.type == ATT_F32 && a.d <= ATT_TENSOR32_CHANNELS && !one_set) {
+        plan = plan_forward(a, kind, true, true);
+        if (plan.parts > MOST_SCRATCH) plan = plan_forward(a, kind, false, true);
+        if (plan.planes <= MOST_PLANES && plan.bytes() <= most) return plan;
+    }
+    plan = plan_forward(a, kind, true, false);
+    if (plan.parts > std::min(most, MOST_SCRATCH)) plan = plan_forward(a, kind, false, false);
     return plan;
 }
 
 int64_t forward_scratch(const KmAttentionArgs* a, Kind kind) {
     if (check(a, kind) || empty(*a)) return 0;
-    return plan_within(*a, kind, MOST_SCRATCH).bytes;
+    return plan_within(*a, kind, MOST_SCRATCH + MOST_PLANES).bytes();
 }
 
 int forward(const KmAttentionArgs* a, Kind kind, void* stream) {
@@ -248,15 +268,16 @@ int forward(const KmAttentionArgs* a, Kind kind, void* stream) {
     rc = require_sm100();
     if (rc) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    Plan plan = plan_within(*a, kind, a->scratch ? std::min<long long>(MOST_SCRATCH, a->scratch_bytes) : 0);
-    if (plan.bytes > 0) {
-        if (!a->scratch || a->scratch_bytes < plan.bytes || !aligned16(a->scratch))
-            return fail(KM_ERR_NULL_POINTER, "attention: %lld bytes of 16-byte aligned scratch are needed", plan.bytes);
+    Plan plan = plan_within(*a, kind, a->scratch && aligned16(a->scratch) ? a->scratch_bytes : 0);
+    if (plan.bytes() > 0) {
+        if (!a->scratch || a->scratch_bytes < plan.bytes() || !aligned16(a->scratch))
+            return fail(KM_ERR_NULL_POINTER, "attention: %lld bytes of 16-byte aligned scratch are needed", plan.bytes());
         plan.p.part_o   = static_cast<float*>(a->scratch);
         plan.p.part_lse = plan.p.part_o + static_cast<long long>(plan.p.parts) * plan.p.L * plan.p.N * plan.p.H * plan.p.D;
     }
     auto launch = [&](const AttentionParams& p, const Form& form) {
         if (form.kernel == TENSOR) return attention_tensor_launch(p, a->type, st);
+        if (form.kernel == TENSOR32) return attention_tensor32_launch(p, static_cast<char*>(a->scratch) + plan.parts, st);
         if (form.kernel == FEW) return attention_few_launch(p, a->type, form.rows, st);
         return attention_rows_launch(p, a->type, form.kernel == SCALAR_FEW, st);
     };
@@ -318,12 +339,6 @@ GradPlan plan_grad(const KmAttentionArgs& a) {
     return plan;
 }
 
-// Zeros for a gradient that no pair of query and key reaches.
-int clear(const Heads& t, int batch, int rows, int n_heads, int d, int type, cudaStream_t st) {
-    if (static_cast<long long>(batch) * rows * n_heads == 0) return 0;
-    return attention_reduce_launch(nullptr, 0, t, batch, rows, n_heads, d, type, st);
-}
-
 int gradient(const KmAttentionArgs* a, void* stream) {
     int rc = check(a, GRAD);
     if (rc) return rc;
@@ -334,10 +349,12 @@ int gradient(const KmAttentionArgs* a, void* stream) {
     GradPlan plan = plan_grad(*a);
     AttentionGradParams& p = plan.p;
     if (empty(*a) || a->m == 0) {
-        rc = clear(p.dq, a->q_batch, p.N, p.H, p.D, a->type, st);
-        if (!rc) rc = clear(p.dk, p.kv_batch, p.M, p.Hk, p.D, a->type, st);
-        if (!rc) rc = clear(p.dv, p.kv_batch, p.M, p.Hk, p.D, a->type, st);
-        return rc;
+        // zeros: no pair of query and key reaches them
+        SliceSums none = {};
+        none.add(nullptr, 0, p.dq, a->q_batch, p.N, p.H, p.D);
+        none.add(nullptr, 0, p.dk, p.kv_batch, p.M, p.Hk, p.D);
+        none.add(nullptr, 0, p.dv, p.kv_batch, p.M, p.Hk, p.D);
+        return attention_reduce_launch(none, a->type, st);
     }
     if (!a->scratch || a->scratch_bytes < plan.bytes() || !aligned16(a->scratch))
         return fail(KM_ERR_NULL_POINTER, "attention gradient: %lld bytes of 16-byte aligned scratch are needed", plan.bytes());
@@ -348,10 +365,13 @@ int gradient(const KmAttentionArgs* a, void* stream) {
     if (plan.dkv) p.dk_part = at, p.dv_part = at + plan.dkv;
     rc = attention_delta_launch(p, a->type, st);
     if (!rc) rc = plan.tensor ? attention_grad_tensor_launch(p, a->type, st) : attention_grad_rows_launch(p, a->type, st);
-    if (!rc && p.q_slices > 1) rc = attention_reduce_launch(p.dq_part, p.q_slices, p.dq, a->q_batch, p.N, p.H, p.D, a->type, st);
-    if (!rc && p.kv_slices > 1) rc = attention_reduce_launch(p.dk_part, p.kv_slices, p.dk, p.kv_batch, p.M, p.Hk, p.D, a->type, st);
-    if (!rc && p.kv_slices > 1) rc = attention_reduce_launch(p.dv_part, p.kv_slices, p.dv, p.kv_batch, p.M, p.Hk, p.D, a->type, st);
-    return rc;
+    SliceSums sums = {};
+    if (p.q_slices > 1) sums.add(p.dq_part, p.q_slices, p.dq, a->q_batch, p.N, p.H, p.D);
+    if (p.kv_slices > 1) {
+        sums.add(p.dk_part, p.kv_slices, p.dk, p.kv_batch, p.M, p.Hk, p.D);
+        sums.add(p.dv_part, p.kv_slices, p.dv, p.kv_batch, p.M, p.Hk, p.D);
+    }
+    return rc ? rc : attention_reduce_launch(sums, a->type, st);
 }
 
 }  // namespace
@@ -378,10 +398,10 @@ int kermac_b200_describe_attention(const KmAttentionArgs* args, int32_t kind, ch
         const GradPlan plan = plan_grad(*args);
         snprintf(buf, buf_len, "grad=%s q_slices=%d kv_slices=%d scratch=%lld", plan.tensor ? "tensor" : "rows", plan.p.q_slices, plan.p.kv_slices, plan.bytes());
     } else {
-        const Plan plan = plan_within(*args, static_cast<Kind>(kind), MOST_SCRATCH);
+        const Plan plan = plan_within(*args, static_cast<Kind>(kind), MOST_SCRATCH + MOST_PLANES);
         snprintf(buf, buf_len, "own=%s rows=%d tiles=%d splits=%d prefix=%s rows=%d tiles=%d splits=%d scratch=%lld", plan.own.name(),
                  plan.own.rows, plan.p.own_tiles, plan.p.own_splits, plan.prefix.name(), plan.prefix.rows, plan.p.prefix_tiles, plan.p.prefix_splits,
-                 plan.bytes);
+                 plan.bytes());
     }
     return 0;
 }

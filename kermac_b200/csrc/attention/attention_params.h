@@ -74,6 +74,11 @@ int  count_blocks(const AttentionParams& p, unsigned* blocks);
 constexpr int ATT_TENSOR_ROWS = 256;
 int  attention_tensor_launch(const AttentionParams& p, int type, cudaStream_t st);
 int  attention_tensor_take_wait_flag();
+// attention_tensor32.cu (tcgen05): float32, up to 64 channels, any layout, with attention_planes_bytes() of scratch (16-byte aligned).
+constexpr int ATT_TENSOR32_CHANNELS = 64;
+long long attention_planes_bytes(const AttentionParams& p);
+int  attention_tensor32_launch(const AttentionParams& p, void* planes, cudaStream_t st);
+int  attention_tensor32_take_wait_flag();
 // attention_grad_rows.cu
 constexpr int ATT_GRAD_ROWS = 64, ATT_PEAK_ROWS = 64;
 int  attention_delta_launch(const AttentionGradParams& p, int type, cudaStream_t st);
@@ -82,9 +87,23 @@ int  attention_grad_rows_launch(const AttentionGradParams& p, int type, cudaStre
 constexpr int ATT_GRAD_TENSOR_ROWS = 128;
 int  attention_grad_tensor_launch(const AttentionGradParams& p, int type, cudaStream_t st);
 int  attention_grad_tensor_take_wait_flag();
-// dst[i] = sum over slices of src[slice][i] for a [rows_l][rows][heads][D] array
-int  attention_reduce_launch(const float* src, int slices, const Heads& dst, int L, int rows, int heads, int D, int type,
-                             cudaStream_t st);
+// dst[l][row][head][c] = sum over the slices of src[slice][l][row][head][c], in their order; no slices: zeros.  Up to three in a launch.
+struct SliceSum {
+    const float* src;
+    Heads        dst;
+    int          slices, L, rows, heads, D;
+};
+struct SliceSums {
+    SliceSum  job[3];
+    long long first[4];                  // elements in front of each
+    int       count;
+    void add(const float* src, int slices, const Heads& dst, int L, int rows, int heads, int D) {
+        job[count]       = {src, dst, slices, L, rows, heads, D};
+        first[count + 1] = first[count] + static_cast<long long>(L) * rows * heads * D;
+        ++count;
+    }
+};
+int attention_reduce_launch(const SliceSums& sums, int type, cudaStream_t st);
 
 inline int padded_channels(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 inline int type_bytes(int type) { return type == ATT_F32 ? 4 : 2; }

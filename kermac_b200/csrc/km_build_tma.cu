@@ -33,6 +33,7 @@ namespace km {
 int attention_tensor_take_wait_flag();     // attention/attention_tensor.cu
 int attention_grad_tensor_take_wait_flag();
 int attention_few_take_wait_flag();
+int attention_tensor32_take_wait_flag();
 
 __device__ int g_tma_wait_expired = 0;
 
@@ -375,6 +376,7 @@ extern "C" int kermac_b200_device_error_flag(void) {
     const int av = km::attention_tensor_take_wait_flag();
     const int dv = km::attention_grad_tensor_take_wait_flag();
     const int fv = km::attention_few_take_wait_flag();
-    if (mv < 0 || gv < 0 || hv < 0 || sv < 0 || av < 0 || dv < 0 || fv < 0) return KM_ERR_INTERNAL;
-    return (v || mv || gv || hv || sv || av || dv || fv) ? 1 : 0;
+    const int tv = km::attention_tensor32_take_wait_flag();
+    if (mv < 0 || gv < 0 || hv < 0 || sv < 0 || av < 0 || dv < 0 || fv < 0 || tv < 0) return KM_ERR_INTERNAL;
+    return (v || mv || gv || hv || sv || av || dv || fv || tv) ? 1 : 0;
 }

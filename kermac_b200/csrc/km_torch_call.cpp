@@ -570,9 +570,13 @@ int launch_attention(KmAttentionArgs& args, AttentionKind kind, int device) {
     at::Tensor scratch;
     const int64_t need = g_lib.attention_scratch[kind](&args);
     if (need > 0) {
-        scratch            = new_float({need / 4}, device);
-        args.scratch       = scratch.data_ptr();
-        args.scratch_bytes = need;
+        try {
+            scratch            = new_float({need / 4}, device);
+            args.scratch       = scratch.data_ptr();
+            args.scratch_bytes = need;
+        } catch (const c10::OutOfMemoryError&) {      // there it only makes the call faster
+            if (kind != CROSS) throw;
+        }
     }
     return g_lib.attention[kind](&args, c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream());
 }

@@ -85,6 +85,55 @@ def test_the_c_abi_refuses(changes, kind, code):
         _native.describe_attention(args, kind)
 
 
+PLANS = [           # what kernel takes a call: changes of _c_args, kind, a part of the description
+    (dict(), 0, "own=few rows=8"),                                                 # 3 queries of 2 heads to a key head
+    (dict(n=4), 0, "own=few rows=8"),
+    (dict(n=8), 0, "own=few rows=16"),
+    (dict(n=9), 0, "own=tensor rows=256"),
+    (dict(d=7, n=9), 0, "own=rows rows=64"),                                       # rows that TMA cannot copy
+    (dict(d=7), 0, "own=scalar few"),
+    (dict(d=136, n=9), 0, "own=rows"),
+    (dict(k=("stride_row", 12)), 0, "own=scalar few"),
+    (dict(v=("ptr", 4098)), 0, "own=scalar few"),
+    (dict(type=0), 0, "own=scalar few"),
+    (dict(type=0, n=9), 0, "own=rows"),                                            # 5 keys
+    (dict(type=0, n=9, m=100), 0, "own=tensor32"),
+    (dict(type=0, n=9, m=100, d=65), 0, "own=rows"),
+    (dict(prefix=6), 1, "own=few rows=16 tiles=1 splits=1 prefix=few rows=16"),
+    (dict(n=9, prefix=6), 1, "own=tensor rows=256 tiles=1 splits=1 prefix=tensor rows=256 tiles=1 splits=1"),
+    (dict(), 2, "grad=tensor q_slices=1 kv_slices=1"),
+    (dict(type=0), 2, "grad=rows"),
+    (dict(d=7), 2, "grad=rows"),
+    (dict(type=0, m=5000), 2, "q_slices=37"),                                      # 8 query tiles for 296 blocks
+]
+
+
+@pytest.mark.parametrize("changes, kind, expected", PLANS, ids=str)
+def test_which_kernel_takes_a_call(changes, kind, expected):
+    args = _c_args(**changes)
+    if "n" in changes or "d" in changes or "m" in changes:                        # dense tensors of the new extents
+        for name, rows, heads in (("q", args.n, 4), ("k", args.m, 2), ("v", args.m, 2), ("out", args.n, 4), ("grad_out", args.n, 4),
+                                  ("grad_q", args.n, 4), ("grad_k", args.m, 2), ("grad_v", args.m, 2), ("k_prefix", 6, 2), ("v_prefix", 6, 2)):
+            setattr(args, name, _native.KmHeads(4096, rows * heads * args.d, heads * args.d, args.d))
+        args.lse_stride_l, args.lse_stride_head = 4 * args.n, args.n
+    assert expected in _native.describe_attention(args, kind), _native.describe_attention(args, kind)
+
+
+def test_scratch_is_bounded():
+    # 2^27 rows of partial sums would be 34 GB: a single piece takes none
+    args = _c_args(l=1, n=1 << 20, m=1 << 20, heads=1, key_heads=1, d=64)
+    for name in ("q", "k", "v", "out"):
+        setattr(args, name, _native.KmHeads(4096, 1 << 26, 64, 64))
+    args.lse_stride_l, args.lse_stride_head = 1 << 20, 1 << 20
+    assert _native.attention_scratch_bytes(args, 0) == 0
+    args.type = _native.TYPE_FLOAT32                                              # 1.2 GB of planes: not asked for
+    assert _native.attention_scratch_bytes(args, 0) == 0
+    args.m = 1 << 10
+    args.n = 1 << 10
+    planes = 3 * (1 << 10) * 64 * 6
+    assert planes <= _native.attention_scratch_bytes(args, 0) <= planes + 4 * (1 << 10) * 65 * 4 + 32
+
+
 def test_the_c_abi_refuses_no_arguments_at_all():
     for kind in range(3):
         assert getattr(_native.lib(), _native.ATTENTION_SYMBOLS[kind])(None, None) == -1

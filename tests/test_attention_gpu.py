@@ -166,6 +166,82 @@ def test_prefix(dtype, shape, D):
     assert _native.device_error_flag() == 0
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("H, Hk", [(3, 1), (10, 2), (8, 1), (6, 6)])
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_heads_of_a_group(dtype, H, Hk, D):
+    # groups of 3 and 5 do not divide a tile of 128 rows, groups of 8 and 1 do; an odd number of tiles
+    check_forward(dtype, 2, 129, 300, H, Hk, D, [300, 140])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("N", [1, 3])
+@pytest.mark.parametrize("spread", ["even", "uneven"])
+def test_prefix_below_queries_that_lie_apart(dtype, N, spread):
+    # queries cut out of a longer tensor: the distance between sequences is not N times that between tokens
+    L, M, P, H, Hk, D = 20, 40, 200, 8, 2, 64
+    whole = make(1, L, N + (2 if spread == "uneven" else 0), H, D, dtype=dtype)
+    q = whole[:, :N]
+    k, v = make(2, L, M, Hk, D, dtype=dtype), make(3, L, M, Hk, D, dtype=dtype)
+    kp, vp = make(4, P, Hk, D, dtype=dtype), make(5, P, Hk, D, dtype=dtype)
+    lengths = torch.tensor([(7 * l) % M + 1 for l in range(L)], dtype=torch.int32, device="cuda")
+    want, _, bound, _ = ao.attention(q, k, v, lengths, prefix=(kp, vp))
+    assert_within(kermac.prefix_attention(q, kp, vp, k, v, lengths=lengths), want, bound, "out")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("N, D", [(1, 64), (1, 128), (40, 64), (40, 128), (40, 200)])
+def test_without_scratch(dtype, N, D):
+    # a caller that gives no scratch gets the same rows from fewer blocks
+    from kermac_b200 import attention
+    L, M, H, Hk = 2, 1500, 4, 2
+    q, k, v = (make(s, L, n, h, D, dtype=dtype) for s, n, h in ((1, N, H), (2, M, Hk), (3, M, Hk)))
+    args, _ = attention._marshal(q, k, v, None, None)
+    out = torch.empty_like(q)
+    args.out = attention._heads(out)
+    assert _native.attention_scratch_bytes(args, _native.ATTENTION_CROSS) > 0
+    _native.launch_attention(args, _native.ATTENTION_CROSS, torch.cuda.current_stream().cuda_stream)
+    want, _, bound, _ = ao.attention(q, k, v)
+    assert_within(out, want, bound, "out")
+    # with both sets of keys the partial sums are needed, and the gradient needs its sums
+    args.prefix, args.k_prefix, args.v_prefix = 10, attention._heads(k[0, :10]), attention._heads(v[0, :10])
+    for kind in (_native.ATTENTION_PREFIX, _native.ATTENTION_GRAD):
+        args.lse, args.lse_stride_l, args.lse_stride_head = out.data_ptr(), H * N, N
+        args.q_batch = args.kv_batch = L
+        args.grad_out = args.grad_q = attention._heads(q)
+        args.grad_k = args.grad_v = attention._heads(k)
+        if kind == _native.ATTENTION_GRAD:
+            args.prefix = 0
+        with pytest.raises(ValueError, match="scratch"):
+            _native.launch_attention(args, kind, torch.cuda.current_stream().cuda_stream)
+
+
+def test_a_full_device_does_without(monkeypatch):
+    from test_grad_split_gpu import full_device
+    # the planes of float32 keys take 30 MB
+    q, k, v = (make(s, 1, n, 2, 64, dtype=torch.float32) for s, n in ((1, 40), (2, 20000), (3, 20000)))
+    want, _, bound, _ = ao.attention(q, k, v)
+    out = torch.empty_like(q)
+    with full_device():
+        kermac.cross_attention(q, k, v, out=out)
+    assert_within(out, want, bound, "out")
+
+
+def test_calls_on_two_streams_at_once():
+    dtype, L, N, M, H, D = torch.bfloat16, 2, 1, 3000, 8, 64
+    inputs = [[make(10 * i + s, L, n, H, D, dtype=dtype) for s, n in ((1, N), (2, M), (3, M))] for i in range(2)]
+    want = [kermac.cross_attention(*x).clone() for x in inputs]
+    streams = [torch.cuda.Stream() for _ in inputs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for x, stream in zip(inputs, streams):
+            with torch.cuda.stream(stream):
+                got.append(kermac.cross_attention(*x))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def check_grad(dtype, q, k, v, lengths, L, g_by=0.5, layout="nhd", scale=None):
     N, H, D = q.shape[-3:]
     lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
