@@ -2,7 +2,11 @@
 //
 // Two kinds of blocks, like the two kernels of attention_grad_rows.cu: one holds 128 keys and streams query tiles (dk, dv), one holds 128 queries and streams
 // key tiles (dq).  One launch has both, the longer ones (of keys) first, so that the SMs that have finished those go on with the others
-// (two launches: a training step of 8 x 512 x 1030 waited twice for its last blocks, 140 of 195 us).  Scores and dout v^T are in tensor memory, the weights and their gradients are written back over them as
+// (two launches: a training step of 8 x 512 x 1030 waited twice for its last blocks, 140 of 195 us).
+//
+// delta from the output as the forward pass rounded it is off by up to half a step of the output's terms, which shows where few keys
+// share a query: with 11 keys dq came out with 1.85 times the error of rounding alone, from 128 on with 1.5.  Where all keys are in one tile
+// the blocks of dq have every term of delta = sum p (dout v^T) at hand; they run first then, and there is no pass over out and dout.  Scores and dout v^T are in tensor memory, the weights and their gradients are written back over them as
 // 16-bit operands.  The keys' kernel computes both transposed, so that its operands need no transposition either: a
 // lane is a key there and a query in the other kernel.
 //
@@ -334,6 +338,7 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
     constexpr int KS = S::K_STAGES, VS = S::V_STAGES;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long s_bars[2 * KS + 2 * VS + 6];
+    __shared__ float s_part[2][TC_ROWS];
     __shared__ uint32_t s_tmem;
     __shared__ int s_expired;
     const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u, bars = smem_addr(s_bars);
@@ -375,9 +380,9 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
         const int      half = warp >> 2, n = n0 + (threadIdx.x & 127);
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, at = lanes + half * 64;
         const float    shift = n < p.N ? -p.lse[l * p.lse_sl + h * p.lse_sh + n] * (1.0f / LN2) : -INFINITY;
-        const float    delta = n < p.N ? -p.delta[(static_cast<long long>(l) * p.H + h) * p.N + n] * factor : 0.0f;
-        const u64      c2 = pack2(p.scale_log2, p.scale_log2), by2 = pack2(factor, factor), shift2 = pack2(shift, shift),
-                       delta2 = pack2(delta, delta);
+        const float    delta = n < p.N && !p.own_delta ? -p.delta[(static_cast<long long>(l) * p.H + h) * p.N + n] * factor : 0.0f;
+        const u64      c2 = pack2(p.scale_log2, p.scale_log2), by2 = pack2(factor, factor), shift2 = pack2(shift, shift);
+        u64            delta2 = pack2(delta, delta);
         for (int i = 0; i < n_items; ++i) {
             uint32_t w[64];
             wait(s_full(i & 1), (i >> 1) & 1);
@@ -407,6 +412,25 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
             }
             wait(dp_full, i & 1);
             tc::fence_after_sync();
+            if (p.own_delta) {
+                // all keys are in this tile: delta = sum_m p (dout v^T)
+                float part = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 64; j += 32) {
+                    uint32_t g[32];
+                    tmem_load32(dp_col + at + j, g);
+                    tmem_wait_load();
+                    tmem_loaded32(g);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (half * 64 + j + e < there) part = fmaf(__uint_as_float(w[j + e]), __uint_as_float(g[e]), part);
+                }
+                s_part[half][threadIdx.x & 127] = part;
+                asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+                const float all = s_part[0][threadIdx.x & 127] + s_part[1][threadIdx.x & 127];
+                if (half == 0 && n < p.N) p.delta[(static_cast<long long>(l) * p.H + h) * p.N + n] = all;
+                delta2 = pack2(-all * factor, -all * factor);
+            }
             uint32_t y[32];
 #pragma unroll
             for (int j = 0; j < 64; j += 32) {
@@ -520,8 +544,13 @@ int launch_grad_tensor(const AttentionGradParams& p, const GradMaps& maps, cudaS
     if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute")) return rc;
     const long long kb = ceil_div_ll(p.M, TC_ROWS) * p.kv_slices * p.Hk * p.kv_batch, qb = ceil_div_ll(p.N, TC_ROWS) * p.H * p.L;
     if (kb + qb > 0x7fffffffLL) return fail(KM_ERR_TOO_LARGE, "attention: more than 2^31 - 1 blocks");
-    return cuda_status(launch_overlapped(kernel, dim3(static_cast<unsigned>(kb + qb)), S::BLOCK, smem, st, p, maps, static_cast<int>(kb)),
-                       "attention_grad_tensor_kernel");
+    auto launch = [&](long long blocks, long long key_blocks) {
+        return cuda_status(launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks)), S::BLOCK, smem, st, p, maps, static_cast<int>(key_blocks)),
+                           "attention_grad_tensor_kernel");
+    };
+    if (!p.own_delta) return launch(kb + qb, kb);
+    if (int rc = launch(qb, 0)) return rc;               // first those that form delta
+    return launch(kb, kb);
 }
 
 }  // namespace

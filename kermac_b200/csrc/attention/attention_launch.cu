@@ -176,7 +176,7 @@ struct Plan {
 // keys: of the set; all_keys: of both.
 Form choose_form(long long rows, bool tma_ok, int type, int d, int keys, int all_keys, bool planes) {
     if (tma_ok && rows > 16) return {TENSOR, ATT_TENSOR_ROWS, 1, 256};
-    if (tma_ok) return {FEW, rows <= 8 ? 8 : 16, d <= 64 || attention_few_tile(d, keys, 0) == 16 ? 2 : 1, 256};
+    if (tma_ok) return {FEW, rows <= 8 ? 8 : 16, d <= 64 || attention_few_tile(d, keys, 0) == 16 ? 2 : 1, 128};
     if (rows <= ATT_FEW_ROWS) return {SCALAR_FEW, ATT_FEW_ROWS, 1, 256};
     if (planes && all_keys > 64) return {TENSOR32, ATT_TENSOR_ROWS, 1, 256};      // measured in attention_tensor32.cu
     return {ROWS, ATT_TILE_ROWS, type == ATT_F32 ? 4 : 2, 256};
@@ -229,7 +229,9 @@ Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool split, bool planes) 
         p.prefix_tiles  = static_cast<int>(ceil_div_ll(prefix_rows, plan.prefix.rows));
         p.prefix_splits = split ? pieces(static_cast<long long>(p.prefix_tiles) * p.Hk, p.P, plan.prefix.per_sm, plan.prefix.least) : 1;
     }
-    p.parts = p.own_splits + p.prefix_splits;
+    p.parts = p.own_splits + p.prefix_splits, p.cluster = 1;
+    if (p.parts > 1 && p.parts <= 8 && (p.own_splits == 0 || p.prefix_splits == 0) && (p.own_splits ? plan.own : plan.prefix).kernel == FEW)
+        p.cluster = p.parts, p.parts = 1;              // 8 blocks: the largest cluster that every GPU of this kind takes
     auto round16 = [](long long n) { return (n + 15) & ~15LL; };
     if (p.parts > 1) plan.parts = round16(static_cast<long long>(p.parts) * p.L * p.N * p.H * (p.D + 1) * 4);
     if ((p.own_splits > 0 && plan.own.kernel == TENSOR32) || (p.prefix_splits > 0 && plan.prefix.kernel == TENSOR32))
@@ -318,6 +320,7 @@ GradPlan plan_grad(const KmAttentionArgs& a) {
     p.vec_grad = rows_aligned(a.grad_q, a.type, a.d) && rows_aligned(a.grad_k, a.type, a.d) && rows_aligned(a.grad_v, a.type, a.d);
     plan.tensor = a.d <= 128 && tma_rows_ok(a.q, a.n, a.heads, a.type, a.d) && tma_rows_ok(a.grad_out, a.n, a.heads, a.type, a.d) &&
                   tma_rows_ok(a.k, a.m, a.key_heads, a.type, a.d) && tma_rows_ok(a.v, a.m, a.key_heads, a.type, a.d);
+    p.own_delta = plan.tensor && a.m <= ATT_GRAD_TENSOR_ROWS;
     // The sum over keys of a query tile is split where the query tiles alone do not fill the SMs (not on the tensor cores, where
     // the blocks of both sums run side by side and a piece would be a few tiles).
     p.q_splits = plan.tensor ? 1 : pieces(ceil_div_ll(a.n, ATT_GRAD_ROWS) * a.heads * a.l, a.m, 2, 128);
@@ -363,7 +366,7 @@ int gradient(const KmAttentionArgs* a, void* stream) {
     if (plan.peaks) p.peaks = at, at += plan.peaks;
     if (plan.dq) p.dq_part = at, at += plan.dq;
     if (plan.dkv) p.dk_part = at, p.dv_part = at + plan.dkv;
-    rc = attention_delta_launch(p, a->type, st);
+    if (!p.own_delta || p.peaks) rc = attention_delta_launch(p, a->type, st);
     if (!rc) rc = plan.tensor ? attention_grad_tensor_launch(p, a->type, st) : attention_grad_rows_launch(p, a->type, st);
     SliceSums sums = {};
     if (p.q_slices > 1) sums.add(p.dq_part, p.q_slices, p.dq, a->q_batch, p.N, p.H, p.D);

@@ -26,6 +26,7 @@ struct AttentionParams {
     int   own_tiles, own_splits;         // row tiles of one (l, key head), pieces of its keys; 0 pieces: no own keys
     int   prefix_tiles, prefix_splits;
     int   parts;                         // pieces of one row: own_splits + prefix_splits; 1: results are written directly
+    int   cluster;                       // FEW: blocks of a cluster that share a row's keys and join its pieces themselves; else 1
     float* part_o;                       // [part][l][n][h][D]
     float* part_lse;                     // [part][l][n][h], log2 domain
     int   vec;                           // every row of k, v, kp, vp and q can be read 16 bytes at a time
@@ -52,6 +53,7 @@ struct AttentionGradParams {
     int   q_splits;                      // pieces of the sum over keys
     int   kv_batch;                      // batch entries of k and v: 1 or L
     int   kv_slices;                     // pieces of the sum over (l of a broadcast k, head of the group, query tile)
+    int   own_delta;                     // tensor cores: the blocks of dq form delta, from weights of one key tile, for those of dk and dv
     int   vec;                           // rows of q, k, v and dout can be read 16 bytes at a time
     int   vec_out;                       // rows of out and dout can
     int   vec_grad;                      // rows of dq, dk and dv can be written so

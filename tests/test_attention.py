@@ -89,6 +89,7 @@ PLANS = [           # what kernel takes a call: changes of _c_args, kind, a part
     (dict(), 0, "own=few rows=8"),                                                 # 3 queries of 2 heads to a key head
     (dict(n=4), 0, "own=few rows=8"),
     (dict(n=8), 0, "own=few rows=16"),
+    (dict(n=4, m=1100), 0, "own=few rows=8 tiles=1 splits=8 prefix=few rows=16 tiles=0 splits=0 scratch=0"),    # joined in a cluster
     (dict(n=9), 0, "own=tensor rows=256"),
     (dict(d=7, n=9), 0, "own=rows rows=64"),                                       # rows that TMA cannot copy
     (dict(d=7), 0, "own=scalar few"),

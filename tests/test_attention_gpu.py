@@ -99,6 +99,18 @@ def test_split_keys(dtype, N, M):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M", [511, 512, 800, 1100, 1300, 1600, 1900, 2047, 2100, 2600])
+@pytest.mark.parametrize("D, Hk", [(64, 1), (128, 4)])
+def test_pieces_of_a_cluster(dtype, M, D, Hk):
+    # two to eight pieces of the keys of one token (joined inside the kernel for 16-bit types), and more; an entry without keys
+    check_forward(dtype, 3, 1, M, 4, Hk, D, [M, 0, 300])
+    q, kp, vp = make(1, 5, 1, 4, D, dtype=dtype), make(2, M, Hk, D, dtype=dtype), make(3, M, Hk, D, dtype=dtype)
+    none = torch.zeros(5, 0, Hk, D, dtype=dtype, device="cuda")
+    want, _, bound, _ = ao.attention(q, none, none, prefix=(kp, vp))
+    assert_within(kermac.prefix_attention(q, kp, vp, none, none), want, bound, "a prefix alone")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("N", [1, 256])
 @pytest.mark.parametrize("scale, by", [(0.0, 1.0), (3.0, 2.0), (0.125, 30.0)])
 def test_scales(dtype, N, scale, by):
@@ -194,7 +206,7 @@ def test_prefix_below_queries_that_lie_apart(dtype, N, spread):
 def test_without_scratch(dtype, N, D):
     # a caller that gives no scratch gets the same rows from fewer blocks
     from kermac_b200 import attention
-    L, M, H, Hk = 2, 1500, 4, 2
+    L, M, H, Hk = 2, 4000 if N == 1 else 1500, 4, 2
     q, k, v = (make(s, L, n, h, D, dtype=dtype) for s, n, h in ((1, N, H), (2, M, Hk), (3, M, Hk)))
     args, _ = attention._marshal(q, k, v, None, None)
     out = torch.empty_like(q)
