@@ -1,7 +1,7 @@
 // Gradient of the attention of 16-bit tensors on the tensor cores (tcgen05), head widths up to 128.
 //
 // Two kinds of blocks, like the two kernels of attention_grad_rows.cu: one holds 128 keys and streams query tiles (dk, dv), one holds 128 queries and streams
-// key tiles (dq).  One launch has both, the longer ones (of keys) first, so that the SMs that have finished those go on with the others
+// key tiles (dq).  One launch has both, the longer ones first, so that the SMs that have finished those go on with the others
 // (two launches: a training step of 8 x 512 x 1030 waited twice for its last blocks, 140 of 195 us).
 //
 // delta from the output as the forward pass rounded it is off by up to half a step of the output's terms, which shows where few keys
@@ -142,8 +142,8 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
     const int l_count = p.kv_batch == 1 ? p.L : 1, l_first = p.kv_batch == 1 ? 0 : kl;
     const int q_tiles = (p.N + TC_ROWS - 1) / TC_ROWS;
     const int all     = l_count * p.G * q_tiles;
-    const int from    = static_cast<int>(static_cast<long long>(all) * slice / p.kv_slices);
-    const int to      = static_cast<int>(static_cast<long long>(all) * (slice + 1) / p.kv_slices);
+    const int each = all / p.kv_slices, more = all % p.kv_slices;       // the first `more` pieces have one item more
+    const int from = slice * each + min(slice, more), to = from + each + (slice < more);
     int longest = 0;                               // keys from here on are in no sum of this block: their gradient is zero
     if (from < to)
         for (int l = l_first + from / (p.G * q_tiles); l <= l_first + (to - 1) / (p.G * q_tiles); ++l)
@@ -362,9 +362,12 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
 
     const int tiles = (p.N + TC_ROWS - 1) / TC_ROWS;
     const int n0 = block % tiles * TC_ROWS; block /= tiles;
+    const int split = block % p.q_splits;   block /= p.q_splits;
     const int h = block % p.H, l = block / p.H, hk = h / p.G;
     const int kl = p.kv_batch == 1 ? 0 : l;
-    const int count = key_count(p.lengths, p.lengths_stride, l, p.M), n_items = (count + TC_ROWS - 1) / TC_ROWS;
+    // this block's piece of the keys: tiles [first, first + n_items)
+    const int count = key_count(p.lengths, p.lengths_stride, l, p.M), key_tiles = (count + TC_ROWS - 1) / TC_ROWS;
+    const int first = key_tiles * split / p.q_splits, n_items = key_tiles * (split + 1) / p.q_splits - first;      // at most 2^23 tiles, 64 pieces
 
     tc::fence_before_sync();
     __syncthreads();
@@ -398,7 +401,7 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
                 unpack2(fma2(pack2(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), c2, shift2), x, y);
                 w[j] = __float_as_uint(ex2_approx(x)), w[j + 1] = __float_as_uint(ex2_approx(y));
             }
-            const int  there = count - i * TC_ROWS;                    // keys of this tile
+            const int  there = count - (first + i) * TC_ROWS;          // keys of this tile
             const bool tail  = there < TC_ROWS;
             if (tail && count < p.M) {
                 // rows of k behind the length hold whatever the memory holds, and 0 * NaN is NaN
@@ -461,14 +464,16 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
             tc::fence_after_sync();
         }
         const bool   good = n < p.N && *reinterpret_cast<volatile int*>(&s_expired) == 0;
-        float* const part = p.q_slices > 1 ? p.dq_part + static_cast<long long>(l) * p.N * p.H * p.D : nullptr;    // q_splits is 1
+        // partial sums [slice][entry of q][n][h][D]: a broadcast q has one entry and a slice for each l and piece
+        const bool   one_q = p.q_slices > p.q_splits;
+        float* const part = p.q_slices > 1 ? p.dq_part + static_cast<long long>(one_q ? l * p.q_splits + split : split * p.L) * p.N * p.H * p.D : nullptr;
         if (n_items > 0) {
             if (half == 0) {                 // the warps of the first half write whole rows, where q was held
                 char* const stage = reinterpret_cast<char*>(smem_raw) + (held_q - raw) + warp * 4096;
-                put_sums<T, DP>(dq_col + lanes, stage, p.dq, part, p.vec_grad, good, part ? 0 : l, n, h, p.N, p.H, p.D, p.scale / factor);
+                put_sums<T, DP>(dq_col + lanes, stage, p.dq, part, p.vec_grad, good, one_q ? 0 : l, n, h, p.N, p.H, p.D, p.scale / factor);
             }
         } else if (half == 0) {
-            put_zeros<T>(p.dq, part, p.vec_grad, good, part ? 0 : l, n, h, p.N, p.H, p.D);
+            put_zeros<T>(p.dq, part, p.vec_grad, good, one_q ? 0 : l, n, h, p.N, p.H, p.D);
         }
     } else if (warp == S::LOAD_WARP) {
         // ------------------------------------------------------------------ copies
@@ -480,10 +485,10 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
                 const int ks = i % KS, vs = i % VS;
                 if (i >= KS) wait(k_empty(ks), (i / KS - 1) & 1);
                 mbar_expect_tx(k_full(ks), S::TILE);
-                load_tile<DP>(ring_k + ks * S::TILE, &maps.k, i * TC_ROWS, hk, p.k.sl == 0 ? 0 : kl, k_full(ks));
+                load_tile<DP>(ring_k + ks * S::TILE, &maps.k, (first + i) * TC_ROWS, hk, p.k.sl == 0 ? 0 : kl, k_full(ks));
                 if (i >= VS) wait(v_empty(vs), (i / VS - 1) & 1);
                 mbar_expect_tx(v_full(vs), S::TILE);
-                load_tile<DP>(ring_v + vs * S::TILE, &maps.v, i * TC_ROWS, hk, p.v.sl == 0 ? 0 : kl, v_full(vs));
+                load_tile<DP>(ring_v + vs * S::TILE, &maps.v, (first + i) * TC_ROWS, hk, p.v.sl == 0 ? 0 : kl, v_full(vs));
             }
             wait.drain(held_full, 0);
             for (int i = max(0, n_items - KS); i < n_items; ++i) wait.drain(k_full(i % KS), (i / KS) & 1);
@@ -527,12 +532,15 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(GradTensorShape<DP>::BLOCK, 1)
-attention_grad_tensor_kernel(const __grid_constant__ AttentionGradParams p, const __grid_constant__ GradMaps maps, const int key_blocks) {
+attention_grad_tensor_kernel(const __grid_constant__ AttentionGradParams p, const __grid_constant__ GradMaps maps, const int first_blocks,
+                             const int keys_first) {
     after_previous_grid();
-    if (static_cast<int>(blockIdx.x) < key_blocks)
-        gradient_of_keys<T, DP>(p, maps, blockIdx.x);
+    const bool first = static_cast<int>(blockIdx.x) < first_blocks;
+    const int  block = first ? blockIdx.x : blockIdx.x - first_blocks;
+    if (first == (keys_first != 0))
+        gradient_of_keys<T, DP>(p, maps, block);
     else
-        gradient_of_queries<T, DP>(p, maps, blockIdx.x - key_blocks);
+        gradient_of_queries<T, DP>(p, maps, block);
 }
 
 template <typename T, int DP>
@@ -542,15 +550,16 @@ int launch_grad_tensor(const AttentionGradParams& p, const GradMaps& maps, cudaS
     static_assert(smem <= 227 * 1024, "more shared memory than a block has");
     auto* const kernel = &attention_grad_tensor_kernel<T, DP>;
     if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute")) return rc;
-    const long long kb = ceil_div_ll(p.M, TC_ROWS) * p.kv_slices * p.Hk * p.kv_batch, qb = ceil_div_ll(p.N, TC_ROWS) * p.H * p.L;
+    const long long kb = ceil_div_ll(p.M, TC_ROWS) * p.kv_slices * p.Hk * p.kv_batch, qb = ceil_div_ll(p.N, TC_ROWS) * p.q_splits * p.H * p.L;
     if (kb + qb > 0x7fffffffLL) return fail(KM_ERR_TOO_LARGE, "attention: more than 2^31 - 1 blocks");
-    auto launch = [&](long long blocks, long long key_blocks) {
-        return cuda_status(launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks)), S::BLOCK, smem, st, p, maps, static_cast<int>(key_blocks)),
+    auto launch = [&](long long first, long long then, bool keys_first) {
+        return cuda_status(launch_overlapped(kernel, dim3(static_cast<unsigned>(first + then)), S::BLOCK, smem, st, p, maps, static_cast<int>(first),
+                                             static_cast<int>(keys_first)),
                            "attention_grad_tensor_kernel");
     };
-    if (!p.own_delta) return launch(kb + qb, kb);
-    if (int rc = launch(qb, 0)) return rc;               // first those that form delta
-    return launch(kb, kb);
+    if (!p.own_delta) return p.keys_first ? launch(kb, qb, true) : launch(qb, kb, false);
+    if (int rc = launch(qb, 0, false)) return rc;        // first those that form delta
+    return launch(kb, 0, true);
 }
 
 }  // namespace

@@ -321,17 +321,33 @@ GradPlan plan_grad(const KmAttentionArgs& a) {
     plan.tensor = a.d <= 128 && tma_rows_ok(a.q, a.n, a.heads, a.type, a.d) && tma_rows_ok(a.grad_out, a.n, a.heads, a.type, a.d) &&
                   tma_rows_ok(a.k, a.m, a.key_heads, a.type, a.d) && tma_rows_ok(a.v, a.m, a.key_heads, a.type, a.d);
     p.own_delta = plan.tensor && a.m <= ATT_GRAD_TENSOR_ROWS;
-    // The sum over keys of a query tile is split where the query tiles alone do not fill the SMs (not on the tensor cores, where
-    // the blocks of both sums run side by side and a piece would be a few tiles).
-    p.q_splits = plan.tensor ? 1 : pieces(ceil_div_ll(a.n, ATT_GRAD_ROWS) * a.heads * a.l, a.m, 2, 128);
-    if (static_cast<long long>(p.q_splits) * a.l * a.n * a.heads * a.d > (MOST_SCRATCH >> 3)) p.q_splits = 1;
-    p.q_slices = (a.q_batch == 1 && a.l > 1 ? a.l : 1) * p.q_splits;
     p.kv_batch = a.kv_batch;
-    // The sum over queries of a key tile is split where the key tiles alone do not fill the SMs.
-    const long long tiles = ceil_div_ll(a.m, plan.tensor ? ATT_GRAD_TENSOR_ROWS : ATT_GRAD_ROWS) * a.key_heads * a.kv_batch;
-    const long long sum   = static_cast<long long>(a.kv_batch == 1 ? a.l : 1) * p.G * a.n;
-    p.kv_slices = plan.tensor ? pieces(tiles, sum, 1, 512) : pieces(tiles, sum, 2, 128);
+    const long long key_sums = static_cast<long long>(a.kv_batch == 1 ? a.l : 1) * p.G;       // heads and entries whose queries a key meets
+    if (plan.tensor) {
+        // Both sums are split to fill the SMs, in pieces of at least four tiles of 128, and so that no block runs on for long when all the others
+        // have ended (us: 1.9 and 1.4 a tile, 5 to start and end; a split that is not there anyway costs a launch that adds up, so it has to
+        // save some 25).  Training steps: 13 queries of 4 x 4064 keys (one head of 112) 83 -> 52 us, 9 of 4396 (32 heads of 40) 92 -> 72; but
+        // split to 12 us, one of 15 queries of 1244 keys (40 heads), whose blocks then start in two rounds, 43 -> 52.
+        const long long key_tiles = ceil_div_ll(a.m, ATT_GRAD_TENSOR_ROWS), query_tiles = ceil_div_ll(a.n, ATT_GRAD_TENSOR_ROWS);
+        const long long key_blocks = key_tiles * a.key_heads * a.kv_batch, query_blocks = query_tiles * a.heads * a.l, sms = sm_count();
+        const double    of_keys = 1.9 * key_sums * query_tiles, of_queries = 1.4 * key_tiles;
+        const double    busy = (key_blocks * (of_keys + 5.0) + query_blocks * (of_queries + 5.0)) / sms, target = std::max(1.5 * busy, 25.0);
+        auto split = [&](long long blocks, long long others, long long tiles, double time) {
+            if (blocks <= 0) return 1;                       // nothing to sum
+            const long long fill = std::min((sms - others) / blocks, tiles / 4), even = static_cast<long long>(std::ceil(time / target));
+            return static_cast<int>(std::min(std::max({1LL, fill, even}), 64LL));
+        };
+        p.kv_slices = split(key_blocks, p.own_delta ? 0 : query_blocks, key_sums * query_tiles, of_keys);
+        p.q_splits  = p.own_delta ? 1 : split(query_blocks, key_blocks * p.kv_slices, key_tiles, of_queries);
+        p.keys_first = of_keys / p.kv_slices >= of_queries / p.q_splits;
+    } else {
+        // pieces of both sums where their tiles alone do not fill the SMs
+        p.kv_slices = pieces(ceil_div_ll(a.m, ATT_GRAD_ROWS) * a.key_heads * a.kv_batch, key_sums * a.n, 2, 128);
+        p.q_splits  = pieces(ceil_div_ll(a.n, ATT_GRAD_ROWS) * a.heads * a.l, a.m, 2, 128);
+    }
+    if (static_cast<long long>(p.q_splits) * a.l * a.n * a.heads * a.d > (MOST_SCRATCH >> 3)) p.q_splits = 1;
     if (static_cast<long long>(p.kv_slices) * a.kv_batch * a.m * a.key_heads * a.d > (MOST_SCRATCH >> 3)) p.kv_slices = 1;
+    p.q_slices = (a.q_batch == 1 && a.l > 1 ? a.l : 1) * p.q_splits;
     plan.delta = round4(static_cast<long long>(a.l) * a.heads * a.n);
     if (a.type == ATT_F16) {
         p.peak_count = static_cast<int>(ceil_div_ll(a.n, ATT_PEAK_ROWS));

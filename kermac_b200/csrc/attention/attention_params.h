@@ -53,6 +53,7 @@ struct AttentionGradParams {
     int   q_splits;                      // pieces of the sum over keys
     int   kv_batch;                      // batch entries of k and v: 1 or L
     int   kv_slices;                     // pieces of the sum over (l of a broadcast k, head of the group, query tile)
+    int   keys_first;                    // tensor cores: blocks of dk and dv are the longer ones
     int   own_delta;                     // tensor cores: the blocks of dq form delta, from weights of one key tile, for those of dk and dv
     int   vec;                           // rows of q, k, v and dout can be read 16 bytes at a time
     int   vec_out;                       // rows of out and dout can

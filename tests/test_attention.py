@@ -120,6 +120,15 @@ def test_which_kernel_takes_a_call(changes, kind, expected):
     assert expected in _native.describe_attention(args, kind), _native.describe_attention(args, kind)
 
 
+@pytest.mark.parametrize("kind", [0, 1, 2])
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("changes", [dict(m=0), dict(n=0), dict(heads=0), dict(l=0, q_batch=0, kv_batch=0), dict(m=0, n=0)], ids=str)
+def test_empty_extents_have_a_plan(kind, dtype, changes):
+    args = _c_args(type=dtype, **changes)
+    assert _native.describe_attention(args, kind)
+    assert _native.attention_scratch_bytes(args, kind) >= 0
+
+
 def test_scratch_is_bounded():
     # 2^27 rows of partial sums would be 34 GB: a single piece takes none
     args = _c_args(l=1, n=1 << 20, m=1 << 20, heads=1, key_heads=1, d=64)
