@@ -218,6 +218,11 @@ Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool split, bool planes) 
     const long long own_rows = static_cast<long long>(p.N) * p.G, prefix_rows = own_rows * p.L;
     plan.own    = choose_form(own_rows, own_ok, a.type, p.D, p.M, p.M + p.P, planes);
     plan.prefix = choose_form(prefix_rows, prefix_ok, a.type, p.D, p.P, p.M + p.P, planes);
+    // A short prefix goes along with few own rows: its keys are read again, from L2, for every 8 or 16 rows, which costs less than a launch
+    // of its own up to some 8 MB (72 sequences with 64 keys before 40 own ones, 2 key heads of 128: 19.2 -> 11.9 us; 1024 keys, 24 MB: 23.4
+    // and 22.2; 4096: 23.6 and 39.0).
+    const double again = plan.own.kernel == FEW ? static_cast<double>(ceil_div_ll(prefix_rows, plan.own.rows)) * p.Hk * p.P * p.D * 4 : 0.0;
+    if (p.M > 0 && p.P > 0 && plan.own.kernel == FEW && plan.prefix.kernel == TENSOR && again <= 8e6) plan.prefix = plan.own;
     // one launch for both sets where the same kernel takes them
     if (p.M > 0 && p.P > 0 && plan.own.kernel == FEW && plan.prefix.kernel == FEW)
         plan.own.rows = plan.prefix.rows = std::max(plan.own.rows, plan.prefix.rows);

@@ -101,6 +101,8 @@ PLANS = [           # what kernel takes a call: changes of _c_args, kind, a part
     (dict(type=0, n=9, m=100), 0, "own=tensor32"),
     (dict(type=0, n=9, m=100, d=65), 0, "own=rows"),
     (dict(prefix=6), 1, "own=few rows=16 tiles=1 splits=1 prefix=few rows=16"),
+    (dict(l=8, prefix=6), 1, "own=few rows=8 tiles=1 splits=1 prefix=few rows=8 tiles=6 splits=1"),        # 48 rows of a short prefix
+    (dict(l=8, prefix=1 << 20), 1, "own=few rows=8 tiles=1 splits=1 prefix=tensor rows=256 tiles=1"),
     (dict(n=9, prefix=6), 1, "own=tensor rows=256 tiles=1 splits=1 prefix=tensor rows=256 tiles=1 splits=1"),
     (dict(), 2, "grad=tensor q_slices=1 kv_slices=1"),
     (dict(type=0), 2, "grad=rows"),
