@@ -177,9 +177,11 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
 
 // Adds up the parts of a row, in a fixed order: out = sum_i 2^(lse_i - lse) o_i.  One warp a row, or WIDE four that take every fourth
 // part each (48 rows of 72 parts, 3 sequences below a prefix of 18192: 28 us with one warp; 4096 rows of 10 parts: 9 us more with four).
-template <typename T, bool WIDE>
+// A lane has four neighbouring channels, or single ones 32 apart where rows are no multiple of four (V = 1); loads are predicated,
+// not branched around, so that those of eight parts are under way at once (4096 rows of 10 parts of 128 channels: 16 -> 11 us).
+template <typename T, bool WIDE, int V>
 __global__ void __launch_bounds__(THREADS) attention_join_kernel(const AttentionParams p) {
-    constexpr int STEP = WIDE ? WARPS : 1;
+    constexpr int STEP = WIDE ? WARPS : 1, SETS = 256 / (32 * V);
     __shared__ float s_sum[WARPS][256], s_total[WARPS];
     after_previous_grid();
     const int       lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -190,35 +192,51 @@ __global__ void __launch_bounds__(THREADS) attention_join_kernel(const Attention
 #pragma unroll
     for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
     const float base = best == -INFINITY ? 0.0f : best;
-    float total = 0.0f, x[8];
+    float total = 0.0f, x[SETS][V];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) x[c] = 0.0f;
+    for (int c = 0; c < SETS; ++c)
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[c][e] = 0.0f;
     for (int i0 = WIDE ? warp : 0; i0 < p.parts; i0 += 32 * STEP) {
         // a lane's part; one without keys has weight 0 and has written no sum
         const float mine = i0 + lane * STEP < p.parts ? ex2_approx(p.part_lse[(i0 + lane * STEP) * rows + row] - base) : 0.0f;
         total += mine;
         const int    many = min(32, (p.parts - i0 + STEP - 1) / STEP);
-        const float* from = p.part_o + (i0 * rows + row) * p.D + lane;
-#pragma unroll 4
+        const float* from = p.part_o + (i0 * rows + row) * p.D + lane * V;
+#pragma unroll 8
         for (int i = 0; i < many; ++i, from += STEP * rows * p.D) {
             const float weight = __shfl_sync(0xffffffffu, mine, i);
-            if (weight == 0.0f) continue;
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                if (c * 32 + lane < p.D) x[c] += weight * from[c * 32];
+            for (int c = 0; c < SETS; ++c) {
+                const bool there = weight != 0.0f && (c * 32 + lane) * V < p.D;
+                if constexpr (V == 4) {
+                    const float4 v = there ? *reinterpret_cast<const float4*>(from + c * 32 * V) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    x[c][0] = fmaf(weight, v.x, x[c][0]), x[c][1] = fmaf(weight, v.y, x[c][1]);
+                    x[c][2] = fmaf(weight, v.z, x[c][2]), x[c][3] = fmaf(weight, v.w, x[c][3]);
+                } else {
+                    x[c][0] = fmaf(weight, there ? from[c * 32] : 0.0f, x[c][0]);
+                }
+            }
         }
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
     if constexpr (WIDE) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) s_sum[warp][c * 32 + lane] = x[c];
+        for (int c = 0; c < SETS; ++c)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s_sum[warp][(c * 32 + lane) * V + e] = x[c][e];
         if (lane == 0) s_total[warp] = total;
         __syncthreads();
         if (warp != 0) return;
         total = (s_total[0] + s_total[1]) + (s_total[2] + s_total[3]);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) x[c] = (s_sum[0][c * 32 + lane] + s_sum[1][c * 32 + lane]) + (s_sum[2][c * 32 + lane] + s_sum[3][c * 32 + lane]);
+        for (int c = 0; c < SETS; ++c)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const int at = (c * 32 + lane) * V + e;
+                x[c][e] = (s_sum[0][at] + s_sum[1][at]) + (s_sum[2][at] + s_sum[3][at]);
+            }
     }
     const int       h = static_cast<int>(row % p.H);
     const long long ln = row / p.H;
@@ -226,8 +244,20 @@ __global__ void __launch_bounds__(THREADS) attention_join_kernel(const Attention
     const float     by = total == 0.0f ? 0.0f : 1.0f / total;
     T* const        o  = reinterpret_cast<T*>(p.out.ptr) + l * p.out.sl + n * p.out.sr + h * p.out.sh;
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
-        if (c * 32 + lane < p.D) o[c * 32 + lane] = Type<T>::to(x[c] * by);
+    for (int c = 0; c < SETS; ++c) {
+        const int at = (c * 32 + lane) * V;
+        if (at >= p.D) continue;
+        alignas(16) T y[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] = Type<T>::to(x[c][e] * by);
+        if (V == 4 && p.vec_out) {
+            if constexpr (V == 4 && sizeof(T) == 2) *reinterpret_cast<uint2*>(o + at) = *reinterpret_cast<const uint2*>(y);
+            if constexpr (V == 4 && sizeof(T) == 4) *reinterpret_cast<uint4*>(o + at) = *reinterpret_cast<const uint4*>(y);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[at + e] = y[e];
+        }
+    }
     if (p.lse && lane == 0) p.lse[l * p.lse_sl + h * p.lse_sh + n] = (best + lg2_approx(total)) * LN2;
 }
 
@@ -262,11 +292,15 @@ int attention_rows_launch(const AttentionParams& p, int type, bool few, cudaStre
 
 namespace att {
 namespace {
-template <typename T>
+template <typename T, int V>
 cudaError_t launch_join(const AttentionParams& p, cudaStream_t st) {
     const long long rows = static_cast<long long>(p.L) * p.N * p.H;              // below 2^31: checked
-    if (p.parts > 16) return launch_overlapped(&attention_join_kernel<T, true>, dim3(static_cast<unsigned>(rows)), THREADS, 0, st, p);
-    return launch_overlapped(&attention_join_kernel<T, false>, dim3(static_cast<unsigned>(ceil_div_ll(rows, WARPS))), THREADS, 0, st, p);
+    if (p.parts > 16) return launch_overlapped(&attention_join_kernel<T, true, V>, dim3(static_cast<unsigned>(rows)), THREADS, 0, st, p);
+    return launch_overlapped(&attention_join_kernel<T, false, V>, dim3(static_cast<unsigned>(ceil_div_ll(rows, WARPS))), THREADS, 0, st, p);
+}
+template <typename T>
+cudaError_t launch_join(const AttentionParams& p, cudaStream_t st) {
+    return p.D % 4 == 0 ? launch_join<T, 4>(p, st) : launch_join<T, 1>(p, st);
 }
 }  // namespace
 }  // namespace att
