@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(THREADS) attention_few_kernel(const __grid_con
                 }
             const Row   row = find_row(p, w, w.row0 + r);
             const float by  = total == 0.0f ? 0.0f : 1.0f / total;
-            if (c == 0) put_lse(p, w, row, best + lg2_approx(total));
+            if (c == 0) put_stats(p, w, row, best, total);
             put_pair<T>(p, w, row, c, x * by, y * by);
         }
     };

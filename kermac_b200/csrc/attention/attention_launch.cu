@@ -238,7 +238,7 @@ Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool split, bool planes) 
     if (p.parts > 1 && p.parts <= 8 && (p.own_splits == 0 || p.prefix_splits == 0) && (p.own_splits ? plan.own : plan.prefix).kernel == FEW)
         p.cluster = p.parts, p.parts = 1;              // 8 blocks: the largest cluster that every GPU of this kind takes
     auto round16 = [](long long n) { return (n + 15) & ~15LL; };
-    if (p.parts > 1) plan.parts = round16(static_cast<long long>(p.parts) * p.L * p.N * p.H * (p.D + 1) * 4);
+    if (p.parts > 1) plan.parts = round16(static_cast<long long>(p.parts) * p.L * p.N * p.H * (p.D + 2) * 4);
     if ((p.own_splits > 0 && plan.own.kernel == TENSOR32) || (p.prefix_splits > 0 && plan.prefix.kernel == TENSOR32))
         plan.planes = round16(attention_planes_bytes(p));
     return plan;
@@ -280,7 +280,7 @@ int forward(const KmAttentionArgs* a, Kind kind, void* stream) {
         if (!a->scratch || a->scratch_bytes < plan.bytes() || !aligned16(a->scratch))
             return fail(KM_ERR_NULL_POINTER, "attention: %lld bytes of 16-byte aligned scratch are needed", plan.bytes());
         plan.p.part_o   = static_cast<float*>(a->scratch);
-        plan.p.part_lse = plan.p.part_o + static_cast<long long>(plan.p.parts) * plan.p.L * plan.p.N * plan.p.H * plan.p.D;
+        plan.p.part_top = plan.p.part_o + static_cast<long long>(plan.p.parts) * plan.p.L * plan.p.N * plan.p.H * plan.p.D;
     }
     auto launch = [&](const AttentionParams& p, const Form& form) {
         if (form.kernel == TENSOR) return attention_tensor_launch(p, a->type, st);

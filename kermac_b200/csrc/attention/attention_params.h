@@ -15,7 +15,7 @@ struct Heads {
 // Forward pass.  For one batch entry and key head the G = H / Hk query heads of N queries are N * G rows (row = n * G + g)
 // against the entry's own keys; against a shared prefix the rows of all batch entries are one matrix (row =
 // (l * N + n) * G + g), so its keys are read once for the whole batch.  Each of the two sets of keys may be split among
-// blocks; every piece leaves a normalised sum and its log2-sum-exp2 (a "part"), which join_kernel adds up.
+// blocks; every piece leaves a normalised sum with its maximum and weight (a "part"), which join_kernel adds up.
 struct AttentionParams {
     int L, N, H, Hk, G, D, M, P;
     Heads q, k, v, kp, vp, out;
@@ -28,7 +28,7 @@ struct AttentionParams {
     int   parts;                         // pieces of one row: own_splits + prefix_splits; 1: results are written directly
     int   cluster;                       // FEW: blocks of a cluster that share a row's keys and join its pieces themselves; else 1
     float* part_o;                       // [part][l][n][h][D]
-    float* part_lse;                     // [part][l][n][h], log2 domain
+    float* part_top;                     // [2][part][l][n][h]: maximum (log2 domain), sum of exp2 of what lies below it
     int   vec;                           // every row of k, v, kp, vp and q can be read 16 bytes at a time
     int   vec_out;                       // rows of out can be written 16 bytes at a time
 };

@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
             if (at >= w.rows) continue;
             const Row   row = find_row(p, w, at);
             const float by  = sum[r] == 0.0f ? 0.0f : 1.0f / sum[r];
-            if (t == 0) put_lse(p, w, row, top[r] + lg2_approx(sum[r]));
+            if (t == 0) put_stats(p, w, row, top[r], sum[r]);
 #pragma unroll
             for (int c = 0; c < CT; ++c) put_pair<T>(p, w, row, c * 8 + 2 * t, o[c][2 * r] * by, o[c][2 * r + 1] * by);
         }
@@ -169,13 +169,13 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
             }
             const Row   row = find_row(p, w, w.row0 + r);
             const float by  = total == 0.0f ? 0.0f : 1.0f / total;
-            if (c == 0) put_lse(p, w, row, best + lg2_approx(total));
+            if (c == 0) put_stats(p, w, row, best, total);
             put_pair<T>(p, w, row, c, x * by, y * by);
         }
     }
 }
 
-// Adds up the parts of a row, in a fixed order: out = sum_i 2^(lse_i - lse) o_i.  One warp a row, or WIDE four that take every fourth
+// Adds up the parts of a row, in a fixed order: out = sum_i 2^(top_i) sum_i o_i / sum_i 2^(top_i) sum_i.  One warp a row, or WIDE four that take every fourth
 // part each (48 rows of 72 parts, 3 sequences below a prefix of 18192: 28 us with one warp; 4096 rows of 10 parts: 9 us more with four).
 // A lane has four neighbouring channels, or single ones 32 apart where rows are no multiple of four (V = 1); loads are predicated,
 // not branched around, so that those of eight parts are under way at once (4096 rows of 10 parts of 128 channels: 16 -> 11 us).
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(THREADS) attention_join_kernel(const Attention
     const long long rows = static_cast<long long>(p.L) * p.N * p.H, row = static_cast<long long>(blockIdx.x) * (WARPS / STEP) + (WIDE ? 0 : warp);
     if (row >= rows) return;                 // WIDE: a block has one row, which is there
     float best = -INFINITY;
-    for (int i = lane; i < p.parts; i += 32) best = fmaxf(best, p.part_lse[i * rows + row]);
+    for (int i = lane; i < p.parts; i += 32) best = fmaxf(best, p.part_top[i * rows + row]);
 #pragma unroll
     for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
     const float base = best == -INFINITY ? 0.0f : best;
@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(THREADS) attention_join_kernel(const Attention
         for (int e = 0; e < V; ++e) x[c][e] = 0.0f;
     for (int i0 = WIDE ? warp : 0; i0 < p.parts; i0 += 32 * STEP) {
         // a lane's part; one without keys has weight 0 and has written no sum
-        const float mine = i0 + lane * STEP < p.parts ? ex2_approx(p.part_lse[(i0 + lane * STEP) * rows + row] - base) : 0.0f;
+        const int   part = i0 + lane * STEP;
+        const float mine = part < p.parts ? ex2_approx(p.part_top[part * rows + row] - base) * p.part_top[(p.parts + part) * rows + row] : 0.0f;
         total += mine;
         const int    many = min(32, (p.parts - i0 + STEP - 1) / STEP);
         const float* from = p.part_o + (i0 * rows + row) * p.D + lane * V;

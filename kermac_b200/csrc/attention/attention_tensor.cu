@@ -192,7 +192,7 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
             tc::fence_after_sync();
             const bool  good = *reinterpret_cast<volatile int*>(&s_expired) == 0 && at < w.rows;
             const float by  = sum == 0.0f ? 0.0f : 1.0f / sum;
-            if (good) put_lse(p, w, row, top * c + lg2_approx(sum));
+            if (good) put_stats(p, w, row, top * c, sum);
             if (p.parts > 1 || p.vec_out) {
                 // the warp's rows of Q have been used for the last time
                 char* const stage = tiles + t * S::TILE + (warp & 3) * 4096;
@@ -215,7 +215,7 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
             }
         } else if (t < groups && at < w.rows) {          // no keys
             const Row row = find_row(p, w, at);
-            put_lse(p, w, row, -INFINITY);
+            put_stats(p, w, row, -INFINITY, 0.0f);
             if (p.parts == 1)
                 for (int j = 0; j < p.D; j += 2) put_pair<T>(p, w, row, j, 0.0f, 0.0f);
         }

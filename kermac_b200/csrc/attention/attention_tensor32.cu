@@ -245,7 +245,7 @@ attention_tensor32_kernel(const __grid_constant__ AttentionParams p, const __gri
             sum = s_half[t][0][r] + s_half[t][1][r];
             const bool  good = *reinterpret_cast<volatile int*>(&s_expired) == 0 && at < w.rows;
             const float by   = sum == 0.0f ? 0.0f : 1.0f / sum;
-            if (good && half == 0) put_lse(p, w, row, (top == -INFINITY ? top : top * c) + lg2_approx(sum));
+            if (good && half == 0) put_stats(p, w, row, top == -INFINITY ? top : top * c, sum);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] *= by;
             float* const out  = reinterpret_cast<float*>(p.out.ptr) + row.l * p.out.sl + row.n * p.out.sr + row.h * p.out.sh + half * 32;

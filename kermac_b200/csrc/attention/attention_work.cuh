@@ -110,12 +110,17 @@ __device__ __forceinline__ void put_pair(const AttentionParams& p, const Work& w
         }
     }
 }
-// lse2: log2 of the sum of exp2; -inf for a row without keys.
-__device__ __forceinline__ void put_lse(const AttentionParams& p, const Work& w, const Row& row, float lse2) {
-    if (p.parts != 1)
-        p.part_lse[((static_cast<long long>(w.part) * p.L + row.l) * p.N + row.n) * p.H + row.h] = lse2;
-    else if (p.lse)
-        p.lse[row.l * p.lse_sl + row.h * p.lse_sh + row.n] = lse2 * LN2;
+// A row's maximum (log2 domain) and its sum of exp2 of what lies below: into its part, or as the logarithm of the whole.  A row without keys
+// has the sum 0.  Parts keep the two apart: as one logarithm of some 11, rounded, they would weigh with errors of 3e-7 each, which
+// made a float32 token against 3000 keys in 11 pieces 2.6 times as inaccurate as fp32 products.
+__device__ __forceinline__ void put_stats(const AttentionParams& p, const Work& w, const Row& row, float top, float sum) {
+    if (sum == 0.0f) top = -INFINITY;
+    if (p.parts != 1) {
+        const long long rows = static_cast<long long>(p.L) * p.N * p.H, at = w.part * rows + (static_cast<long long>(row.l) * p.N + row.n) * p.H + row.h;
+        p.part_top[at] = top, p.part_top[p.parts * rows + at] = sum;
+    } else if (p.lse) {
+        p.lse[row.l * p.lse_sl + row.h * p.lse_sh + row.n] = (top + lg2_approx(sum)) * LN2;
+    }
 }
 
 }  // namespace att

@@ -290,7 +290,7 @@ def test_grad_widths_and_layouts(dtype, D, layout):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("N, M", [(20, 140), (150, 300)])
+@pytest.mark.parametrize("N, M", [(20, 140), (150, 300), (140, 100)])      # the last: all keys in one tile
 @pytest.mark.parametrize("D", [64, 128])
 def test_grad_of_broadcast_inputs(dtype, N, M, D):
     L, H, Hk = 3, 4, 2
@@ -310,6 +310,33 @@ def test_float16_gradients_keep_their_range(N, M, by):
     # weights of 1/2000 times gradients of 1e-4 lie below the smallest float16
     q, k, v = (make(s, 1, n, 2, 64, dtype=torch.float16) for s, n in ((1, N), (2, M), (3, M)))
     check_grad(torch.float16, q, k, v, None, 1, g_by=by, scale=0.02)
+
+
+@pytest.mark.parametrize("N, M, D", [(1, 3000, 64), (300, 2000, 64), (300, 700, 128), (300, 30, 64)])
+def test_float32_is_no_less_accurate_than_fp32_products(N, M, D):
+    # the bounds above are for the worst case; the errors of products in torch's fp32 are what a caller would get otherwise.
+    # Root mean squares over some 10^5 values: a quarter more than theirs is far outside what chance does to them.
+    q, k, v, g = (make(s, 1, n, 2, D, dtype=torch.float32, by=by) for s, n, by in ((1, N, 1.5), (2, M, 1.0), (3, M, 1.0), (9, N, 0.5)))
+    assert not torch.backends.cuda.matmul.allow_tf32
+
+    def formulas(q, k, v, g):
+        q, k, v, g = (t[0].transpose(0, 1) for t in (q, k, v, g))
+        s = torch.matmul(q, k.transpose(1, 2)) / math.sqrt(D)
+        e = torch.exp(s - s.amax(dim=-1, keepdim=True))
+        p = e / e.sum(dim=-1, keepdim=True)
+        out = torch.matmul(p, v)
+        ds = p * (torch.matmul(g, v.transpose(1, 2)) - (g * out).sum(dim=-1, keepdim=True)) / math.sqrt(D)
+        return [t.transpose(0, 1)[None] for t in (out, torch.matmul(ds, k), torch.matmul(ds.transpose(1, 2), q), torch.matmul(p.transpose(1, 2), g))]
+
+    exact, plain = formulas(*(t.double() for t in (q, k, v, g))), formulas(q, k, v, g)
+    out, lse = kermac.cross_attention(q, k, v, return_lse=True)
+    # The gradient takes its weights from the lse that the caller holds as float32.  That number is off by half a step, 2^-24 of its size,
+    # and so is its product with log2(e); lg2.approx adds 2^-22.  An error of lse is a factor on all of a row's weights, which one
+    # query does not average away (the formulas above normalise by the sum itself).
+    of_lse = 2 * 2.0 ** -24 * float(lse.abs().max()) + 2.0 ** -22
+    for i, (got, fp32, want) in enumerate(zip((out, *kermac.cross_attention_grad(q, k, v, out, lse, g)), plain, exact)):
+        ours, theirs = ((t.double() - want).square().mean().sqrt() for t in (got, fp32))
+        assert ours <= 1.25 * theirs + (2.0 ** -26 if i == 0 else of_lse) * want.square().mean().sqrt(), i
 
 
 def test_gradient_against_differences():
