@@ -185,10 +185,12 @@ def cross_attention(
     behind is never used, whatever it holds.  A query without a state to look at gets zeros and lse = -inf.
 
     `out`: (L, N, H, D), allocated when None.  `lse`: (L, H, N) float32 for the logarithm of each query's sum of exponentials, which
-    `cross_attention_grad` needs; with `return_lse` the call returns (out, lse).  `scale` is 1 / sqrt(D) when None.
+    `cross_attention_grad` needs; with `return_lse` the call returns (out, lse).  Neither may share memory with an input.  `scale` is
+    1 / sqrt(D) when None.
 
-    Scores, softmax and sums are 32-bit; with 16-bit types the weights are rounded to that type for the product with v.  Equal
-    calls give equal bits.  Partial sums, where few queries look at many states (at most 512 MB), and copies of float32 inputs
+    Scores, softmax and sums are 32-bit; with 16-bit types the weights are rounded to that type for the product with v.  float32 inputs
+    are taken apart into three bfloat16 or two tf32 parts: those that are used have to be finite and below 2^127.  Equal calls give
+    equal bits.  Partial sums, where few queries look at many states (at most 512 MB), and copies of float32 inputs
     of up to 64 channels (1.5 times their size, at most 1 GiB) are taken from torch's allocator for the duration of the call.
     Launches on torch's current stream and returns without synchronising; like every allocation by torch that has to be
     captured through torch.cuda.graph.
@@ -240,7 +242,8 @@ def cross_attention_grad(
     `out` (L, N, H, D) and `lse` (L, H, N) are what cross_attention(..., return_lse=True) returned for the same q, k, v, lengths and
     scale; grad_out has the shape of out.  Each gradient has its input's shape with a batch dimension: an input that was broadcast
     over the batch (extent 1) gets the sum over the batch, key heads that several query heads share the sum over these, and
-    states behind `lengths` get zeros.  grad_q, grad_k, grad_v: destinations of those shapes, allocated when None.
+    states behind `lengths` get zeros.  grad_q, grad_k, grad_v: destinations of those shapes, which share memory with nothing else that
+    the call is given, allocated when None.
 
     Sums are 32-bit and in a fixed order: equal calls give equal bits.  Takes scratch from torch's allocator for the duration
     of the call: 4 bytes a query and head, and partial sums where an input is broadcast or few states meet many queries.

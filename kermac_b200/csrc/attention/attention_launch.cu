@@ -366,7 +366,8 @@ GradPlan plan_grad(const KmAttentionArgs& a) {
 int gradient(const KmAttentionArgs* a, void* stream) {
     int rc = check(a, GRAD);
     if (rc) return rc;
-    if (empty(*a) && (a->m == 0 || a->kv_batch == 0)) return 0;
+    const bool no_queries = a->q_batch == 0 || a->n == 0 || a->heads == 0, no_keys = a->kv_batch == 0 || a->m == 0;
+    if (no_queries && no_keys) return 0;                   // no gradient has a row
     rc = require_sm100();
     if (rc) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -109,7 +109,8 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
             const float c = p.scale_log2;
             const int   limit = min(row_limit(p, w, at < w.rows ? at : w.rows - 1), w.end);
             const int   all_see = w.causal ? w.length - p.N + 1 : w.length;     // keys in front of it are seen by every row
-            float top = 0.0f, sum = 0.0f;
+            // slack: how far a row's maximum may grow; -inf where nothing but scores of -inf has come, whose maximum of 0 any other replaces
+            float top = 0.0f, sum = 0.0f, slack = 8.0f;
             for (int i = 0; i < n_tiles; ++i) {
                 const int first = w.first + i * TC_ROWS;
                 wait(s_full(t), i & 1);
@@ -132,13 +133,13 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
                         best[e] = fmaxf(fmaxf(best[e], __uint_as_float(x[j + e])), __uint_as_float(x[j + 4 + e]));
                 const float high = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
                 if (i == 0) {
-                    top = high == -INFINITY ? 0.0f : high;      // a row that sees nothing: exp2(-inf - 0) = 0
+                    if (high == -INFINITY) slack = -INFINITY; else top = high;      // a row that sees nothing: exp2(-inf - 0) = 0
                 } else {
-                    const bool grown = (high - top) * c > 8.0f;
+                    const bool grown = (high - top) * c > slack;
                     if (__any_sync(0xffffffffu, grown)) {
                         // the products into O that were issued before this S are complete
-                        const float shrink = grown ? ex2_approx((top - high) * c) : 1.0f;
-                        if (grown) top = high;
+                        const float shrink = grown && slack > 0.0f ? ex2_approx((top - high) * c) : 1.0f;
+                        if (grown) top = high, slack = 8.0f;
                         sum *= shrink;
 #pragma unroll
                         for (int j = 0; j < DP; j += 32) {

@@ -537,3 +537,36 @@ def test_same_bits_as_the_ctypes_marshalling(dtype, N, capsys):
     for bad in (dict(k=k.cpu()), dict(scale=-1.0), dict(lengths=lengths.long())):
         with pytest.raises((TypeError, ValueError)):
             kermac.cross_attention(**dict(dict(q=q, k=k, v=v), **bad))
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=str)
+@pytest.mark.parametrize("N", [1, 20, 300])
+@pytest.mark.parametrize("D", [64, 128])
+def test_scores_of_minus_infinity_in_front(dtype, N, D):
+    # the first 150 keys have no weight, whatever the level of the others' scores: here at some -40 * 64 / 8, where exp underflows
+    q = (torch.rand(1, N, 2, D, generator=torch.Generator().manual_seed(1)) + 0.5).cuda().to(dtype)
+    k, v = make(2, 1, 400, 2, D, dtype=dtype), make(3, 1, 400, 2, D, dtype=dtype)
+    k -= 5.0
+    k[:, :150, :, 0] = -math.inf
+    out, lse = kermac.cross_attention(q, k, v, scale=1.0, return_lse=True)
+    want, want_lse, bound, lse_bound = ao.attention(q, k[:, 150:], v[:, 150:], scale=1.0)
+    assert_within(out, want, bound, "out")
+    assert_within(lse, want_lse, lse_bound, "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_gradient_of_broadcast_inputs_over_an_empty_batch(dtype):
+    # a sum over no batch entry is zero, and is written
+    def t(*shape):
+        return torch.full(shape, 7.0, dtype=dtype, device="cuda")
+    lse = torch.zeros(0, 2, 3, device="cuda")
+    none = t(0, 3, 2, 8)
+    grad_q = t(1, 3, 2, 8)
+    kermac.cross_attention_grad(t(1, 3, 2, 8), t(0, 4, 2, 8), t(0, 4, 2, 8), none, lse, none, grad_q=grad_q)
+    assert torch.all(grad_q == 0)
+    lengths = torch.zeros(0, dtype=torch.int32, device="cuda")
+    for M in (0, 4):
+        grads = t(1, 3, 2, 8), t(1, M, 2, 8), t(1, M, 2, 8)
+        kermac.cross_attention_grad(t(3, 2, 8), t(M, 2, 8), t(M, 2, 8), none, lse, none, lengths=lengths, grad_q=grads[0], grad_k=grads[1],
+                                    grad_v=grads[2])
+        assert all(torch.all(g == 0) for g in grads)
