@@ -2,8 +2,12 @@
 //
 // With p = exp(s - lse) recomputed from the forward pass's lse and delta = sum_d dout * out,
 //   dv = p^T dout,   ds = p * (dout v^T - delta),   dk = scale ds^T q,   dq = scale ds k.
-// Two kernels, so that every sum has one owner and a fixed order: one holds 64 keys and streams the queries (dk, dv), one holds 64
-// queries and streams the keys (dq).  The price is that s and dout v^T are computed twice, 7 products instead of 5.
+// Two kinds of blocks, so that every sum has one owner and a fixed order: one holds 64 keys and streams the queries (dk, dv), one holds
+// 64 queries and streams the keys (dq).  The price is that s and dout v^T are computed twice, 7 products instead of 5.
+//
+// One launch has both, so that few rows of either fill the SMs together: a block is four warps, one for each scheduler of an SM, and one
+// warp alone issues in 0.38 of the cycles.  float32 gradients, two launches and one: 2 x 300 x 500, 4 heads of 64, 80 and 63 us;
+// 2 x 77 x 300, 8 heads of 64, 55 and 35; 300 x 300, 4 heads of 250, 307 and 184.
 #include "attention_grad.cuh"
 
 namespace km {
@@ -21,8 +25,9 @@ struct GradShape {
     static constexpr int SMEM   = 2 * HELD + 2 * 2 * MOVED + STATS;
 };
 
+// `block`: (key tile, slice, key head, batch entry of k and v, channel part)
 template <typename T, int DP>
-__global__ void __launch_bounds__(THREADS) attention_grad_keys_kernel(const AttentionGradParams p) {
+__device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, int block) {
     typedef GradShape<T, DP> S;
     typedef Tile<T, DP>      TL;
     constexpr int NT = S::STREAM / 8, CT = S::CT;
@@ -32,15 +37,12 @@ __global__ void __launch_bounds__(THREADS) attention_grad_keys_kernel(const Atte
     char* const  ring   = smem + 2 * S::HELD;
     float* const stats  = reinterpret_cast<float*>(ring + 4 * S::MOVED);
     const int    warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    after_previous_grid();
 
-    // (key tile, slice, key head, batch entry of k and v); channel part in y
     const int tiles = (p.M + S::ROWS - 1) / S::ROWS;
-    int       block = blockIdx.x;
-    const int tile = block % tiles;   block /= tiles;
-    const int slice = block % p.kv_slices; block /= p.kv_slices;
-    const int hk = block % p.Hk, kl = block / p.Hk;
-    const int c0 = blockIdx.y * CT * 8, key0 = tile * S::ROWS;
+    const int key0 = block % tiles * S::ROWS; block /= tiles;
+    const int slice = block % p.kv_slices;    block /= p.kv_slices;
+    const int hk = block % p.Hk;              block /= p.Hk;
+    const int kl = block % p.kv_batch, c0 = block / p.kv_batch * CT * 8;
 
     // the sum runs over (batch entries of a broadcast k, heads of the group, query tiles): this block's piece of it
     const int l_count = p.kv_batch == 1 ? p.L : 1, l_first = p.kv_batch == 1 ? 0 : kl;
@@ -132,7 +134,7 @@ __global__ void __launch_bounds__(THREADS) attention_grad_keys_kernel(const Atte
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(THREADS) attention_grad_queries_kernel(const AttentionGradParams p) {
+__device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p, int block) {
     typedef GradShape<T, DP> S;
     typedef Tile<T, DP>      TL;
     constexpr int NT = S::STREAM / 8, CT = DP / 8;
@@ -141,10 +143,8 @@ __global__ void __launch_bounds__(THREADS) attention_grad_queries_kernel(const A
     T* const    held_d = reinterpret_cast<T*>(smem + S::HELD);
     char* const ring   = smem + 2 * S::HELD;
     const int   warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    after_previous_grid();
 
     const int tiles = (p.N + S::ROWS - 1) / S::ROWS;
-    int       block = blockIdx.x;
     const int n0 = block % tiles * S::ROWS; block /= tiles;
     const int split = block % p.q_splits;   block /= p.q_splits;
     const int h = block % p.H, l = block / p.H, hk = h / p.G;
@@ -213,6 +213,18 @@ __global__ void __launch_bounds__(THREADS) attention_grad_queries_kernel(const A
         for (int c = 0; c < CT; ++c)
             put_grad<T>(p.dq, part, one_q ? 0 : l, n, h, p.N, p.H, p.D, c * 8 + 2 * t, dq[c][2 * r] * by, dq[c][2 * r + 1] * by);
     }
+}
+
+// float32 with up to 64 channels: three blocks an SM (1000 x 1500, 8 heads: 415 -> 380 us); 16-bit types are
+// slower with a limit (140 us against 136 at 2 x 500 x 700, 8 heads of 100).
+template <typename T, int DP>
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 0 : DP == 64 ? 3 : 1) attention_grad_rows_kernel(const AttentionGradParams p, const int key_blocks) {
+    after_previous_grid();
+    const int block = static_cast<int>(blockIdx.x);
+    if (block < key_blocks)                  // four products a tile first, then three
+        gradient_of_keys<T, DP>(p, block);
+    else
+        gradient_of_queries<T, DP>(p, block - key_blocks);
 }
 
 // delta[l][h][n], and for float16 the largest |dout| of ATT_PEAK_ROWS queries.  One block for ATT_PEAK_ROWS queries of a head.
@@ -293,19 +305,13 @@ template <typename T, int DP>
 int launch_grad(const AttentionGradParams& p, cudaStream_t st) {
     typedef GradShape<T, DP> S;
     static_assert(S::SMEM <= 227 * 1024, "more shared memory than a block has");
-    auto* const keys    = &attention_grad_keys_kernel<T, DP>;
-    auto* const queries = &attention_grad_queries_kernel<T, DP>;
-    int rc = cuda_status(cudaFuncSetAttribute(keys, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "cudaFuncSetAttribute");
-    if (!rc) rc = cuda_status(cudaFuncSetAttribute(queries, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "cudaFuncSetAttribute");
-    const long long kb = ceil_div_ll(p.M, S::ROWS) * p.kv_slices * p.Hk * p.kv_batch;
-    const long long qb = ceil_div_ll(p.N, S::ROWS) * p.q_splits * p.H * p.L;
-    if (!rc) rc = check_blocks(kb > qb ? kb : qb);
-    if (!rc && kb)
-        rc = cuda_status(launch_overlapped(keys, dim3(static_cast<unsigned>(kb), DP / (S::CT * 8)), THREADS, S::SMEM, st, p),
-                         "attention_grad_keys_kernel");
-    if (!rc && qb)
-        rc = cuda_status(launch_overlapped(queries, dim3(static_cast<unsigned>(qb)), THREADS, S::SMEM, st, p), "attention_grad_queries_kernel");
-    return rc;
+    auto* const kernel = &attention_grad_rows_kernel<T, DP>;
+    if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "cudaFuncSetAttribute")) return rc;
+    const long long keys    = ceil_div_ll(p.M, S::ROWS) * p.kv_slices * p.Hk * p.kv_batch * (DP / (S::CT * 8));
+    const long long queries = ceil_div_ll(p.N, S::ROWS) * p.q_splits * p.H * p.L;
+    if (int rc = check_blocks(keys + queries)) return rc;
+    return cuda_status(launch_overlapped(kernel, dim3(static_cast<unsigned>(keys + queries)), THREADS, S::SMEM, st, p, static_cast<int>(keys)),
+                       "attention_grad_rows_kernel");
 }
 template <typename T>
 int launch_type(const AttentionGradParams& p, cudaStream_t st) {

@@ -346,9 +346,9 @@ GradPlan plan_grad(const KmAttentionArgs& a) {
         p.q_splits  = p.own_delta ? 1 : split(query_blocks, key_blocks * p.kv_slices, key_tiles, of_queries);
         p.keys_first = of_keys / p.kv_slices >= of_queries / p.q_splits;
     } else {
-        // pieces of both sums where their tiles alone do not fill the SMs
-        p.kv_slices = pieces(ceil_div_ll(a.m, ATT_GRAD_ROWS) * a.key_heads * a.kv_batch, key_sums * a.n, 2, 128);
-        p.q_splits  = pieces(ceil_div_ll(a.n, ATT_GRAD_ROWS) * a.heads * a.l, a.m, 2, 128);
+        // pieces of both sums where their tiles alone do not fill the SMs (of 64 against 128: 2 x 2000 x 40, 4 heads, 56 -> 50 us)
+        p.kv_slices = pieces(ceil_div_ll(a.m, ATT_GRAD_ROWS) * a.key_heads * a.kv_batch, key_sums * a.n, 2, 64);
+        p.q_splits  = pieces(ceil_div_ll(a.n, ATT_GRAD_ROWS) * a.heads * a.l, a.m, 2, 64);
     }
     if (static_cast<long long>(p.q_splits) * a.l * a.n * a.heads * a.d > (MOST_SCRATCH >> 3)) p.q_splits = 1;
     if (static_cast<long long>(p.kv_slices) * a.kv_batch * a.m * a.key_heads * a.d > (MOST_SCRATCH >> 3)) p.kv_slices = 1;
