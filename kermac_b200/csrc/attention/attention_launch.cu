@@ -379,7 +379,7 @@ int gradient(const KmAttentionArgs* a, void* stream) {
         none.add(nullptr, 0, p.dq, a->q_batch, p.N, p.H, p.D);
         none.add(nullptr, 0, p.dk, p.kv_batch, p.M, p.Hk, p.D);
         none.add(nullptr, 0, p.dv, p.kv_batch, p.M, p.Hk, p.D);
-        return attention_reduce_launch(none, a->type, st);
+        return attention_reduce_launch(none, a->type, p.vec_grad, st);
     }
     if (!a->scratch || a->scratch_bytes < plan.bytes() || !aligned16(a->scratch))
         return fail(KM_ERR_NULL_POINTER, "attention gradient: %lld bytes of 16-byte aligned scratch are needed", plan.bytes());
@@ -396,7 +396,7 @@ int gradient(const KmAttentionArgs* a, void* stream) {
         sums.add(p.dk_part, p.kv_slices, p.dk, p.kv_batch, p.M, p.Hk, p.D);
         sums.add(p.dv_part, p.kv_slices, p.dv, p.kv_batch, p.M, p.Hk, p.D);
     }
-    return rc ? rc : attention_reduce_launch(sums, a->type, st);
+    return rc ? rc : attention_reduce_launch(sums, a->type, p.vec_grad, st);
 }
 
 }  // namespace

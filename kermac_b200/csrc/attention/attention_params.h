@@ -106,7 +106,8 @@ struct SliceSums {
         ++count;
     }
 };
-int attention_reduce_launch(const SliceSums& sums, int type, cudaStream_t st);
+// vec: rows of every dst can be written 16 bytes at a time.
+int attention_reduce_launch(const SliceSums& sums, int type, bool vec, cudaStream_t st);
 
 inline int padded_channels(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 inline int type_bytes(int type) { return type == ATT_F32 ? 4 : 2; }
