@@ -178,7 +178,9 @@ Form choose_form(long long rows, bool tma_ok, int type, int d, int keys, int all
     if (tma_ok && rows > 16) return {TENSOR, ATT_TENSOR_ROWS, 1, 256};
     if (tma_ok) return {FEW, rows <= 8 ? 8 : 16, d <= 64 || attention_few_tile(d, keys, 0) == 16 ? 2 : 1, 128};
     if (rows <= ATT_FEW_ROWS) return {SCALAR_FEW, ATT_FEW_ROWS, 1, 256};
-    if (planes && all_keys > 64) return {TENSOR32, ATT_TENSOR_ROWS, 1, 256};      // measured in attention_tensor32.cu
+    // Above 64 keys: see attention_tensor32.cu.  Pieces of 192 keys: a tile of 128 is 5 us, the join 4 to 6 (2 x 300 x 500, 4 heads: one piece
+    // 27.5 us, two 21.2; but 2 x 2000 x 260, which 128 would split, 23.7 and 28.5).
+    if (planes && all_keys > 64) return {TENSOR32, ATT_TENSOR_ROWS, 1, 192};
     return {ROWS, ATT_TILE_ROWS, type == ATT_F32 ? 4 : 2, 256};
 }
 

@@ -143,7 +143,8 @@ def test_scratch_is_bounded():
     args.m = 1 << 10
     args.n = 1 << 10
     planes = 3 * (1 << 10) * 64 * 6
-    assert planes <= _native.attention_scratch_bytes(args, 0) <= planes + 4 * (1 << 10) * 66 * 4 + 32
+    pieces = args.m // 192                                                        # no piece is shorter than that: maximum, sum and 64 channels each
+    assert planes <= _native.attention_scratch_bytes(args, 0) <= planes + pieces * (1 << 10) * 66 * 4 + 32
 
 
 def test_the_c_abi_refuses_no_arguments_at_all():
