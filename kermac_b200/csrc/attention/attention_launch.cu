@@ -177,11 +177,14 @@ struct Plan {
 Form choose_form(long long rows, bool tma_ok, int type, int d, int keys, int all_keys, bool planes) {
     if (tma_ok && rows > 16) return {TENSOR, ATT_TENSOR_ROWS, 1, 256};
     if (tma_ok) return {FEW, rows <= 8 ? 8 : 16, d <= 64 || attention_few_tile(d, keys, 0) == 16 ? 2 : 1, 128};
-    if (rows <= ATT_FEW_ROWS) return {SCALAR_FEW, ATT_FEW_ROWS, 1, 256};
+    // These two take long for a key, and their pieces are short: 64 keys against 256, a token of 500 (8 heads of 128) in float32 42.0 -> 17.5 us;
+    // 32 against 256, 2 x 300 x 500 (4 heads of 128) 120 -> 42, and against 64, 300 x 300 (4 heads of 256) 54 -> 42.  As many blocks as the shared
+    // memory of an SM holds; with twice as many 2 x 2000 x 200 (4 heads of 128) 71.8 -> 100.8.
+    if (rows <= ATT_FEW_ROWS) return {SCALAR_FEW, ATT_FEW_ROWS, d <= 64 ? 2 : 1, 64};
     // Above 64 keys: see attention_tensor32.cu.  Pieces of 192 keys: a tile of 128 is 5 us, the join 4 to 6 (2 x 300 x 500, 4 heads: one piece
     // 27.5 us, two 21.2; but 2 x 2000 x 260, which 128 would split, 23.7 and 28.5).
     if (planes && all_keys > 64) return {TENSOR32, ATT_TENSOR_ROWS, 1, 192};
-    return {ROWS, ATT_TILE_ROWS, type == ATT_F32 ? 4 : 2, 256};
+    return {ROWS, ATT_TILE_ROWS, type != ATT_F32 ? 2 : d <= 64 ? 4 : d <= 128 ? 2 : 1, 32};
 }
 
 // How many pieces the keys of `blocks` blocks are split into: as many as the SMs hold at once, no piece shorter than `least` keys.
