@@ -181,10 +181,12 @@ Form choose_form(long long rows, bool tma_ok, int type, int d, int keys, int all
     // 32 against 256, 2 x 300 x 500 (4 heads of 128) 120 -> 42, and against 64, 300 x 300 (4 heads of 256) 54 -> 42.  As many blocks as the shared
     // memory of an SM holds; with twice as many 2 x 2000 x 200 (4 heads of 128) 71.8 -> 100.8.
     if (rows <= ATT_FEW_ROWS) return {SCALAR_FEW, ATT_FEW_ROWS, d <= 64 ? 2 : 1, 64};
-    // Above 64 keys: see attention_tensor32.cu.  Pieces of 192 keys: a tile of 128 is 5 us, the join 4 to 6 (2 x 300 x 500, 4 heads: one piece
+    // Above 32 keys: see attention_tensor32.cu.  Pieces of 192 keys: a tile of 128 is 5 us, the join 4 to 6 (2 x 300 x 500, 4 heads: one piece
     // 27.5 us, two 21.2; but 2 x 2000 x 260, which 128 would split, 23.7 and 28.5).
-    if (planes && all_keys > 64) return {TENSOR32, ATT_TENSOR_ROWS, 1, 192};
-    return {ROWS, ATT_TILE_ROWS, type != ATT_F32 ? 2 : d <= 64 ? 4 : d <= 128 ? 2 : 1, 32};
+    if (planes && all_keys > 32) return {TENSOR32, ATT_TENSOR_ROWS, 1, 192};
+    // (float32 of up to 64 channels, which has more than 32 keys here where planes cannot be had: 64; 1024 queries of 64 keys, 8 heads, 12.8, with 32 16.6)
+    if (type == ATT_F32 && d <= 64) return {ROWS, ATT_TILE_ROWS, 4, 64};
+    return {ROWS, ATT_TILE_ROWS, type != ATT_F32 || d <= 128 ? 2 : 1, 32};
 }
 
 // How many pieces the keys of `blocks` blocks are split into: as many as the SMs hold at once, no piece shorter than `least` keys.

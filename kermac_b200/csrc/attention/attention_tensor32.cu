@@ -8,9 +8,9 @@
 // bits that matter.  For the same reason a tile's O_i starts from zero, and the sum over the tiles is kept in registers, rounded.
 //
 // Two threads share a row, 64 keys and 32 channels each.  2 x 1000 x 1500 (8 heads of 64, ragged): the form on mma.sync
-// (attention_rows.cu), whose warps split every value they read, takes 220 us a pass, this 52 (7 of them for the planes).  A call has
-// to have more than 64 keys: 1024 queries (8 heads) with 64 take 13.1 us this way and 12.8 the other, with 14 keys 11.4 and 8.2, but 17 with
-// 128 10.3 and 17.7.
+// (attention_rows.cu), whose warps split every value they read, takes 220 us a pass, this 53 (7 of them for the planes).  A call has
+// to have more than 32 keys: 4 x 2000 queries (8 heads) with 33 take 28.1 us this way and 48.3 the other, 1024 queries 12.9 and 12.7, 17 of
+// 4 heads 10.6 and 11.5; with 14 keys 28.0 and 32.1, 12.9 and 9.7, 10.5 and 8.4.
 #include <algorithm>
 
 #include "../km_build_tma.cuh"
