@@ -11,23 +11,52 @@ constexpr float F16_WEIGHT = 256.0f, F16_WEIGHT_LOG2 = 8.0f;
 
 template <typename T> constexpr bool is_f16 = std::is_same<T, __half>::value;
 
-// 2^-e with 2^e the power of two at or below the largest of the peaks of entries [l0, l1) and heads [h0, h1); 1 when they are zero,
-// infinite or NaN, and for the types that have the range.  Called by whole warps, each for itself.
+// What a weight's gradient ds = p (dout v^T - delta) is multiplied by before it is rounded to float16; the sums are divided by it.
+// |dout v^T| and |delta| are at most x = D max|dout| max|v|, over the keys that are seen: with 2^13 over the power of two at or below x the product
+// stays below 2^15, half of what float16 has, and a ds of 2^-27 x still has all its bits (dout v^T of random signs is some 2^-7 x at 128
+// channels, which leaves 2^-20 for p).  From |dout| alone, which this was once, keys of +-1200 in 128 channels became infinite, and v of size 0.01
+// before 5000 keys gave four times the error of rounding.
+// 1 where x is zero, and for the types that have the range.
 template <typename T>
-__device__ __forceinline__ float find_factor(const AttentionGradParams& p, int l0, int l1, int h0, int h1) {
-    if constexpr (!is_f16<T>) {
-        return 1.0f;
-    } else {
-        float     best  = 0.0f;
-        const int per_l = (h1 - h0) * p.peak_count;
-        for (int l = l0; l < l1; ++l)
-            for (int i = threadIdx.x & 31; i < per_l; i += 32)
-                best = fmaxf(best, p.peaks[(static_cast<long long>(l) * p.H + h0) * p.peak_count + i]);
+__device__ __forceinline__ float factor_for(float x) {
+    if constexpr (!is_f16<T>) return 1.0f;
+    const uint32_t e = __float_as_uint(x) >> 23;                         // x is zero or 2^-48 .. 2^40
+    return x > 0.0f ? __uint_as_float((267u - e) << 23) : 1.0f;
+}
+__device__ __forceinline__ float warp_max(float best) {
 #pragma unroll
-        for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
-        const uint32_t e = __float_as_uint(best) >> 23;                  // best is a float16 magnitude: 2^-24 .. 65504
-        return (best > 0.0f && e < 255) ? __uint_as_float((254u - e) << 23) : 1.0f;
+    for (int d = 16; d; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
+    return best;
+}
+// The largest |v| among the first `count` keys of a head; 0 for the types that need none.  Called by whole warps, each for itself.
+template <typename T>
+__device__ __forceinline__ float find_v_peak(const AttentionGradParams& p, int kl, int hk, int count) {
+    if constexpr (!is_f16<T>) return 0.0f;
+    const float* from = p.v_peaks + (static_cast<long long>(kl) * p.Hk + hk) * p.v_peak_count;
+    const int    many = (count + ATT_PEAK_ROWS - 1) / ATT_PEAK_ROWS;
+    float        best = 0.0f;
+#pragma unroll 4
+    for (int i = threadIdx.x & 31; i < many; i += 32) best = fmaxf(best, from[i]);
+    return warp_max(best);
+}
+// For a row of dq, whose sum is its own.
+template <typename T>
+__device__ __forceinline__ float row_factor(const AttentionGradParams& p, int l, int h, int n, float v_peak) {
+    if constexpr (!is_f16<T>) return 1.0f;
+    return n < p.N ? factor_for<T>(p.D * p.peaks[(static_cast<long long>(l) * p.H + h) * p.peak_count + n / ATT_PEAK_ROWS] * v_peak) : 1.0f;
+}
+// One factor for a sum over the queries of entries [l0, l1) and the heads of a group, and `count` keys.
+template <typename T>
+__device__ __forceinline__ float find_factor(const AttentionGradParams& p, int l0, int l1, int hk, int kl, int count) {
+    if constexpr (!is_f16<T>) return 1.0f;
+    const int per_l = p.G * p.peak_count;        // neighbours
+    float     best  = 0.0f;
+#pragma unroll 4
+    for (int i = threadIdx.x & 31; i < (l1 - l0) * per_l; i += 32) {
+        const int l = i / per_l;
+        best = fmaxf(best, p.peaks[(static_cast<long long>(l0 + l) * p.H + hk * p.G) * p.peak_count + i - l * per_l]);
     }
+    return factor_for<T>(p.D * warp_max(best) * find_v_peak<T>(p, kl, hk, count));
 }
 
 template <typename T>

@@ -59,7 +59,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, i
             longest = n > longest ? n : longest;
         }
     const bool  idle   = key0 >= longest;
-    const float factor = find_factor<T>(p, l_first, l_first + l_count, hk * p.G, hk * p.G + p.G);
+    const float factor = idle ? 1.0f : find_factor<T>(p, l_first, l_first + l_count, hk, kl, longest);
     const float by     = is_f16<T> ? factor / F16_WEIGHT : 1.0f;
 
     float dk[CT][4], dv[CT][4];
@@ -152,7 +152,7 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
     const int h = block % p.H, l = block / p.H, hk = h / p.G;
     const int   count  = key_count(p.lengths, p.lengths_stride, l, p.M);
     const int   kl     = p.kv_batch == 1 ? 0 : l;
-    const float factor = find_factor<T>(p, l, l + 1, h, h + 1);
+    const float v_peak = find_v_peak<T>(p, kl, hk, count);
 
     copy_rows<T, DP>(held_q, head_of<T>(p.q, l, h), p.q.sr, n0, p.N, S::ROWS, p.D, p.vec, threadIdx.x, THREADS);
     copy_rows<T, DP>(held_d, head_of<T>(p.dout, l, h), p.dout.sr, n0, p.N, S::ROWS, p.D, p.vec, threadIdx.x, THREADS);
@@ -170,12 +170,13 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
         }
         copy_commit();
     };
-    float lse[2], delta[2], dq[CT][4];
+    float lse[2], delta[2], factor[2], dq[CT][4];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const int n = n0 + warp * 16 + g + 8 * r;
         lse[r]   = n < p.N ? p.lse[l * p.lse_sl + h * p.lse_sh + n] * (1.0f / LN2) : 0.0f;
         delta[r] = n < p.N ? p.delta[(static_cast<long long>(l) * p.H + h) * p.N + n] : 0.0f;
+        factor[r] = row_factor<T>(p, l, h, n, v_peak);
     }
 #pragma unroll
     for (int c = 0; c < CT; ++c) dq[c][0] = dq[c][1] = dq[c][2] = dq[c][3] = 0.0f;
@@ -197,7 +198,7 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float w = ex2_approx(fmaf(s[j][e], p.scale_log2, -lse[e >> 1]));
-                ds[j][e] = i * S::STREAM + j * 8 + 2 * t + (e & 1) < count ? w * ((ds[j][e] - delta[e >> 1]) * factor) : 0.0f;
+                ds[j][e] = i * S::STREAM + j * 8 + 2 * t + (e & 1) < count ? w * ((ds[j][e] - delta[e >> 1]) * factor[e >> 1]) : 0.0f;
             }
         product_nn<T, DP, NT, CT>(dq, ds, k);
         __syncthreads();
@@ -206,10 +207,10 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
     // partial sums [slice][entry of q][n][h][D]: a broadcast q has one entry and a slice for each l and piece
     const bool   one_q = p.q_slices > p.q_splits;
     float* const part = p.q_slices > 1 ? p.dq_part + static_cast<long long>(one_q ? l * p.q_splits + split : split * p.L) * p.N * p.H * p.D : nullptr;
-    const float  by = p.scale / factor;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        const int n = n0 + warp * 16 + g + 8 * r;
+        const int   n  = n0 + warp * 16 + g + 8 * r;
+        const float by = p.scale / factor[r];
         if (n >= p.N) continue;
 #pragma unroll
         for (int c = 0; c < CT; ++c)
@@ -229,20 +230,75 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 0 : DP == 64 ? 3 : 1
         gradient_of_queries<T, DP>(p, block - key_blocks);
 }
 
-// delta[l][h][n], and for float16 the largest |dout| of ATT_PEAK_ROWS queries.  One block for ATT_PEAK_ROWS queries of a head.
+// The largest of a block.
+__device__ __forceinline__ float block_peak(float peak, float* of_warp) {
+    peak = warp_max(peak);
+    if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = peak;
+    __syncthreads();
+    return fmaxf(fmaxf(of_warp[0], of_warp[1]), fmaxf(of_warp[2], of_warp[3]));
+}
+// What is infinite or no number, like the results that it enters, says nothing of the others.
+__device__ __forceinline__ float finite_size(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.0f; }
+// Lanes of a row, which take its 16-byte units in turn: a warp has 32 / lanes rows at a time.
+__device__ __forceinline__ int row_lanes(int units) { return units > 16 ? 32 : units > 8 ? 16 : 8; }
+
+// float16: v_peaks of ATT_PEAK_ROWS keys of a head; rows behind the longest sequence hold whatever the memory holds.
+__device__ __forceinline__ void find_v_peaks(const AttentionGradParams& p, int block, float* of_warp) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = block % p.v_peak_count; block /= p.v_peak_count;
+    const int hk = block % p.Hk, kl = block / p.Hk;
+    int       there = p.M;
+    if (p.lengths != nullptr) {
+        there = 0;
+        if (p.kv_batch == p.L) {
+            there = key_count(p.lengths, p.lengths_stride, kl, p.M);
+        } else {
+            for (int l = lane; l < p.L; l += 32) there = max(there, key_count(p.lengths, p.lengths_stride, l, p.M));
+            there = __reduce_max_sync(0xffffffffu, there);
+        }
+    }
+    const __half* v    = head_of<__half>(p.v, kl, hk);
+    float         peak = 0.0f;
+    // as in attention_delta_kernel
+    const int units = (p.D + 7) / 8, lanes = row_lanes(units), sub = lane & (lanes - 1);
+#pragma unroll 4
+    for (int r = (warp * 32 + lane) / lanes; r < ATT_PEAK_ROWS; r += THREADS / lanes) {
+        const int key = group * ATT_PEAK_ROWS + r;
+        for (int u = sub; u < units; u += lanes) {
+            alignas(16) __half x[8];
+            if (key < there && p.vec) {
+                *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(v + key * p.v.sr + u * 8);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = key < there && u * 8 + e < p.D ? v[key * p.v.sr + u * 8 + e] : Type<__half>::to(0.0f);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) peak = fmaxf(peak, finite_size(__half2float(x[e])));
+        }
+    }
+    peak = block_peak(peak, of_warp);
+    if (threadIdx.x == 0) p.v_peaks[(static_cast<long long>(kl) * p.Hk + hk) * p.v_peak_count + group] = peak;
+}
+
+// delta[l][h][n], and for float16 the peaks of dout.  One block for ATT_PEAK_ROWS queries of a head; those from `query_blocks` on
+// find the peaks of v.
 template <typename T>
-__global__ void __launch_bounds__(THREADS) attention_delta_kernel(const AttentionGradParams p) {
+__global__ void __launch_bounds__(THREADS) attention_delta_kernel(const AttentionGradParams p, const int query_blocks) {
     __shared__ float of_warp[WARPS];
     after_previous_grid();
-    int       block = blockIdx.x;
+    int block = blockIdx.x;
+    if constexpr (is_f16<T>)
+        if (block >= query_blocks) {
+            find_v_peaks(p, block - query_blocks, of_warp);
+            return;
+        }
     const int groups = (p.N + ATT_PEAK_ROWS - 1) / ATT_PEAK_ROWS, group = block % groups;
     block /= groups;
     const int h = block % p.H, l = block / p.H, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const T * out = head_of<T>(p.out, l, h), *dout = head_of<T>(p.dout, l, h);
     float     peak = 0.0f;
-    // `lanes` lanes a row, a 16-byte unit each in turn, so a warp takes 32 / lanes rows at a time
     constexpr int CHUNK = Type<T>::CHUNK;
-    const int units = (p.D + CHUNK - 1) / CHUNK, lanes = units > 16 ? 32 : units > 8 ? 16 : 8, sub = lane & (lanes - 1);
+    const int units = (p.D + CHUNK - 1) / CHUNK, lanes = row_lanes(units), sub = lane & (lanes - 1);
 #pragma unroll 4
     for (int r = (warp * 32 + lane) / lanes; r < ATT_PEAK_ROWS; r += THREADS / lanes) {     // uniform: a multiple of lanes rows
         const int n = group * ATT_PEAK_ROWS + r;
@@ -262,21 +318,16 @@ __global__ void __launch_bounds__(THREADS) attention_delta_kernel(const Attentio
             }
 #pragma unroll
             for (int e = 0; e < CHUNK; ++e) {
-                sum  = fmaf(Type<T>::from(x[e]), Type<T>::from(y[e]), sum);
-                peak = fmaxf(peak, fabsf(Type<T>::from(x[e])));
+                sum = fmaf(Type<T>::from(x[e]), Type<T>::from(y[e]), sum);
+                if constexpr (is_f16<T>) peak = fmaxf(peak, finite_size(Type<T>::from(x[e])));
             }
         }
         for (int d = lanes >> 1; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (sub == 0 && n < p.N) p.delta[(static_cast<long long>(l) * p.H + h) * p.N + n] = sum;
     }
-    if (p.peaks) {
-#pragma unroll
-        for (int d = 16; d; d >>= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, d));
-        if (lane == 0) of_warp[warp] = peak;
-        __syncthreads();
-        if (threadIdx.x == 0)
-            p.peaks[(static_cast<long long>(l) * p.H + h) * p.peak_count + group] =
-                fmaxf(fmaxf(of_warp[0], of_warp[1]), fmaxf(of_warp[2], of_warp[3]));
+    if constexpr (is_f16<T>) {
+        peak = block_peak(peak, of_warp);
+        if (threadIdx.x == 0) p.peaks[(static_cast<long long>(l) * p.H + h) * p.peak_count + group] = peak;
     }
 }
 
@@ -352,12 +403,13 @@ int attention_grad_rows_launch(const AttentionGradParams& p, int type, cudaStrea
 
 int attention_delta_launch(const AttentionGradParams& p, int type, cudaStream_t st) {
     using namespace att;
-    const long long blocks = ceil_div_ll(p.N, ATT_PEAK_ROWS) * p.H * p.L;
+    const long long queries = ceil_div_ll(p.N, ATT_PEAK_ROWS) * p.H * p.L, blocks = queries + static_cast<long long>(p.v_peak_count) * p.Hk * p.kv_batch;
     if (int rc = check_blocks(blocks)) return rc;
     const dim3 grid(static_cast<unsigned>(blocks));
-    const cudaError_t e = type == ATT_F32    ? launch_overlapped(&attention_delta_kernel<float>, grid, THREADS, 0, st, p)
-                          : type == ATT_BF16 ? launch_overlapped(&attention_delta_kernel<__nv_bfloat16>, grid, THREADS, 0, st, p)
-                                             : launch_overlapped(&attention_delta_kernel<__half>, grid, THREADS, 0, st, p);
+    const int  query_blocks = static_cast<int>(queries);
+    const cudaError_t e = type == ATT_F32    ? launch_overlapped(&attention_delta_kernel<float>, grid, THREADS, 0, st, p, query_blocks)
+                          : type == ATT_BF16 ? launch_overlapped(&attention_delta_kernel<__nv_bfloat16>, grid, THREADS, 0, st, p, query_blocks)
+                                             : launch_overlapped(&attention_delta_kernel<__half>, grid, THREADS, 0, st, p, query_blocks);
     return cuda_status(e, "attention_delta_kernel");
 }
 

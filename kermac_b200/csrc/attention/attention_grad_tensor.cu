@@ -150,7 +150,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
             longest = max(longest, key_count(p.lengths, p.lengths_stride, l, p.M));
     const int n_items = key0 < longest ? to - from : 0;
     // asked for by the warps that need it, while the copies are under way
-    auto find_this_factor = [&] { return n_items > 0 ? find_factor<T>(p, l_first, l_first + l_count, hk * p.G, hk * p.G + p.G) : 1.0f; };
+    auto find_this_factor = [&] { return n_items > 0 ? find_factor<T>(p, l_first, l_first + l_count, hk, kl, longest) : 1.0f; };
 
     tc::fence_before_sync();
     __syncthreads();
@@ -379,8 +379,8 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
 
     if (warp < S::WARPS_ON_WEIGHTS) {
         // ------------------------------------------------------------------ weights: lane = query, 64 keys of a tile
-        const float    factor = n_items > 0 ? find_factor<T>(p, l, l + 1, h, h + 1) : 1.0f;
         const int      half = warp >> 2, n = n0 + (threadIdx.x & 127);
+        const float    factor = n_items > 0 ? row_factor<T>(p, l, h, n, find_v_peak<T>(p, kl, hk, count)) : 1.0f;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16, at = lanes + half * 64;
         const float    shift = n < p.N ? -p.lse[l * p.lse_sl + h * p.lse_sh + n] * (1.0f / LN2) : -INFINITY;
         const float    delta = n < p.N && !p.own_delta ? -p.delta[(static_cast<long long>(l) * p.H + h) * p.N + n] * factor : 0.0f;

@@ -312,8 +312,8 @@ int forward(const KmAttentionArgs* a, Kind kind, void* stream) {
 struct GradPlan {
     AttentionGradParams p;
     bool tensor;
-    long long delta, peaks, dq, dkv;     // floats of scratch, each a multiple of 4
-    long long bytes() const { return 4 * (delta + peaks + dq + 2 * dkv); }
+    long long delta, peaks, v_peaks, dq, dkv;     // floats of scratch, each a multiple of 4
+    long long bytes() const { return 4 * (delta + peaks + v_peaks + dq + 2 * dkv); }
 };
 long long round4(long long n) { return (n + 3) & ~3LL; }
 
@@ -364,6 +364,8 @@ GradPlan plan_grad(const KmAttentionArgs& a) {
     if (a.type == ATT_F16) {
         p.peak_count = static_cast<int>(ceil_div_ll(a.n, ATT_PEAK_ROWS));
         plan.peaks   = round4(static_cast<long long>(a.l) * a.heads * p.peak_count);
+        p.v_peak_count = static_cast<int>(ceil_div_ll(a.m, ATT_PEAK_ROWS));
+        plan.v_peaks   = round4(static_cast<long long>(a.kv_batch) * a.key_heads * p.v_peak_count);
     }
     if (p.q_slices > 1) plan.dq = round4(static_cast<long long>(p.q_slices) * a.q_batch * a.n * a.heads * a.d);
     if (p.kv_slices > 1) plan.dkv = round4(static_cast<long long>(p.kv_slices) * a.kv_batch * a.m * a.key_heads * a.d);
@@ -392,7 +394,10 @@ int gradient(const KmAttentionArgs* a, void* stream) {
         return fail(KM_ERR_NULL_POINTER, "attention gradient: %lld bytes of 16-byte aligned scratch are needed", plan.bytes());
     float* at = static_cast<float*>(a->scratch);
     p.delta = at, at += plan.delta;
-    if (plan.peaks) p.peaks = at, at += plan.peaks;
+    if (plan.peaks) {
+        p.peaks = at, at += plan.peaks;
+        p.v_peaks = at, at += plan.v_peaks;
+    }
     if (plan.dq) p.dq_part = at, at += plan.dq;
     if (plan.dkv) p.dk_part = at, p.dv_part = at + plan.dkv;
     if (!p.own_delta || p.peaks) rc = attention_delta_launch(p, a->type, st);

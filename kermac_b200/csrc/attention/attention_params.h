@@ -41,10 +41,10 @@ struct AttentionGradParams {
     const float* lse; long long lse_sl, lse_sh;
     float scale, scale_log2;
     float* delta;                        // [l][h][n]: sum over channels of dout * out
-    // float16 only, else null: [l][h][peaks], the largest |dout| of ATT_PEAK_ROWS queries.  The weights' gradients are
-    // multiplied by the power of two that brings the largest |dout| of the sum they enter to [1, 2) before they are rounded
-    // to 16 bits, and the sums divided by it: float16 ends at 6e-8, and a weight of 1e-4 times a gradient of 1e-3 does not.
-    float* peaks; int peak_count;
+    // float16 only, else null: from these find_factor() (attention_grad.cuh) takes the power of two that keeps the weights' gradients in
+    // float16's range.
+    float* peaks; int peak_count;        // [l][h][peaks]: the largest |dout| of ATT_PEAK_ROWS queries
+    float* v_peaks; int v_peak_count;    // [entry of v][key head][peaks]: the largest |v| of ATT_PEAK_ROWS keys that a query sees
     // Destinations.  slices 1: the gradients in the inputs' type.  More: 32-bit partial sums [slice][...] that
     // grad_reduce adds up, where a broadcast input's gradient is a sum over the batch or the sum is split.
     Heads dq, dk, dv;

@@ -91,6 +91,10 @@ def attention_grad(q, k, v, grad_out, lengths=None, scale=None):
     sums = {n: [torch.zeros(s, dtype=torch.float64) for _ in range(2)]
             for n, s in (("grad_q", q.shape), ("grad_k", k.shape), ("grad_v", k.shape))}
     terms = max(M, N * L * H // Hk) / 8 * STEP
+    # float16: ds is multiplied by at least 2^13 / x, x = D max|dout| max|v| of the keys that are seen, before it is rounded, and half of the
+    # smallest step there is 2^-25
+    there = torch.stack([torch.arange(M) < (M if lengths is None else int(lengths[l])) for l in range(L)])
+    v_peak = v.abs().amax(dim=-1).masked_fill(~there[:, :, None], 0.0).amax(dim=(0, 1)) if M else torch.zeros(Hk)
     for l in range(L):
         seen = visible(N, M, 0, M if lengths is None else int(lengths[l]), False)
         for h in range(H):
@@ -109,7 +113,7 @@ def attention_grad(q, k, v, grad_out, lengths=None, scale=None):
             ds_off = ds.abs() * (weight + rounded + terms) + p * (1.0 + weight) * (dp_off + delta_off)
             p_off = p * (weight + rounded + terms)
             if f16:
-                ds_off = ds_off + 2.0 ** -25 * max(1.0, 2.0 * float(g[:, :, hk * (H // Hk):(hk + 1) * (H // Hk)].abs().max()))
+                ds_off = ds_off + 2.0 ** -38 * D * float(g[:, :, hk * (H // Hk):(hk + 1) * (H // Hk)].abs().max() * v_peak[hk])
                 p_off = p_off + 2.0 ** -33
             for name, value, off in (("grad_q", scale * ds @ kk, scale * ds_off @ kk.abs()),
                                      ("grad_k", scale * ds.T @ qq, scale * ds_off.T @ qq.abs()),

@@ -570,3 +570,70 @@ def test_gradient_of_broadcast_inputs_over_an_empty_batch(dtype):
         kermac.cross_attention_grad(t(3, 2, 8), t(M, 2, 8), t(M, 2, 8), none, lse, none, lengths=lengths, grad_q=grads[0], grad_k=grads[1],
                                     grad_v=grads[2])
         assert all(torch.all(g == 0) for g in grads)
+
+
+def grad_rms(dtype, q, k, v, g, grads, lengths=None):
+    """Root mean squares of the gradients' errors over what rounding alone may cost them, one number each.
+
+    Roundings are independent of one another, so their squares add: at most u |ds| (and u p) of each weight for its product, u of the
+    result, and on delta that of the output it is taken from, which shifts a whole row of ds by p.  u is the largest error of a rounding;
+    its root mean square is 0.41 of that over the mantissas, which is the room that this leaves.
+    """
+    L, N, H, D = g.shape
+    M, Hk = k.shape[1:3]
+    u, tiny = torch.finfo(dtype).eps / 2, 2.0 ** -25 if dtype == torch.float16 else 0.0
+    q, k, v, g = (t.expand(L, *t.shape[1:]).double().transpose(1, 2) for t in (q, k, v, g))
+    k, v = (t.repeat_interleave(H // Hk, dim=1) for t in (k, v))
+    s = torch.matmul(q, k.transpose(2, 3)) / math.sqrt(D)
+    if lengths is not None:
+        hidden = torch.arange(M, device="cuda")[None, :] >= torch.tensor(lengths, device="cuda")[:, None]
+        s = s.masked_fill(hidden[:, None, None, :], -math.inf)
+        k, v = (t.masked_fill(hidden[:, None, :, None], 0.0) for t in (k, v))
+    p = torch.softmax(s, dim=-1).nan_to_num(0.0)
+    out = torch.matmul(p, v)
+    ds = p * (torch.matmul(g, v.transpose(2, 3)) - (g * out).sum(dim=-1, keepdim=True))
+    of_delta = (g ** 2 * (u * out.abs() + tiny) ** 2).sum(dim=-1, keepdim=True)
+    rows = torch.matmul(p, k) ** 2 * of_delta                       # what a row's error of delta does to grad_q
+    keys = torch.matmul((p ** 2 * of_delta).transpose(2, 3), q ** 2)
+    found = []
+    for name, got, want, off in (("q", grads[0], torch.matmul(ds, k) / math.sqrt(D), (u ** 2 * torch.matmul(ds ** 2, k ** 2) + rows) / D),
+                                 ("k", grads[1], torch.matmul(ds.transpose(2, 3), q) / math.sqrt(D),
+                                  (u ** 2 * torch.matmul((ds ** 2).transpose(2, 3), q ** 2) + keys) / D),
+                                 ("v", grads[2], torch.matmul(p.transpose(2, 3), g), u ** 2 * torch.matmul((p ** 2).transpose(2, 3), g ** 2))):
+        if name != "q":
+            want, off = (t.unflatten(1, (Hk, H // Hk)).sum(dim=2) for t in (want, off))
+        if got.shape[0] == 1:
+            want, off = want.sum(dim=0, keepdim=True), off.sum(dim=0, keepdim=True)
+        off = off + (u * want.abs() + tiny) ** 2
+        found.append(float((got.double().transpose(1, 2) - want).square().mean().sqrt() / off.mean().sqrt()))
+    return found
+
+
+@pytest.mark.parametrize("D", [64, 100, 128])                      # 100: on mma.sync
+@pytest.mark.parametrize("v_by, g_by", [(0.01, 1.0), (0.002, 1.0), (1000.0, 1e-3), (1.0, 1e-3), (100.0, 100.0)])
+@pytest.mark.parametrize("N, M", [(64, 5000), (300, 600), (200, 100)])
+def test_float16_gradients_whatever_the_size_of_the_values(N, M, D, v_by, g_by):
+    # the weights' gradients are of the size |dout| |v| / M: far below float16's range, or above it.  q makes up for it in grad_k where the
+    # result itself would leave the range.
+    q, k, v, g = (make(s, 2, n, h, D, dtype=torch.float16, by=by) for s, n, h, by in ((1, N, 4, 1.0), (2, M, 2, 1.0), (3, M, 2, v_by), (9, N, 4, g_by)))
+    lengths = [M, M - M // 3]
+    spoil(k, lengths), spoil(v, lengths)
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out, lse = kermac.cross_attention(q, k, v, lengths=lens, return_lse=True)
+    grads = kermac.cross_attention_grad(q, k, v, out, lse, g, lengths=lens)
+    found = grad_rms(torch.float16, q, k, v, g, grads, lengths)
+    assert all(x <= 1.0 for x in found), found
+
+
+@pytest.mark.parametrize("D", [128, 136])                          # on the tensor cores and on mma.sync
+@pytest.mark.parametrize("M", [2, 200])
+def test_float16_gradients_of_values_with_equal_signs(D, M):
+    # dout v^T adds up over the channels: 1200 * 2^-10 * 128 = 150 of ds = 75, which once was multiplied by 2^10 and became infinite
+    q, k = torch.full((1, 4, 1, D), 0.05, device="cuda").half(), torch.zeros(1, M, 1, D, dtype=torch.float16, device="cuda")
+    v = torch.full((1, M, 1, D), 1200.0, device="cuda").half()
+    v[:, M // 2:] = -1200.0
+    g = torch.full((1, 4, 1, D), 2.0 ** -10, device="cuda").half()
+    out, lse = kermac.cross_attention(q, k, v, return_lse=True)
+    want = ao.attention_grad(q, k, v, g)
+    for name, got in zip(("grad_q", "grad_k", "grad_v"), kermac.cross_attention_grad(q, k, v, out, lse, g)):
+        assert_within(got, *want[name], name)
