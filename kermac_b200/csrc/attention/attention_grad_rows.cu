@@ -16,6 +16,10 @@ namespace km {
 namespace att {
 namespace {
 
+// Whether an entry's queries take delta from its own terms, for the reason in attention_grad_tensor.cu: where a block of keys holds all of them.
+template <typename T>
+__device__ __forceinline__ constexpr bool exact_delta(int count) { return sizeof(T) == 2 && count <= ATT_GRAD_ROWS; }
+
 template <typename T, int DP>
 struct GradShape {
     static constexpr int ROWS   = ATT_GRAD_ROWS;
@@ -23,7 +27,7 @@ struct GradShape {
     static constexpr int CT     = (DP > 128 ? 128 : DP) / 8;             // channel groups of a block's dk and dv
     static constexpr int HELD   = Tile<T, DP>::bytes(ROWS);
     static constexpr int MOVED  = Tile<T, DP>::bytes(STREAM);
-    static constexpr int STATS  = 2 * 2 * STREAM * 4;                    // two stages of lse and delta
+    static constexpr int STATS  = 2 * 2 * STREAM * 4 + WARPS * STREAM * 4;      // two stages of lse and delta; the warps' parts of an exact delta
     static constexpr int SMEM   = 2 * HELD + 2 * 2 * MOVED + STATS;
 };
 
@@ -38,6 +42,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, i
     T* const     held_v = reinterpret_cast<T*>(smem + S::HELD);
     char* const  ring   = smem + 2 * S::HELD;
     float* const stats  = reinterpret_cast<float*>(ring + 4 * S::MOVED);
+    float* const parts  = stats + 4 * S::STREAM;
     const int    warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
     const int tiles = (p.M + S::ROWS - 1) / S::ROWS;
@@ -94,7 +99,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, i
             const T* const     q     = reinterpret_cast<const T*>(ring + (i & 1) * 2 * S::MOVED);
             const T* const     dout  = q + S::STREAM * TL::LD;
             const float* const lse   = stats + (i & 1) * 2 * S::STREAM;
-            const float* const delta = lse + S::STREAM;
+            float* const       delta = stats + ((i & 1) * 2 + 1) * S::STREAM;
             const int          l     = l_first + i / (q_tiles * p.G), n0 = (i % q_tiles) * S::STREAM;
             const int          count = key_count(p.lengths, p.lengths_stride, l, p.M);
             float s[NT][4], ds[NT][4];
@@ -103,6 +108,28 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, i
                 s[j][0] = s[j][1] = s[j][2] = s[j][3] = ds[j][0] = ds[j][1] = ds[j][2] = ds[j][3] = 0.0f;
             product_nt<T, DP, NT>(s, held_k + warp * 16 * TL::LD, q);
             product_nt<T, DP, NT>(ds, held_v + warp * 16 * TL::LD, dout);
+            if (exact_delta<T>(count) && key0 == 0) {          // this block has every key of the entry
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int col  = j * 8 + 2 * t + e;
+                        float     part = 0.0f;
+#pragma unroll
+                        for (int r = 0; r < 2; ++r)
+                            if (warp * 16 + g + 8 * r < count)
+                                part = fmaf(ex2_approx(fmaf(s[j][e + 2 * r], p.scale_log2, -lse[col] * (1.0f / LN2))), ds[j][e + 2 * r], part);
+#pragma unroll
+                        for (int d = 4; d <= 16; d <<= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+                        if (g == 0) parts[warp * S::STREAM + col] = part;
+                    }
+                __syncthreads();
+                if (threadIdx.x < S::STREAM) {
+                    const float* const of = parts + threadIdx.x;
+                    delta[threadIdx.x] = (of[0] + of[S::STREAM]) + (of[2 * S::STREAM] + of[3 * S::STREAM]);
+                }
+                __syncthreads();
+            }
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -181,6 +208,31 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
 #pragma unroll
     for (int c = 0; c < CT; ++c) dq[c][0] = dq[c][1] = dq[c][2] = dq[c][3] = 0.0f;
 
+    if (exact_delta<T>(count)) {
+        float sum[2] = {0.0f, 0.0f};
+        for (int i = 0; i < key_tiles; ++i) {
+            T* const k = reinterpret_cast<T*>(ring);
+            copy_rows<T, DP>(k, head_of<T>(p.k, kl, hk), p.k.sr, i * S::STREAM, count, S::STREAM, p.D, p.vec, threadIdx.x, THREADS);
+            copy_rows<T, DP>(k + S::STREAM * TL::LD, head_of<T>(p.v, kl, hk), p.v.sr, i * S::STREAM, count, S::STREAM, p.D, p.vec, threadIdx.x, THREADS);
+            copy_commit();
+            copy_wait<0>();
+            __syncthreads();
+            float s[NT][4], dp[NT][4];
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                s[j][0] = s[j][1] = s[j][2] = s[j][3] = dp[j][0] = dp[j][1] = dp[j][2] = dp[j][3] = 0.0f;
+            product_nt<T, DP, NT>(s, held_q + warp * 16 * TL::LD, k);
+            product_nt<T, DP, NT>(dp, held_d + warp * 16 * TL::LD, k + S::STREAM * TL::LD);
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i * S::STREAM + j * 8 + 2 * t + (e & 1) < count)
+                        sum[e >> 1] = fmaf(ex2_approx(fmaf(s[j][e], p.scale_log2, -lse[e >> 1])), dp[j][e], sum[e >> 1]);
+            __syncthreads();
+        }
+        delta[0] = quad_sum(sum[0]), delta[1] = quad_sum(sum[1]);
+    }
     load(i_first);
     for (int i = i_first; i < i_end; ++i) {
         load(i + 1);

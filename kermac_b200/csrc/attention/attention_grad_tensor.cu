@@ -5,9 +5,10 @@
 // (two launches: a training step of 8 x 512 x 1030 waited twice for its last blocks, 140 of 195 us).
 //
 // delta from the output as the forward pass rounded it is off by up to half a step of the output's terms, which shows where few keys
-// share a query: with 11 keys dq came out with 1.85 times the error of rounding alone, from 128 on with 1.5.  Where all keys are in one tile
-// the blocks of dq have every term of delta = sum p (dout v^T) at hand; they run first then, and there is no pass over out and dout.  Scores and dout v^T are in tensor memory, the weights and their gradients are written back over them as
-// 16-bit operands.  The keys' kernel computes both transposed, so that its operands need no transposition either: a
+// share a query: dq and dk had 1.9 times the error of rounding the weights' gradients and the results with 2 keys, 1.36 with 5, 1.2 with 11, 1.04
+// with 128.  Entries of the batch whose keys are in one tile, however far they are padded, form it from its own terms, sum_m p (dout v^T), which
+// both kinds of blocks have at hand (1.0 then); where no entry can have more there is no pass over out and dout.  Scores and dout v^T are in
+// tensor memory, the weights and their gradients are written back over them as 16-bit operands.  The keys' kernel computes both transposed, so that its operands need no transposition either: a
 // lane is a key there and a query in the other kernel.
 //
 // Tensor memory has no room for a second set of both products beside the 128-channel sums dk and dv, and needs none: what the tensor
@@ -31,7 +32,7 @@ struct GradTensorShape {
     static constexpr int WARPS_ON_WEIGHTS = 8, LOAD_WARP = 8, MMA_WARP = 9, STATS_WARP = 10, BLOCK = 384;
     static constexpr int KEYS_STAGES = 2;                                   // keys' kernel: tiles of q, and of dout, under way
     static constexpr int K_STAGES = 3, V_STAGES = 2;                        // queries' kernel: k is needed again for dq
-    static constexpr int KEYS_SMEM    = 1024 + (2 + 2 * KEYS_STAGES) * TILE + 2 * 2 * TC_ROWS * 4;
+    static constexpr int KEYS_SMEM    = 1024 + (2 + 2 * KEYS_STAGES) * TILE + (2 * 2 + 4) * TC_ROWS * 4;      // with lse and delta, and parts of an exact delta
     static constexpr int QUERIES_SMEM = 1024 + (2 + K_STAGES + V_STAGES) * TILE;
     // more than half of an SM's shared memory: a second block would wait inside tcgen05.alloc
     static constexpr int at_least_half(int n) { return n > 115 * 1024 ? n : 115 * 1024; }
@@ -158,6 +159,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
     const uint32_t tmem = s_tmem, s_col = tmem, dp_col = tmem + 128, dv_col = tmem + 256, dk_col = tmem + 256 + DP;
     const uint32_t held_k = base, held_v = base + S::TILE, ring_q = base + 2 * S::TILE, ring_d = ring_q + ST * S::TILE;
     float* const   stats = reinterpret_cast<float*>(smem_raw + (base - raw) + (2 + 2 * ST) * S::TILE);
+    float* const   parts = stats + 2 * 2 * TC_ROWS;        // [4][128]: the sums of 32 keys each
     Waits wait{&s_expired};
 
     if (warp < S::WARPS_ON_WEIGHTS) {
@@ -168,7 +170,8 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
         const u64      c2 = pack2(p.scale_log2, p.scale_log2), by2 = pack2(by, by);
         for (int i = 0; i < n_items; ++i) {
             const int  st   = i % ST;
-            const bool seen = key < key_count(p.lengths, p.lengths_stride, l_first + (from + i) / (p.G * q_tiles), p.M);
+            const int  count = key_count(p.lengths, p.lengths_stride, l_first + (from + i) / (p.G * q_tiles), p.M);
+            const bool seen = key < count;
             const ulonglong2* const lse   = reinterpret_cast<const ulonglong2*>(stats + st * 2 * TC_ROWS + half * 64);
             const ulonglong2* const delta = reinterpret_cast<const ulonglong2*>(stats + st * 2 * TC_ROWS + TC_ROWS + half * 64);
             uint32_t w[64];
@@ -200,6 +203,35 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
 
             wait(dp_full, i & 1);
             tc::fence_after_sync();
+            if (count <= TC_ROWS && key0 == 0) {
+                // every key of the entry is here: delta = sum_m p (dout v^T), over the lanes
+#pragma unroll
+                for (int j = 0; j < 64; j += 32) {
+                    uint32_t g[32];
+                    tmem_load32(dp_col + at + j, g);
+                    tmem_wait_load();
+                    tmem_loaded32(g);
+                    float x[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[e] = seen ? __uint_as_float(w[j + e]) * __uint_as_float(g[e]) : 0.0f;
+                    // each step halves the columns that a lane has and adds those of its partner; column `lane` is left
+#pragma unroll
+                    for (int d = 16; d; d >>= 1)
+#pragma unroll
+                        for (int e = 0; e < d; ++e) {
+                            const bool  upper = lane & d;
+                            const float other = __shfl_xor_sync(0xffffffffu, upper ? x[e] : x[e + d], d);
+                            x[e] = (upper ? x[e + d] : x[e]) + other;
+                        }
+                    parts[(warp & 3) * TC_ROWS + half * 64 + j + lane] = is_f16<T> ? x[0] * (1.0f / F16_WEIGHT) : x[0];
+                }
+                asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+                if (half == 0) {
+                    const int n = threadIdx.x & 127;
+                    stats[st * 2 * TC_ROWS + TC_ROWS + n] = -((parts[n] + parts[TC_ROWS + n]) + (parts[2 * TC_ROWS + n] + parts[3 * TC_ROWS + n])) * by;
+                }
+                asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+            }
 #pragma unroll
             for (int j = 0; j < 64; j += 32) {
                 uint32_t g[32];
@@ -279,7 +311,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
             for (int e = 0; e < 4; ++e) {
                 const int n = n0 + e * 32 + lane;
                 a[e] = n < p.N ? (is_f16<T> ? F16_WEIGHT_LOG2 : 0.0f) - lse[n] * (1.0f / LN2) : -INFINITY;
-                d[e] = n < p.N ? -delta[n] * by : 0.0f;
+                d[e] = n < p.N && !p.own_delta ? -delta[n] * by : 0.0f;
             }
             if (i >= ST) wait(t_empty(st), (i / ST - 1) & 1);
 #pragma unroll
@@ -415,8 +447,8 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
             }
             wait(dp_full, i & 1);
             tc::fence_after_sync();
-            if (p.own_delta) {
-                // all keys are in this tile: delta = sum_m p (dout v^T)
+            if (count <= TC_ROWS) {
+                // every key of the entry is here: delta = sum_m p (dout v^T)
                 float part = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 64; j += 32) {
@@ -431,7 +463,6 @@ __device__ __forceinline__ void gradient_of_queries(const AttentionGradParams& p
                 s_part[half][threadIdx.x & 127] = part;
                 asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
                 const float all = s_part[0][threadIdx.x & 127] + s_part[1][threadIdx.x & 127];
-                if (half == 0 && n < p.N) p.delta[(static_cast<long long>(l) * p.H + h) * p.N + n] = all;
                 delta2 = pack2(-all * factor, -all * factor);
             }
             uint32_t y[32];
@@ -557,9 +588,7 @@ int launch_grad_tensor(const AttentionGradParams& p, const GradMaps& maps, cudaS
                                              static_cast<int>(keys_first)),
                            "attention_grad_tensor_kernel");
     };
-    if (!p.own_delta) return p.keys_first ? launch(kb, qb, true) : launch(qb, kb, false);
-    if (int rc = launch(qb, 0, false)) return rc;        // first those that form delta
-    return launch(kb, 0, true);
+    return p.keys_first ? launch(kb, qb, true) : launch(qb, kb, false);
 }
 
 }  // namespace

@@ -332,7 +332,7 @@ GradPlan plan_grad(const KmAttentionArgs& a) {
     p.vec_grad = rows_aligned(a.grad_q, a.type, a.d) && rows_aligned(a.grad_k, a.type, a.d) && rows_aligned(a.grad_v, a.type, a.d);
     plan.tensor = a.d <= 128 && tma_rows_ok(a.q, a.n, a.heads, a.type, a.d) && tma_rows_ok(a.grad_out, a.n, a.heads, a.type, a.d) &&
                   tma_rows_ok(a.k, a.m, a.key_heads, a.type, a.d) && tma_rows_ok(a.v, a.m, a.key_heads, a.type, a.d);
-    p.own_delta = plan.tensor && a.m <= ATT_GRAD_TENSOR_ROWS;
+    p.own_delta = a.type != ATT_F32 && a.m <= (plan.tensor ? ATT_GRAD_TENSOR_ROWS : ATT_GRAD_ROWS);
     p.kv_batch = a.kv_batch;
     const long long key_sums = static_cast<long long>(a.kv_batch == 1 ? a.l : 1) * p.G;       // heads and entries whose queries a key meets
     if (plan.tensor) {
@@ -349,8 +349,8 @@ GradPlan plan_grad(const KmAttentionArgs& a) {
             const long long fill = std::min((sms - others) / blocks, tiles / 4), even = static_cast<long long>(std::ceil(time / target));
             return static_cast<int>(std::min(std::max({1LL, fill, even}), 64LL));
         };
-        p.kv_slices = split(key_blocks, p.own_delta ? 0 : query_blocks, key_sums * query_tiles, of_keys);
-        p.q_splits  = p.own_delta ? 1 : split(query_blocks, key_blocks * p.kv_slices, key_tiles, of_queries);
+        p.kv_slices = split(key_blocks, query_blocks, key_sums * query_tiles, of_keys);
+        p.q_splits  = split(query_blocks, key_blocks * p.kv_slices, key_tiles, of_queries);
         p.keys_first = of_keys / p.kv_slices >= of_queries / p.q_splits;
     } else {
         // pieces of both sums where their tiles alone do not fill the SMs (of 64 against 128: 2 x 2000 x 40, 4 heads, 56 -> 50 us)

@@ -40,7 +40,7 @@ struct AttentionGradParams {
     const int* lengths; long long lengths_stride;
     const float* lse; long long lse_sl, lse_sh;
     float scale, scale_log2;
-    float* delta;                        // [l][h][n]: sum over channels of dout * out
+    float* delta;                        // [l][h][n]: sum over channels of dout * out, unused where few 16-bit keys share a query (attention_grad_tensor.cu)
     // float16 only, else null: from these find_factor() (attention_grad.cuh) takes the power of two that keeps the weights' gradients in
     // float16's range.
     float* peaks; int peak_count;        // [l][h][peaks]: the largest |dout| of ATT_PEAK_ROWS queries
@@ -54,7 +54,7 @@ struct AttentionGradParams {
     int   kv_batch;                      // batch entries of k and v: 1 or L
     int   kv_slices;                     // pieces of the sum over (l of a broadcast k, head of the group, query tile)
     int   keys_first;                    // tensor cores: blocks of dk and dv are the longer ones
-    int   own_delta;                     // tensor cores: the blocks of dq form delta, from weights of one key tile, for those of dk and dv
+    int   own_delta;                     // no query has more keys than that: nothing forms delta beforehand
     int   vec;                           // rows of q, k, v and dout can be read 16 bytes at a time
     int   vec_out;                       // rows of out and dout can
     int   vec_grad;                      // rows of dq, dk and dv can be written so
