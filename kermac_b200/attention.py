@@ -16,6 +16,7 @@ from .build_a_kernel import _call_result, _current_stream_for, _is_cuda, _torch_
 
 __all__ = ["cross_attention", "cross_attention_grad", "prefix_attention"]
 
+_MAX_EXTENT = 0x7fffffff      # of the 32-bit fields of KmAttentionArgs
 _TYPES = {torch.float32: _native.TYPE_FLOAT32, torch.bfloat16: _native.TYPE_BFLOAT16, torch.float16: _native.TYPE_FLOAT16}
 
 
@@ -33,6 +34,8 @@ def _check_operand(name, t, like, dims):
         raise ValueError(f"{name} must have {' or '.join(map(str, dims))} dimensions, got {t.dim()}")
     if t.size(-1) > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must have stride 1 in last dimension")
+    if max(t.shape) > _MAX_EXTENT:
+        raise ValueError(f"the extents of {name} must be below 2^31, got {tuple(t.shape)}")
 
 
 def _batch(name: str, L: int, t: torch.Tensor) -> int:
@@ -100,6 +103,8 @@ def _marshal(q, k, v, lengths, scale, prefix=None):
             raise ValueError("lengths must be on the same CUDA device as inputs")
         if lengths.dim() != 1 or (lengths.size(0) != L and L != 1):
             raise ValueError(f"lengths must have shape (L={L},), got {tuple(lengths.shape)}")
+        if lengths.size(0) > _MAX_EXTENT:
+            raise ValueError(f"the extents of lengths must be below 2^31, got {tuple(lengths.shape)}")
         L = lengths.size(0)
         args.lengths, args.lengths_stride = lengths.data_ptr(), lengths.stride(0) if L > 1 else 0
     if prefix is not None:

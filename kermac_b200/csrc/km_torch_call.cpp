@@ -543,7 +543,7 @@ bool read_attention(PyObject* pq, PyObject* pk, PyObject* pv, PyObject* lengths,
         if (!THPVariable_CheckExact(lengths)) return false;
         const at::Tensor& t = THPVariable_Unpack(lengths);
         if (!t.is_cuda() || t.scalar_type() != at::kInt || t.layout() != at::kStrided || t.device().index() != in.device || t.dim() != 1 ||
-            (t.size(0) != in.L && in.L != 1))
+            (t.size(0) != in.L && in.L != 1) || t.size(0) > MAX_EXTENT)
             return false;
         in.L = t.size(0);
         args.lengths = static_cast<const int32_t*>(t.data_ptr()), args.lengths_stride = in.L > 1 ? t.stride(0) : 0;

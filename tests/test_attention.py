@@ -314,3 +314,22 @@ def test_kernels_keep_the_order_of_overlapped_launches():
         before, wait, _ = body.partition("after_previous_grid();")
         assert wait and "return;" not in before and "tmem_alloc" not in before, name
         assert "__restrict__" not in parameters + body and "__ldg" not in body, name
+
+
+LONG = (1 << 32) + 1          # 1 in the 32 bits of the argument struct
+TOO_LONG = [
+    dict(q=_t(1, 4, 8).expand(LONG, 4, 8)),
+    dict(q=_t(1, 3, 4, 8).expand(LONG, 3, 4, 8), k=_t(1, 5, 2, 8), v=_t(1, 5, 2, 8)),
+    dict(q=_t(3, 1, 8).expand(3, LONG, 8), k=_t(5, 1, 8), v=_t(5, 1, 8)),
+    dict(k=_t(2, 1, 2, 8).expand(2, LONG, 2, 8), v=_t(2, 1, 2, 8).expand(2, LONG, 2, 8)),
+    dict(q=_t(3, 4, 8), k=_t(5, 2, 8), v=_t(5, 2, 8), lengths=_t(1, dtype=torch.int32).expand(LONG)),
+    dict(k_prefix=_t(1, 2, 8).expand(LONG, 2, 8), v_prefix=_t(1, 2, 8).expand(LONG, 2, 8)),
+]
+
+
+@pytest.mark.parametrize("changes", TOO_LONG, ids="-".join)
+def test_extents_beyond_the_argument_struct_are_refused(changes, monkeypatch):
+    _called(monkeypatch)
+    given = dict(dict(q=_t(*Q), k_prefix=_t(6, 2, 8), v_prefix=_t(6, 2, 8), k=_t(*K), v=_t(*K)), **changes)
+    with pytest.raises(ValueError, match="below 2.31"):
+        attention._marshal(given["q"], given["k"], given["v"], given.get("lengths"), None, prefix=(given["k_prefix"], given["v_prefix"]))
