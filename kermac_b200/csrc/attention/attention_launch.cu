@@ -72,6 +72,7 @@ namespace {
 enum Kind { CROSS = 0, PREFIX = 1, GRAD = 2 };
 
 constexpr long long MAX_STRIDE = 1LL << 40;
+constexpr float     LOG2E = 1.4426950408889634f;
 
 int check_heads(const char* name, const KmHeads& t, long long rows, long long heads, long long batch) {
     if (batch * rows * heads > 0 && !t.ptr) return fail(KM_ERR_NULL_POINTER, "%s must not be NULL", name);
@@ -204,8 +205,8 @@ Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool split, bool planes) 
     p.q = heads(a.q), p.k = heads(a.k), p.v = heads(a.v), p.out = heads(a.out), p.kp = heads(a.k_prefix), p.vp = heads(a.v_prefix);
     p.lengths = a.lengths, p.lengths_stride = a.lengths_stride;
     p.lse = a.lse, p.lse_sl = a.lse_stride_l, p.lse_sh = a.lse_stride_head;
-    // a scale of 0 becomes 2^-100: the same weights, and the -inf of a masked score stays -inf
-    p.scale_log2 = std::max(a.scale * 1.4426950408889634f, 0x1p-100f);
+    // a scale of 0 becomes 2^-149: the -inf of a masked score stays -inf, and no finite score, below 2^128, moves a weight by more than 2^-21
+    p.scale_log2 = std::max(a.scale * LOG2E, 0x1p-149f);
     p.causal = kind == PREFIX;
     // Keys that a whole batch shares are a prefix without own keys.
     if (kind == CROSS && a.l > 1 && a.k.stride_l == 0 && !a.lengths && a.m > 0) {
@@ -325,7 +326,7 @@ GradPlan plan_grad(const KmAttentionArgs& a) {
     p.dq = heads(a.grad_q), p.dk = heads(a.grad_k), p.dv = heads(a.grad_v);
     p.lengths = a.lengths, p.lengths_stride = a.lengths_stride;
     p.lse = a.lse, p.lse_sl = a.lse_stride_l, p.lse_sh = a.lse_stride_head;
-    p.scale = a.scale, p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.scale = a.scale, p.scale_log2 = a.scale * LOG2E;
     p.vec = rows_aligned(a.q, a.type, a.d) && rows_aligned(a.k, a.type, a.d) && rows_aligned(a.v, a.type, a.d) &&
             rows_aligned(a.grad_out, a.type, a.d);
     p.vec_out  = rows_aligned(a.out, a.type, a.d) && rows_aligned(a.grad_out, a.type, a.d);

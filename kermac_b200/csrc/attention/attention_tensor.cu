@@ -105,7 +105,7 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
                 if (lane == 0) mbar_arrive(q_full(t));
             }
 
-            // -inf times the scale of 0 would be NaN; the launcher passes at least 2^-100
+            // -inf times the scale of 0 would be NaN; the launcher passes at least 2^-149
             const float c = p.scale_log2;
             const int   limit = min(row_limit(p, w, at < w.rows ? at : w.rows - 1), w.end);
             const int   all_see = w.causal ? w.length - p.N + 1 : w.length;     // keys in front of it are seen by every row

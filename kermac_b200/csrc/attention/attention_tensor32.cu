@@ -150,7 +150,7 @@ attention_tensor32_kernel(const __grid_constant__ AttentionParams p, const __gri
         const uint32_t mine = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + t * P32_COLS, s_col = mine + half * 64;
         const Row      row = find_row(p, w, min(at, w.rows - 1));
         if (t < groups) {
-            const float c = p.scale_log2;                // at least 2^-100: -inf stays -inf
+            const float c = p.scale_log2;                // at least 2^-149: -inf stays -inf
             const int   limit = min(row_limit(p, w, min(at, w.rows - 1)), w.end) - half * 64;
             const int   all_see = min(w.causal ? w.length - p.N + 1 : w.length, w.end);     // keys in front of it are seen by every row
             float top = -INFINITY, sum = 0.0f, o[32];

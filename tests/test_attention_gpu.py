@@ -656,3 +656,17 @@ def test_sequences_of_few_keys_have_an_exact_delta(dtype, D, layout, M, keys):
     # a tenth above 0.425: some 10^5 independent values of grad_q, and 10^3 of the others
     assert found[0] <= 0.47, found
     assert max(found[1:]) <= 0.55, found
+
+
+@pytest.mark.parametrize("dtype", TYPES[:2], ids=str)             # float16 scores do not get that far
+@pytest.mark.parametrize("N, D", [(1, 64), (150, 64), (150, 128), (150, 136)])
+def test_a_scale_of_zero_makes_all_weights_equal(dtype, N, D):
+    # scores of 2^106 and more, which a factor of 2^-100 in the place of the zero did not make equal
+    M = 300
+    q = torch.full((1, N, 2, D), 2.0 ** 50, device="cuda").to(dtype)
+    k = make(2, 1, M, 2, D, dtype=dtype, by=2.0 ** 50)
+    v = make(3, 1, M, 2, D, dtype=dtype)
+    out, lse = kermac.cross_attention(q, k, v, scale=0.0, return_lse=True)
+    want, want_lse, bound, lse_bound = ao.attention(q * 2.0 ** -50, k * 2.0 ** -50, v, scale=0.0)
+    assert_within(out, want, bound, "out")
+    assert_within(lse, want_lse, lse_bound, "lse")
