@@ -103,7 +103,7 @@ int check(const KmAttentionArgs* a, Kind kind) {
         return fail(KM_ERR_BAD_SHAPE, "heads (%d) must be a multiple of key_heads (%d)", a->heads, a->key_heads);
     if (a->d < 1 || a->d > 256) return fail(KM_ERR_BAD_SHAPE, "the number of channels must be in [1, 256], got %d", a->d);
     if (a->type < ATT_F32 || a->type > ATT_F16) return fail(KM_ERR_BAD_ENUM, "type must be a KM_TYPE_*");
-    if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return fail(KM_ERR_BAD_HYPERPARAM, "scale must be finite and not negative");
+    if (!(a->scale >= 0.0f) || std::isinf(a->scale * LOG2E)) return fail(KM_ERR_BAD_HYPERPARAM, "scale must be finite and not negative (and below 2^127)");
     if (kind != PREFIX && a->prefix != 0) return fail(KM_ERR_BAD_SHAPE, "only prefix_attention has a prefix");
     if (a->m > (1 << 30) || a->prefix > (1 << 30)) return fail(KM_ERR_TOO_LARGE, "more than 2^30 keys");
     const long long rows = static_cast<long long>(a->l) * a->n * a->heads;

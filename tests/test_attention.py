@@ -333,3 +333,10 @@ def test_extents_beyond_the_argument_struct_are_refused(changes, monkeypatch):
     given = dict(dict(q=_t(*Q), k_prefix=_t(6, 2, 8), v_prefix=_t(6, 2, 8), k=_t(*K), v=_t(*K)), **changes)
     with pytest.raises(ValueError, match="below 2.31"):
         attention._marshal(given["q"], given["k"], given["v"], given.get("lengths"), None, prefix=(given["k_prefix"], given["v_prefix"]))
+
+
+def test_a_scale_that_overflows_in_powers_of_two_is_refused():
+    for kind in range(3):
+        args = _c_args(scale=3.0e38)                                              # times log2(e): infinity
+        assert getattr(_native.lib(), _native.ATTENTION_SYMBOLS[kind])(ctypes.byref(args), None) == -5
+    assert _native.describe_attention(_c_args(scale=2.0e38), 0)
