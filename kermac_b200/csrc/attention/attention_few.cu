@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(THREADS) attention_few_kernel(const __grid_con
         for (int r = 0; r < NR; ++r) {
             float minus[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) minus[e] = top[r][e] == -INFINITY ? 0.0f : -top[r][e] * p.scale_log2;
+            for (int e = 0; e < 2; ++e) minus[e] = top[r][e] == -INFINITY ? 0.0f : weight_log2<T> - top[r][e] * p.scale_log2;
 #pragma unroll
             for (int m = 0; m < BLOCKS; ++m) {
 #pragma unroll
@@ -244,8 +244,8 @@ __global__ void __launch_bounds__(THREADS) attention_few_kernel(const __grid_con
         for (int e = 0; e < 2; ++e) {
             float* const at = sums + (warp * S::ROWS + r * 8 + 2 * t + e) * S::W;
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d) at[d * 16 + g] = o[d][r][e], at[d * 16 + g + 8] = o[d][r][e + 2];
-            const float total = column_sum(sum[r][e]);
+            for (int d = 0; d < DP / 16; ++d) at[d * 16 + g] = o[d][r][e] * per_weight<T>, at[d * 16 + g + 8] = o[d][r][e + 2] * per_weight<T>;
+            const float total = column_sum(sum[r][e]) * per_weight<T>;
             if (g == 0) at[DP] = top[r][e] == -INFINITY ? -INFINITY : top[r][e] * p.scale_log2, at[DP + 1] = total;
         }
     __syncthreads();

@@ -6,11 +6,6 @@
 namespace km {
 namespace att {
 
-// float16 weights are multiplied by this before they are rounded: they are at most 1, and float16 ends at 6e-8.
-constexpr float F16_WEIGHT = 256.0f, F16_WEIGHT_LOG2 = 8.0f;
-
-template <typename T> constexpr bool is_f16 = std::is_same<T, __half>::value;
-
 // What a weight's gradient ds = p (dout v^T - delta) is multiplied by before it is rounded to float16; the sums are divided by it.
 // |dout v^T| and |delta| are at most x = D max|dout| max|v|, over the keys that are seen: with 2^13 over the power of two at or below x the product
 // stays below 2^15, half of what float16 has, and a ds of 2^-27 x still has all its bits (dout v^T of random signs is some 2^-7 x at 128

@@ -65,7 +65,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, i
         }
     const bool  idle   = key0 >= longest;
     const float factor = idle ? 1.0f : find_factor<T>(p, l_first, l_first + l_count, hk, kl, longest);
-    const float by     = is_f16<T> ? factor / F16_WEIGHT : 1.0f;
+    const float by     = factor * per_weight<T>;
 
     float dk[CT][4], dv[CT][4];
 #pragma unroll
@@ -136,7 +136,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, i
                 for (int e = 0; e < 4; ++e) {
                     const int   col  = j * 8 + 2 * t + (e & 1);
                     const bool  seen = key0 + warp * 16 + g + 8 * (e >> 1) < count && n0 + col < p.N;
-                    const float w    = ex2_approx(fmaf(s[j][e], p.scale_log2, (is_f16<T> ? F16_WEIGHT_LOG2 : 0.0f) - lse[col] * (1.0f / LN2)));
+                    const float w    = ex2_approx(fmaf(s[j][e], p.scale_log2, weight_log2<T> - lse[col] * (1.0f / LN2)));
                     ds[j][e] = seen ? w * ((ds[j][e] - delta[col]) * by) : 0.0f;
                     s[j][e]  = seen ? w : 0.0f;
                 }
@@ -148,7 +148,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, i
     }
     float* const dk_part = p.kv_slices > 1 ? p.dk_part + static_cast<long long>(slice) * p.kv_batch * p.M * p.Hk * p.D : nullptr;
     float* const dv_part = p.kv_slices > 1 ? p.dv_part + static_cast<long long>(slice) * p.kv_batch * p.M * p.Hk * p.D : nullptr;
-    const float  k_by = p.scale / factor, v_by = is_f16<T> ? 1.0f / F16_WEIGHT : 1.0f;
+    const float  k_by = p.scale / factor, v_by = per_weight<T>;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const int key = key0 + warp * 16 + g + 8 * r;

@@ -164,7 +164,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
 
     if (warp < S::WARPS_ON_WEIGHTS) {
         // ------------------------------------------------------------------ weights: lane = key, 64 queries of a tile
-        const float    factor = find_this_factor(), by = is_f16<T> ? factor / F16_WEIGHT : 1.0f;
+        const float    factor = find_this_factor(), by = factor * per_weight<T>;
         const int      half = warp >> 2, key = key0 + (threadIdx.x & 127);
         const uint32_t at   = (static_cast<uint32_t>((warp & 3) * 32) << 16) + half * 64;
         const u64      c2 = pack2(p.scale_log2, p.scale_log2), by2 = pack2(by, by);
@@ -223,7 +223,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
                             const float other = __shfl_xor_sync(0xffffffffu, upper ? x[e] : x[e + d], d);
                             x[e] = (upper ? x[e + d] : x[e]) + other;
                         }
-                    parts[(warp & 3) * TC_ROWS + half * 64 + j + lane] = is_f16<T> ? x[0] * (1.0f / F16_WEIGHT) : x[0];
+                    parts[(warp & 3) * TC_ROWS + half * 64 + j + lane] = x[0] * per_weight<T>;
                 }
                 asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
                 if (half == 0) {
@@ -265,7 +265,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
         const Heads& dst   = half == 0 ? p.dv : p.dk;
         float* const whole = half == 0 ? p.dv_part : p.dk_part;
         float* const part  = p.kv_slices > 1 ? whole + static_cast<long long>(slice) * p.kv_batch * p.M * p.Hk * p.D : nullptr;
-        const float  times = half == 0 ? (is_f16<T> ? 1.0f / F16_WEIGHT : 1.0f) : p.scale / factor;
+        const float  times = half == 0 ? per_weight<T> : p.scale / factor;
         const uint32_t sums = (half == 0 ? dv_col : dk_col) + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         if (n_items > 0) {
             // q and dout tiles have been used for the last time
@@ -300,7 +300,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
         __syncwarp();
     } else if (warp == S::STATS_WARP) {
         // ------------------------------------------------------------------ lse and delta of the query tiles
-        const float by = is_f16<T> ? find_this_factor() / F16_WEIGHT : 1.0f;
+        const float by = find_this_factor() * per_weight<T>;
         for (int i = 0; i < n_items; ++i) {
             const int st = i % ST, item = from + i, lg = item / q_tiles, l = l_first + lg / p.G, h = hk * p.G + lg % p.G;
             const int n0 = item % q_tiles * TC_ROWS;
@@ -310,7 +310,7 @@ __device__ __forceinline__ void gradient_of_keys(const AttentionGradParams& p, c
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int n = n0 + e * 32 + lane;
-                a[e] = n < p.N ? (is_f16<T> ? F16_WEIGHT_LOG2 : 0.0f) - lse[n] * (1.0f / LN2) : -INFINITY;
+                a[e] = n < p.N ? weight_log2<T> - lse[n] * (1.0f / LN2) : -INFINITY;
                 d[e] = n < p.N && !p.own_delta ? -delta[n] * by : 0.0f;
             }
             if (i >= ST) wait(t_empty(st), (i / ST - 1) & 1);

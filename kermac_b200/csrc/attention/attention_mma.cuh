@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "../km_common.cuh"
 #include "attention_params.h"
@@ -47,6 +48,14 @@ template <> struct Type<__half> {
         return r;
     }
 };
+
+template <typename T> constexpr bool is_f16 = std::is_same<T, __half>::value;
+
+// float16 weights are multiplied by 2^8 before they are rounded, and the sums divided by it: they are at most 1 (in attention_tensor.cu 2^5), and
+// float16 ends at 2^-24.  131072 keys of weight 2^-25 beside one of weight 1 are 1/256 of the result and were none of it without.
+constexpr float F16_WEIGHT = 256.0f, F16_WEIGHT_LOG2 = 8.0f;
+template <typename T> constexpr float weight_log2 = is_f16<T> ? F16_WEIGHT_LOG2 : 0.0f;
+template <typename T> constexpr float per_weight  = is_f16<T> ? 1.0f / F16_WEIGHT : 1.0f;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 

@@ -122,13 +122,13 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[j][e] = ex2_approx(s[j][e] - base[e >> 1]);
+                s[j][e] = ex2_approx(s[j][e] - (base[e >> 1] - weight_log2<T>));
                 sum[e >> 1] += s[j][e];
             }
         product_nn<T, DP, NT, CT>(o, s, tile_k + S::KEYS * TL::LD);
         group_sync();
     }
-    sum[0] = quad_sum(sum[0]), sum[1] = quad_sum(sum[1]);
+    sum[0] = quad_sum(sum[0]) * per_weight<T>, sum[1] = quad_sum(sum[1]) * per_weight<T>;
 
     if constexpr (!FEW) {
 #pragma unroll
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
             const int at = w.row0 + my_row + 8 * r;
             if (at >= w.rows) continue;
             const Row   row = find_row(p, w, at);
-            const float by  = sum[r] == 0.0f ? 0.0f : 1.0f / sum[r];
+            const float by  = sum[r] == 0.0f ? 0.0f : per_weight<T> / sum[r];
             if (t == 0) put_stats(p, w, row, top[r], sum[r]);
 #pragma unroll
             for (int c = 0; c < CT; ++c) put_pair<T>(p, w, row, c * 8 + 2 * t, o[c][2 * r] * by, o[c][2 * r + 1] * by);
@@ -150,7 +150,8 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
         for (int r = 0; r < 2; ++r) {
             float* const mine_at = sums + (warp * S::ROWS + g + 8 * r) * W;
 #pragma unroll
-            for (int c = 0; c < CT; ++c) *reinterpret_cast<float2*>(mine_at + c * 8 + 2 * t) = make_float2(o[c][2 * r], o[c][2 * r + 1]);
+            for (int c = 0; c < CT; ++c)
+                *reinterpret_cast<float2*>(mine_at + c * 8 + 2 * t) = make_float2(o[c][2 * r] * per_weight<T>, o[c][2 * r + 1] * per_weight<T>);
             if (t == 0) mine_at[DP] = top[r], mine_at[DP + 1] = sum[r];
         }
         __syncthreads();

@@ -5,7 +5,8 @@
 // O stays in tensor memory.  While one tile's warps work on their weights the tensor cores multiply for the other tile.
 //
 // The running maximum that weights are taken against may lag: it is raised, and O scaled, only where a row's maximum has grown by more
-// than 2^8, so that weights are at most 256 (the first tile sets it; after that it seldom happens).
+// than 2^8, so that weights are at most 256 (the first tile sets it; after that it seldom happens).  float16 weights, which are 2^8 times as large, see
+// attention_mma.cuh, have 2^5, an eighth of that type's range.
 //
 // 4 x 4096 x 8192, 16 heads of 128, bf16: 887 us, 1.24 PFLOP/s at the 1.65 GHz that the power limit leaves; the products alone, without
 // a softmax, take 783.  A step (two tiles of rows, 128 keys) is 3440 cycles for products of 2048.  Tried: two threads a row (eight
@@ -110,7 +111,8 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
             const int   limit = min(row_limit(p, w, at < w.rows ? at : w.rows - 1), w.end);
             const int   all_see = w.causal ? w.length - p.N + 1 : w.length;     // keys in front of it are seen by every row
             // slack: how far a row's maximum may grow; -inf where nothing but scores of -inf has come, whose maximum of 0 any other replaces
-            float top = 0.0f, sum = 0.0f, slack = 8.0f;
+            constexpr float SLACK = is_f16<T> ? 5.0f : 8.0f;
+            float top = 0.0f, sum = 0.0f, slack = SLACK;
             for (int i = 0; i < n_tiles; ++i) {
                 const int first = w.first + i * TC_ROWS;
                 wait(s_full(t), i & 1);
@@ -139,7 +141,7 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
                     if (__any_sync(0xffffffffu, grown)) {
                         // the products into O that were issued before this S are complete
                         const float shrink = grown && slack > 0.0f ? ex2_approx((top - high) * c) : 1.0f;
-                        if (grown) top = high, slack = 8.0f;
+                        if (grown) top = high, slack = SLACK;
                         sum *= shrink;
 #pragma unroll
                         for (int j = 0; j < DP; j += 32) {
@@ -153,7 +155,7 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
                         }
                     }
                 }
-                const u64 c2 = pack2(c, c), m2 = pack2(-top * c, -top * c);
+                const u64 c2 = pack2(c, c), m2 = pack2(weight_log2<T> - top * c, weight_log2<T> - top * c);
                 u64 total[2] = {0, 0};
 #pragma unroll
                 for (int j = 0; j < 64; j += 32) {
@@ -192,7 +194,8 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
             wait(o_full(t), 0);
             tc::fence_after_sync();
             const bool  good = *reinterpret_cast<volatile int*>(&s_expired) == 0 && at < w.rows;
-            const float by  = sum == 0.0f ? 0.0f : 1.0f / sum;
+            sum *= per_weight<T>;
+            const float by  = sum == 0.0f ? 0.0f : per_weight<T> / sum;
             if (good) put_stats(p, w, row, top * c, sum);
             if (p.parts > 1 || p.vec_out) {
                 // the warp's rows of Q have been used for the last time

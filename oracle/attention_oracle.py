@@ -49,7 +49,8 @@ def _one(q, k, v, seen, scale, dtype):
     if dtype == torch.float32:
         bound = bound + (p @ v.abs()) * 2.0 ** -21
     if dtype == torch.float16:
-        bound = bound + 2.0 ** -25 * (1.0 + v.abs().sum(dim=0))
+        # half of the smallest step: of the result, and of a weight, which the kernels multiply by 2^8 before they round it
+        bound = bound + 2.0 ** -25 + 2.0 ** -33 * v.abs().sum(dim=0)
     return p, out, lse, bound, weight, E * off
 
 

@@ -670,3 +670,19 @@ def test_a_scale_of_zero_makes_all_weights_equal(dtype, N, D):
     want, want_lse, bound, lse_bound = ao.attention(q * 2.0 ** -50, k * 2.0 ** -50, v, scale=0.0)
     assert_within(out, want, bound, "out")
     assert_within(lse, want_lse, lse_bound, "lse")
+
+
+@pytest.mark.parametrize("L, N", [(148, 1), (148, 9), (37, 300), (20, 600)])      # as many blocks as there are SMs: the keys are not divided
+@pytest.mark.parametrize("D", [64, 128, 136])
+def test_float16_weights_below_the_smallest_float16(L, N, D):
+    # one key takes nearly all of the weight and has v = 0 (as a first token may); the others' weights of 2^-25 make the result
+    M = 20000
+    q, k = torch.zeros(L, N, 1, D, dtype=torch.float16, device="cuda"), torch.zeros(1, M, 1, D, dtype=torch.float16, device="cuda")
+    q[..., 0], k[:, 7, :, 0] = 4.0, 25.1 * math.log(2.0) / 4
+    v = torch.ones_like(k)
+    v[:, 7] = 0.0
+    k, v = (t.expand(L, M, 1, D).contiguous() for t in (k, v))
+    out = kermac.cross_attention(q, k, v, scale=1.0)
+    others = (M - 1) * math.exp(-4.0 * float(k[0, 7, 0, 0]))
+    # half a step of the result, 2^-11 of it, and of each weight of 2^-25.1 before 2^-33
+    assert (out.double() - others / (1.0 + others)).abs().max() <= others * (2.0 ** -11 + 2.0 ** -7) + 2.0 ** -25
