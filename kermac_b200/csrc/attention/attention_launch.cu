@@ -174,17 +174,17 @@ struct Plan {
     long long bytes() const { return parts + planes; }
 };
 
-// keys: of the set; all_keys: of both.
-Form choose_form(long long rows, bool tma_ok, int type, int d, int keys, int all_keys, bool planes) {
+// keys: of both sets.
+Form choose_form(long long rows, bool tma_ok, int type, int d, long long keys, bool planes) {
     if (tma_ok && rows > 16) return {TENSOR, ATT_TENSOR_ROWS, 1, 256};
-    if (tma_ok) return {FEW, rows <= 8 ? 8 : 16, d <= 64 || attention_few_tile(d, keys, 0) == 16 ? 2 : 1, 128};
+    if (tma_ok) return {FEW, rows <= 8 ? 8 : 16, 0, 128};             // plan_forward() knows how many blocks an SM holds
     // These two take long for a key, and their pieces are short: 64 keys against 256, a token of 500 (8 heads of 128) in float32 42.0 -> 17.5 us;
     // 32 against 256, 2 x 300 x 500 (4 heads of 128) 120 -> 42, and against 64, 300 x 300 (4 heads of 256) 54 -> 42.  As many blocks as the shared
     // memory of an SM holds; with twice as many 2 x 2000 x 200 (4 heads of 128) 71.8 -> 100.8.
     if (rows <= ATT_FEW_ROWS) return {SCALAR_FEW, ATT_FEW_ROWS, d <= 64 ? 2 : 1, 64};
     // Above 32 keys: see attention_tensor32.cu.  Pieces of 192 keys: a tile of 128 is 5 us, the join 4 to 6 (2 x 300 x 500, 4 heads: one piece
     // 27.5 us, two 21.2; but 2 x 2000 x 260, which 128 would split, 23.7 and 28.5).
-    if (planes && all_keys > 32) return {TENSOR32, ATT_TENSOR_ROWS, 1, 192};
+    if (planes && keys > 32) return {TENSOR32, ATT_TENSOR_ROWS, 1, 192};
     // (float32 of up to 64 channels, which has more than 32 keys here where planes cannot be had: 64; 1024 queries of 64 keys, 8 heads, 12.8, with 32 16.6)
     if (type == ATT_F32 && d <= 64) return {ROWS, ATT_TILE_ROWS, 4, 64};
     return {ROWS, ATT_TILE_ROWS, type != ATT_F32 || d <= 128 ? 2 : 1, 32};
@@ -224,8 +224,9 @@ Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool split, bool planes) 
                                           : own_ok;
     p.vec_out = rows_aligned(a.out, a.type, a.d);
     const long long own_rows = static_cast<long long>(p.N) * p.G, prefix_rows = own_rows * p.L;
-    plan.own    = choose_form(own_rows, own_ok, a.type, p.D, p.M, p.M + p.P, planes);
-    plan.prefix = choose_form(prefix_rows, prefix_ok, a.type, p.D, p.P, p.M + p.P, planes);
+    const long long keys = static_cast<long long>(p.M) + p.P;
+    plan.own    = choose_form(own_rows, own_ok, a.type, p.D, keys, planes);
+    plan.prefix = choose_form(prefix_rows, prefix_ok, a.type, p.D, keys, planes);
     // A short prefix goes along with few own rows: its keys are read again, from L2, for every 8 or 16 rows, which costs less than a launch
     // of its own up to some 8 MB (72 sequences with 64 keys before 40 own ones, 2 key heads of 128: 19.2 -> 11.9 us; 1024 keys, 24 MB: 23.4
     // and 22.2; 4096: 23.6 and 39.0).
@@ -234,6 +235,11 @@ Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool split, bool planes) 
     // one launch for both sets where the same kernel takes them
     if (p.M > 0 && p.P > 0 && plan.own.kernel == FEW && plan.prefix.kernel == FEW)
         plan.own.rows = plan.prefix.rows = std::max(plan.own.rows, plan.prefix.rows);
+    // the tiles of the launch, which may have both sets, and so the blocks that an SM holds
+    const int few_tile   = attention_few_tile(p.D, plan.own.kernel == FEW ? p.M : 0, plan.prefix.kernel == FEW ? p.P : 0);
+    const int few_per_sm = p.D <= 64 || few_tile == 16 ? 2 : 1;
+    for (Form* form : {&plan.own, &plan.prefix})
+        if (form->kernel == FEW) form->per_sm = few_per_sm;
     if (p.M > 0 || p.P == 0) {
         p.own_tiles  = static_cast<int>(ceil_div_ll(own_rows, plan.own.rows));
         p.own_splits = split ? pieces(static_cast<long long>(p.own_tiles) * p.L * p.Hk, p.M, plan.own.per_sm, plan.own.least) : 1;

@@ -340,3 +340,13 @@ def test_a_scale_that_overflows_in_powers_of_two_is_refused():
         args = _c_args(scale=3.0e38)                                              # times log2(e): infinity
         assert getattr(_native.lib(), _native.ATTENTION_SYMBOLS[kind])(ctypes.byref(args), None) == -5
     assert _native.describe_attention(_c_args(scale=2.0e38), 0)
+
+
+def test_pieces_are_planned_for_the_blocks_that_the_launch_has():
+    # 4 tokens of 8 heads of 128, 1024 own keys below 4000 of a prefix: one launch of 32-key tiles, of which an SM holds one block, so that the
+    # 32 blocks of own keys get 148 / 32 pieces, not the 296 / 32 of short keys alone
+    args = _c_args(l=4, n=1, m=1024, heads=8, key_heads=8, d=128, prefix=4000)
+    for name, rows in (("q", 1), ("out", 1), ("k", 1024), ("v", 1024), ("k_prefix", 4000), ("v_prefix", 4000)):
+        setattr(args, name, _native.KmHeads(4096, rows * 8 * 128, 8 * 128, 128))
+    args.lse_stride_l, args.lse_stride_head = 8, 1
+    assert "own=few rows=8 tiles=1 splits=4 prefix=few rows=8 tiles=1 splits=18" in _native.describe_attention(args, 1)
