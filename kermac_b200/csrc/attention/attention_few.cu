@@ -5,13 +5,22 @@
 // are the narrow side of an instruction, eight at a time, where the other way round 16 rows would be computed for one
 // token.  Q stays in registers; P^T passes from accumulator to operand layout by movmatrix.
 //
-// Measured at 64 sequences x 1 x 4096 keys (ragged), 32 heads of 128, 8 key heads, float16, 674 MB: copies by the lanes
-// (cp.async, 480 of some 700 instructions a tile) with 16 rows an instruction took 294 us, this takes 105: 6.4 TB/s, 99 % of a plain
-// copy.  Two warps a block and two blocks an SM: 118.
+// Measured at 64 sequences x 1 x 4096 keys (ragged), 32 heads of 128, 8 key heads, float16, 674 MB, back-to-back passes over three sets of
+// inputs: 111 us, 6.1 TB/s, 94 % of a plain copy.  While it was written, one pass at a time: copies by the lanes (cp.async, 480 of some 700
+// instructions a tile) with 16 rows an instruction 294 us, this 105; two warps a block and two blocks an SM 118.
 //
 // Two blocks an SM hide what a block does before its first and behind its last tile.  Up to 64 channels they fit; above, tiles of 16
-// keys make room for them and pay where a block has few keys: 128 sequences with 100 to 1024 keys below a prefix of 32768 143.9 -> 138.4 us
-// a pass, but the 64 x 4096 keys above 110.4 -> 113.9.
+// keys make room for them: attention_few_tile().  It goes by the keys that an entry may have, M, because lengths are on the device.  With tiles of 32 and
+// of 16, us, one token of 4 query heads to each of 8 key heads of 128 (of 80):
+//     keys              512          1024          2048          3000          4096          8192
+//     4 sequences       6.9   7.4    8.3  10.8    11.6  13.7    14.7  17.6    17.1  20.1    27.6  30.7
+//     16                9.6  10.4   14.7  16.2    24.4  26.3    33.3  35.7    43.2  46.1    80.0  86.2
+//     32               18.7  14.5   27.8  24.7    45.4  44.5    62.6  62.9    81.0  84.3     154   162
+//     64               34.6  27.1   52.2  45.4    88.8  80.9     124   116     162   155     309   302
+//     32, 80 channels  16.6  12.4   24.3  18.9    38.7  31.5    52.8  43.3    67.3  56.4     124   106
+// Tiles of 16 gain up to 26 % where there are more blocks than SMs, up to some 2500 keys (ragged 64 x 4096: 110.4 and 113.9), and lose up to 30 % where there
+// are fewer and their keys are divided.  Taking 32 there as well is not the better rule: one block an SM leaves room for fewer clusters, and 8 pieces of 1081
+// keys, 16 heads, went from 9.7 to 15.6 us, 5 pieces of 1718 keys, 40 heads, from 18.5 to 10.6.
 #include <algorithm>
 
 #include "attention_tcgen05.cuh"

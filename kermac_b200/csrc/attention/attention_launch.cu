@@ -176,7 +176,12 @@ struct Plan {
 
 // keys: of both sets.
 Form choose_form(long long rows, bool tma_ok, int type, int d, long long keys, bool planes) {
+    // 16 rows: two tiles of FEW for 17 to 32 rows against one block of TENSOR, us: 64 channels 85 and 114 (64 x 2000 keys, 8 key heads), 28 and 35
+    // (32 x 1000); 128 channels 131 and 132, 45 and 41, 88 and 64 (16 x 4000, 32 rows).  Pieces of 256 keys, two tiles, against 128 and 512: 100 rows
+    // of 2000 keys, 8 heads, 15.6, 15.3 and 19.5; 100 of 500, 11.0, 11.7 and 11.0; 256 of 4000, 4 heads, 19.0, 17.7 and 21.2.
     if (tma_ok && rows > 16) return {TENSOR, ATT_TENSOR_ROWS, 1, 256};
+    // Pieces of 128 keys, a tile for each warp, against 64 and 256: a token of 8 heads of 128 and 1000 keys 8.4, 10.2 and 9.3; of 500 7.1, 7.8 and 8.6; of 8 heads
+    // of 64 and 1000 keys 7.6, 9.6 and 6.9; 2 tokens of 2000 keys, 2 key heads, 11.5, 9.5 and 10.8.
     if (tma_ok) return {FEW, rows <= 8 ? 8 : 16, 0, 128};             // plan_forward() knows how many blocks an SM holds
     // These two take long for a key, and their pieces are short: 64 keys against 256, a token of 500 (8 heads of 128) in float32 42.0 -> 17.5 us;
     // 32 against 256, 2 x 300 x 500 (4 heads of 128) 120 -> 42, and against 64, 300 x 300 (4 heads of 256) 54 -> 42.  As many blocks as the shared
