@@ -56,9 +56,13 @@ int kermac_b200_prefix_attention(const KmAttentionArgs* args, void* stream);
 /* grad_q, grad_k and grad_v from grad_out and the forward pass's out and lse.  Every row is written, those of keys behind
  * lengths[l] with zeros.  The sums have a fixed order: equal calls give equal bits. */
 int kermac_b200_cross_attention_grad(const KmAttentionArgs* args, void* stream);
-/* Bytes of scratch that the three calls use (0: none): partial sums, 512 MB at most, and copies of float32 inputs of up to 64
- * channels, 1 GiB at most.  The two forward calls take less or none, and are slower then, unless there are both a prefix and own
- * keys, whose partial sums they need; the gradient needs all of it. */
+/* Bytes of scratch that the three calls use (0: none), with MB = 2^20 bytes.
+ * Forward: partial sums where keys are divided, 512 MB at most, and copies of float32 inputs of up to 64 channels, 384 bytes a row of a
+ * head of each of them (whatever d is), 1024 MB at most.  These two calls take less or none, and are slower then.  But where there are both
+ * a prefix and own keys a row has a part for each: 8 * l * n * heads * (d + 2) bytes at least, however much that is, and without it the
+ * call is refused.
+ * Gradient: 4 * l * n * heads bytes, with float16 a 64th of that and 4 bytes for 64 keys of a head besides; 4 * l * n * heads * d for the sum
+ * over the batch where q_batch is 1 and l is not; where sums are divided 256 MB at most for each of the three gradients.  It needs all of it. */
 int64_t kermac_b200_cross_attention_scratch_bytes(const KmAttentionArgs* args);
 int64_t kermac_b200_prefix_attention_scratch_bytes(const KmAttentionArgs* args);
 int64_t kermac_b200_cross_attention_grad_scratch_bytes(const KmAttentionArgs* args);

@@ -196,7 +196,7 @@ def cross_attention(
     Scores, softmax and sums are 32-bit; with 16-bit types the weights are rounded to that type for the product with v.  float32 inputs
     are taken apart into three bfloat16 or two tf32 parts: those that are used have to be finite and below 2^127.  Equal calls give
     equal bits.  Partial sums, where few queries look at many states (at most 512 MB), and copies of float32 inputs
-    of up to 64 channels (1.5 times their size, at most 1 GiB) are taken from torch's allocator for the duration of the call.
+    of up to 64 channels (384 bytes a row of a head, at most 1 GiB) are taken from torch's allocator for the duration of the call.
     Launches on torch's current stream and returns without synchronising; like every allocation by torch that has to be
     captured through torch.cuda.graph.
 
@@ -223,7 +223,8 @@ def prefix_attention(
 
     q: (L, N, H, D); k_prefix, v_prefix: (P, Hk, D), the prefix, read and multiplied once for the whole batch; k, v: (L, M, Hk, D),
     each sequence's own tokens, of which `lengths` (or all M) are there, the N newest included.  Query n sees the whole prefix
-    and own token j when j <= lengths[l] - N + n.  P and M may be 0.  Everything else as in `cross_attention`.
+    and own token j when j <= lengths[l] - N + n.  P and M may be 0.  Everything else as in `cross_attention`, but for the partial sums: where
+    there are both a prefix and own tokens each of the two takes 4 (D + 2) bytes a query and head at least, without a limit.
     """
     return _forward(_native.ATTENTION_PREFIX, q, k, v, lengths, scale, out, lse, return_lse, debug, prefix=(k_prefix, v_prefix))
 
@@ -251,7 +252,8 @@ def cross_attention_grad(
     the call is given, allocated when None.
 
     Sums are 32-bit and in a fixed order: equal calls give equal bits.  Takes scratch from torch's allocator for the duration
-    of the call: 4 bytes a query and head, and partial sums where an input is broadcast or few states meet many queries.
+    of the call: 4 bytes a query and head (float16: some more), another 4 D where q is broadcast over the batch, and partial sums where
+    sums over states or queries are divided (at most 256 MB for each gradient).
     """
     call = _native._call
     if call is None:

@@ -265,10 +265,10 @@ Plan plan_forward(const KmAttentionArgs& a, Kind kind, bool split, bool planes) 
 
 bool empty(const KmAttentionArgs& a) { return a.l == 0 || a.n == 0 || a.heads == 0; }
 
-// The most scratch that a call asks for: partial sums, and planes of float32 inputs.
+// The most scratch that a call asks for beyond the two parts of a row that both sets of keys need: partial sums, and planes of float32 inputs.
 constexpr long long MOST_SCRATCH = 512LL << 20, MOST_PLANES = 1LL << 30;
 
-// The plan that a scratch of `most` bytes allows: first without planes, then with a single piece for each set of keys.
+// The plan that a scratch of `most` bytes allows: first without planes, then with a single piece for each set of keys, whatever these two take.
 Plan plan_within(const KmAttentionArgs& a, Kind kind, long long most) {
     Plan plan = {};
     const bool one_set = a.l > 1 && a.k.stride_l == 0 && a.lengths;      // see attention_tensor32_launch

@@ -54,7 +54,7 @@ struct AttentionGradParams {
     int   kv_batch;                      // batch entries of k and v: 1 or L
     int   kv_slices;                     // pieces of the sum over (l of a broadcast k, head of the group, query tile)
     int   keys_first;                    // tensor cores: blocks of dk and dv are the longer ones
-    int   own_delta;                     // no query has more keys than that: nothing forms delta beforehand
+    int   own_delta;                     // 16 bits and no more keys than a block holds: every block forms delta itself, nothing does beforehand
     int   vec;                           // rows of q, k, v and dout can be read 16 bytes at a time
     int   vec_out;                       // rows of out and dout can
     int   vec_grad;                      // rows of dq, dk and dv can be written so
@@ -62,7 +62,7 @@ struct AttentionGradParams {
 
 enum { ATT_F32 = KM_TYPE_FLOAT32, ATT_BF16 = KM_TYPE_BFLOAT16, ATT_F16 = KM_TYPE_FLOAT16 };
 
-// attention_rows.cu (mma.sync): any layout and type.  rows_tile() rows per block; `few` is the form whose warps share 16 rows.
+// attention_rows.cu (mma.sync): any layout and type.  ATT_TILE_ROWS rows a block; `few`: the form whose warps share ATT_FEW_ROWS.
 int  attention_rows_launch(const AttentionParams& p, int type, bool few, cudaStream_t st);
 constexpr int ATT_FEW_ROWS = 16, ATT_TILE_ROWS = 64;
 int  attention_join_launch(const AttentionParams& p, int type, cudaStream_t st);

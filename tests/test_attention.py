@@ -350,3 +350,47 @@ def test_pieces_are_planned_for_the_blocks_that_the_launch_has():
         setattr(args, name, _native.KmHeads(4096, rows * 8 * 128, 8 * 128, 128))
     args.lse_stride_l, args.lse_stride_head = 8, 1
     assert "own=few rows=8 tiles=1 splits=4 prefix=few rows=8 tiles=1 splits=18" in _native.describe_attention(args, 1)
+
+
+def _big(**kw):
+    """Dense tensors of the extents; nothing is launched."""
+    args = _c_args(**kw)
+    l, d, Hk = args.l, args.d, args.key_heads
+    for name, rows, heads, batch in (("q", args.n, args.heads, args.q_batch), ("k", args.m, Hk, args.kv_batch), ("v", args.m, Hk, args.kv_batch),
+                                     ("out", args.n, args.heads, l), ("grad_out", args.n, args.heads, l), ("grad_q", args.n, args.heads, args.q_batch),
+                                     ("grad_k", args.m, Hk, args.kv_batch), ("grad_v", args.m, Hk, args.kv_batch),
+                                     ("k_prefix", args.prefix, Hk, 1), ("v_prefix", args.prefix, Hk, 1)):
+        setattr(args, name, _native.KmHeads(4096, rows * heads * d if batch > 1 else 0, heads * d, d))
+    args.lse_stride_l, args.lse_stride_head = args.heads * args.n, args.n
+    return args
+
+
+SCRATCH = [         # sizes, kind; the second and the last two take more than 512 MB
+    (dict(l=1, n=1, m=100000, heads=8, key_heads=8, d=128), 0),
+    (dict(l=16, q_batch=16, kv_batch=16, n=1024, m=1100, prefix=4000, heads=32, key_heads=8, d=128), 1),
+    (dict(l=16, q_batch=16, kv_batch=16, n=1, m=1100, prefix=4000, heads=32, key_heads=8, d=128), 1),
+    (dict(l=2, n=3000, m=3500, heads=8, key_heads=8, d=8), 0),
+    (dict(l=2, n=3000, m=3500, heads=8, key_heads=8, d=40), 2),
+    (dict(l=4, q_batch=4, kv_batch=4, n=64, m=100000, heads=8, key_heads=8, d=128), 2),
+    (dict(l=4, q_batch=4, kv_batch=1, n=5000, m=600, heads=32, key_heads=4, d=128), 2),
+    (dict(l=64, q_batch=1, kv_batch=64, n=1024, m=200, heads=16, key_heads=16, d=128), 2),
+    (dict(l=64, q_batch=64, kv_batch=64, n=2048, m=300, prefix=300, heads=16, key_heads=16, d=64), 1),
+]
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("sizes, kind", SCRATCH, ids=str)
+def test_scratch_is_what_the_header_says(sizes, kind, dtype):
+    args = _big(type=dtype, **sizes)
+    l, n, m, H, Hk, d, MB = args.l, args.n, args.m, args.heads, args.key_heads, args.d, 1 << 20
+    if kind == 2:
+        most = 4 * l * n * H + (dtype == 2) * (4 * l * -(-n // 64) * H + 4 * args.kv_batch * -(-m // 64) * Hk) + 3 * 256 * MB
+        if args.q_batch == 1 and l > 1:
+            most += 4 * l * n * H * d
+    else:
+        parts = 8 * l * n * H * (d + 2) if args.prefix and m else 0
+        rows = l * n * H + 2 * Hk * (args.kv_batch * m + args.prefix)
+        most = max(512 * MB, parts) + (min(384 * rows, 1024 * MB) if dtype == 0 and d <= 64 else 0)
+        least = parts
+        assert _native.attention_scratch_bytes(args, kind) >= least
+    assert 0 <= _native.attention_scratch_bytes(args, kind) <= most + 64
