@@ -686,3 +686,140 @@ def test_float16_weights_below_the_smallest_float16(L, N, D):
     others = (M - 1) * math.exp(-4.0 * float(k[0, 7, 0, 0]))
     # half a step of the result, 2^-11 of it, and of each weight of 2^-25.1 before 2^-33
     assert (out.double() - others / (1.0 + others)).abs().max() <= others * (2.0 ** -11 + 2.0 ** -7) + 2.0 ** -25
+
+
+def weights_of(q, k, lengths=None, causal_from=None):
+    """softmax in the tensors' own arithmetic, (L, H, N, M); key m of the last M - causal_from belongs to query m - causal_from - (length - N)."""
+    L, N, H, D = q.shape
+    M, Hk = k.shape[1:3]
+    s = torch.matmul(q.transpose(1, 2), k.transpose(1, 2).repeat_interleave(H // Hk, dim=1).transpose(2, 3)) / math.sqrt(D)
+    at = torch.arange(M, device="cuda")
+    if causal_from is not None:
+        last = causal_from + (torch.tensor(lengths, device="cuda")[:, None] - N + torch.arange(N, device="cuda")).clamp_min(-1)      # (L, N)
+        s = s.masked_fill(at > last[:, None, :, None], -math.inf)
+    elif lengths is not None:
+        s = s.masked_fill((at >= torch.tensor(lengths, device="cuda")[:, None])[:, None, None, :], -math.inf)
+    top = s.amax(dim=-1, keepdim=True)
+    e = torch.exp(s - top.masked_fill(top == -math.inf, 0.0))
+    total = e.sum(dim=-1, keepdim=True)
+    return e / total.masked_fill(total == 0.0, 1.0)
+
+
+ROUNDED = [         # L, N, M, H, Hk, D, lengths, layout: the kernel for few rows, those on tcgen05, those on mma.sync
+    (8, 1, 2000, 16, 4, 128, [2000, 500, 1, 0, 1999, 64, 1024, 700], "nhd"),
+    (4, 2, 300, 32, 8, 80, None, "hnd"),
+    (2, 300, 700, 8, 2, 64, [700, 130], "nhd"),
+    (1, 200, 5000, 4, 4, 128, None, "nhd"),
+    (2, 100, 333, 6, 2, 40, [333, 200], "hnd"),
+    (2, 300, 700, 8, 2, 136, [700, 130], "nhd"),
+    (2, 150, 300, 4, 4, 64, None, "odd"),
+    (8, 1, 600, 8, 2, 200, None, "nhd"),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=str)
+@pytest.mark.parametrize("shape", ROUNDED, ids=str)
+def test_16_bit_results_are_as_near_as_their_roundings(dtype, shape):
+    # As in grad_rms: half a step of each weight and of the result, squares added; 0.425 of that is what roundings make, and a tenth more is left
+    # for chance.  The worst-case bounds above are some ten times that.
+    L, N, M, H, Hk, D, lengths, layout = shape
+    q, k, v = (make(s, L, n, h, D, dtype=dtype, by=by, layout=layout) for s, n, h, by in ((1, N, H, 1.5), (2, M, Hk, 1.0), (3, M, Hk, 1.0)))
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    got = kermac.cross_attention(q, k, v, lengths=lens)
+    kp, vp, own_k, own_v = k[0, :M // 2].contiguous(), v[0, :M // 2].contiguous(), k[:, M // 2:], v[:, M // 2:]
+    below = kermac.prefix_attention(q, kp, vp, own_k, own_v)
+    u = torch.finfo(dtype).eps / 2
+    q, k, v, kp, vp, own_k, own_v = (t.double() for t in (q, k, v, kp, vp, own_k, own_v))
+    whole_k, whole_v = (torch.cat([a.expand(L, *a.shape), b], dim=1) for a, b in ((kp, own_k), (vp, own_v)))
+    for what, p, values, result in (("cross", weights_of(q, k, lengths), v, got),
+                                    ("prefix", weights_of(q, whole_k, [M - M // 2] * L, causal_from=M // 2), whole_v, below)):
+        values = values.transpose(1, 2).repeat_interleave(H // Hk, dim=1)
+        want = torch.matmul(p, values)
+        off = u ** 2 * torch.matmul(p ** 2, values ** 2) + (u * want.abs()) ** 2
+        found = float((result.double().transpose(1, 2) - want).square().mean().sqrt() / off.mean().sqrt())
+        assert found <= 0.47, (what, found)
+
+
+GRADIENTS = [       # L, N, M, H, Hk, D, lengths, layout, broadcast
+    (2, 300, 700, 8, 2, 64, [700, 330], "nhd", ""),
+    (2, 100, 5000, 4, 2, 128, [5000, 400], "nhd", ""),                   # the keys divided, some pieces of the shorter entry empty
+    (3, 40, 4000, 4, 4, 64, [4000, 0, 140], "nhd", "q"),                 # and one q for all
+    (4, 700, 300, 4, 2, 128, [300, 150, 0, 299], "hnd", "kv"),           # queries divided
+    (4, 700, 300, 4, 2, 80, None, "nhd", "kv"),
+    (1, 2000, 200, 8, 1, 96, None, "nhd", ""),
+    (2, 300, 700, 8, 2, 136, [700, 330], "nhd", ""),                     # on mma.sync
+    (3, 40, 4000, 4, 4, 64, [4000, 0, 140], "odd", "q"),
+    (4, 700, 300, 4, 2, 200, [300, 150, 0, 299], "nhd", "kv"),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=str)
+@pytest.mark.parametrize("shape", GRADIENTS, ids=str)
+def test_16_bit_gradients_are_as_near_as_their_roundings(dtype, shape):
+    L, N, M, H, Hk, D, lengths, layout, broadcast = shape
+    q, k, v, g = (make(s, 1 if name in broadcast else L, n, h, D, dtype=dtype, by=by, layout=layout)
+                  for s, name, n, h, by in ((1, "q", N, H, 1.5), (2, "k", M, Hk, 1.0), (3, "v", M, Hk, 1.0), (9, "g", N, H, 0.5)))
+    if "k" not in broadcast:
+        spoil(k, lengths), spoil(v, lengths)
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out, lse = kermac.cross_attention(q, k, v, lengths=lens, return_lse=True)
+    found = grad_rms(dtype, q, k, v, g, kermac.cross_attention_grad(q, k, v, out, lse, g, lengths=lens), lengths)
+    # 0.425, and a tenth for chance
+    assert max(found) <= 0.47, found
+
+
+FLOAT32 = [         # L, N, M, H, Hk, D, lengths, layout, broadcast
+    (2, 200, 700, 4, 4, 64, [700, 350], "nhd", ""),                      # in three planes
+    (2, 200, 700, 8, 2, 64, None, "nhd", ""),
+    (3, 100, 500, 6, 2, 40, [500, 33, 129], "hnd", ""),
+    (3, 100, 500, 6, 2, 33, None, "odd", ""),
+    (3, 100, 500, 4, 4, 64, None, "nhd", "kv"),
+    (2, 1, 3000, 8, 2, 64, [3000, 1234], "nhd", ""),                     # on mma.sync
+    (2, 200, 700, 8, 2, 128, [700, 350], "nhd", ""),
+    (2, 100, 300, 4, 2, 201, None, "odd", ""),
+    (2, 100, 30, 4, 2, 64, [30, 11], "nhd", ""),
+]
+
+
+@pytest.mark.parametrize("shape", FLOAT32, ids=str)
+def test_float32_forms_are_no_less_accurate_than_fp32_products(shape):
+    # test_float32_is_no_less_accurate_than_fp32_products over the forms that it leaves out, and its tolerances.  To the result's is added what the tensor
+    # cores cut off, which is of one sign: a chain of two instructions loses up to 2^-23 of the sum at each, half of that in the mean, together
+    # 2^-23.  (It shows in single tokens: their fp32 products are summed by another algorithm in torch, with half of the error of larger ones.)
+    chopped = 2.0 ** -23
+    L, N, M, H, Hk, D, lengths, layout, broadcast = shape
+    q, k, v, g = (make(s, 1 if name in broadcast else L, n, h, D, dtype=torch.float32, by=by, layout=layout)
+                  for s, name, n, h, by in ((1, "q", N, H, 1.5), (2, "k", M, Hk, 1.0), (3, "v", M, Hk, 1.0), (9, "g", N, H, 0.5)))
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    assert not torch.backends.cuda.matmul.allow_tf32
+
+    def formulas(q, k, v, g):
+        kk, vv = (t.expand(L, *t.shape[1:]) for t in (k, v))
+        p = weights_of(q, kk, lengths)
+        kh, vh = (t.transpose(1, 2).repeat_interleave(H // Hk, dim=1) for t in (kk, vv))
+        qh, gh = q.transpose(1, 2), g.transpose(1, 2)
+        out = torch.matmul(p, vh)
+        ds = p * (torch.matmul(gh, vh.transpose(2, 3)) - (gh * out).sum(dim=-1, keepdim=True)) / math.sqrt(D)
+        grads = [torch.matmul(ds, kh)] + [t.unflatten(1, (Hk, H // Hk)).sum(dim=2) for t in (torch.matmul(ds.transpose(2, 3), qh), torch.matmul(p.transpose(2, 3), gh))]
+        grads = [grads[0]] + [t.sum(dim=0, keepdim=True) if broadcast else t for t in grads[1:]]
+        return [t.transpose(1, 2) for t in (out, *grads)]
+
+    exact, plain = formulas(*(t.double() for t in (q, k, v, g))), formulas(q, k, v, g)
+    out, lse = kermac.cross_attention(q, k, v, lengths=lens, return_lse=True)
+    of_lse = 2 * 2.0 ** -24 * float(lse[lse != -math.inf].abs().max()) + 2.0 ** -22
+    for i, (got, fp32, want) in enumerate(zip((out, *kermac.cross_attention_grad(q, k, v, out, lse, g, lengths=lens)), plain, exact)):
+        ours, theirs = ((t.double() - want).square().mean().sqrt() for t in (got, fp32))
+        assert ours <= 1.25 * theirs + (chopped if i == 0 else of_lse) * want.square().mean().sqrt(), (i, float(ours / theirs))
+    # a prefix and own tokens: both in planes, one of them, neither
+    P = M // 3
+    kp, vp = k[0, :P].contiguous(), v[0, :P].contiguous()
+    own_k, own_v = (t.expand(L, *t.shape[1:])[:, P:].contiguous() for t in (k, v))
+
+    def prefixed(q, kp, vp, own_k, own_v):
+        kk, vv = (torch.cat([a.expand(L, *a.shape), b], dim=1) for a, b in ((kp, own_k), (vp, own_v)))
+        p = weights_of(q, kk, [M - P] * L, causal_from=P)
+        return torch.matmul(p, vv.transpose(1, 2).repeat_interleave(H // Hk, dim=1)).transpose(1, 2)
+
+    want, fp32 = (prefixed(*(t.to(x) for t in (q, kp, vp, own_k, own_v))) for x in (torch.float64, torch.float32))
+    ours, theirs = ((t.double() - want).square().mean().sqrt() for t in (kermac.prefix_attention(q, kp, vp, own_k, own_v), fp32))
+    assert ours <= 1.25 * theirs + chopped * want.square().mean().sqrt(), float(ours / theirs)
