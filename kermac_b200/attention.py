@@ -223,7 +223,7 @@ def prefix_attention(
 
     q: (L, N, H, D); k_prefix, v_prefix: (P, Hk, D), the prefix, read and multiplied once for the whole batch; k, v: (L, M, Hk, D),
     each sequence's own tokens, of which `lengths` (or all M) are there, the N newest included.  Query n sees the whole prefix
-    and own token j when j <= lengths[l] - N + n.  P and M may be 0.  Everything else as in `cross_attention`, but for the partial sums: where
+    and own token j when j <= lengths[l] - N + n; a v that is not finite reaches, as 0 * inf, the queries before it too.  P and M may be 0.  Everything else as in `cross_attention`, but for the partial sums: where
     there are both a prefix and own tokens each of the two takes 4 (D + 2) bytes a query and head at least, without a limit.
     """
     return _forward(_native.ATTENTION_PREFIX, q, k, v, lengths, scale, out, lse, return_lse, debug, prefix=(k_prefix, v_prefix))
