@@ -141,9 +141,11 @@ __global__ void __launch_bounds__(THREADS) attention_few_kernel(const __grid_con
     const int all_see = min(w.causal ? w.length - p.N + 1 : w.length, w.end), held = prefix ? p.P : p.M;
 
     float o[DP / 16][NR][4], top[NR][2], sum[NR][2];
+    Exponent<T> exponent[NR][2];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
         top[r][0] = top[r][1] = -INFINITY, sum[r][0] = sum[r][1] = 0.0f;
+        exponent[r][0] = exponent[r][1] = {p.scale_log2, weight_log2<T>};
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d) o[d][r][0] = o[d][r][1] = o[d][r][2] = o[d][r][3] = 0.0f;
     }
@@ -206,6 +208,7 @@ __global__ void __launch_bounds__(THREADS) attention_few_kernel(const __grid_con
                 for (int e = 0; e < 2; ++e) {
                     // (-inf) - (-inf) of a row that has seen nothing yet must not become NaN
                     shrink[e] = top[r][e] == -INFINITY ? 0.0f : ex2_approx((top[r][e] - base_m[r][e]) * p.scale_log2);
+                    exponent[r][e].raise(base_m[r][e], p.scale_log2);
                     top[r][e] = base_m[r][e];
                     sum[r][e] *= shrink[e];
                 }
@@ -217,14 +220,17 @@ __global__ void __launch_bounds__(THREADS) attention_few_kernel(const __grid_con
         uint32_t weights[BLOCKS][NR][2];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
+            // float16 takes the maximum off beforehand, which is as good (Exponent for both: 64 x 4096 keys, float16, 107.9 -> 110.1 us; this for both:
+            // 128 sequences below a prefix, bfloat16, 134.9 -> 136.3)
             float minus[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) minus[e] = top[r][e] == -INFINITY ? 0.0f : weight_log2<T> - top[r][e] * p.scale_log2;
+            for (int e = 0; e < 2; ++e) minus[e] = top[r][e] == -INFINITY ? 0.0f : -top[r][e] * (is_f16<T> ? 1.0f : exponent[r][e].by);
 #pragma unroll
             for (int m = 0; m < BLOCKS; ++m) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[m][r][e] = ex2_approx(fmaf(s[m][r][e], p.scale_log2, minus[e & 1]));
+                    s[m][r][e] = ex2_approx(is_f16<T> ? fmaf(s[m][r][e] + minus[e & 1], p.scale_log2, weight_log2<T>)
+                                                      : fmaf(s[m][r][e], exponent[r][e & 1].by, minus[e & 1]));
                     sum[r][e & 1] += s[m][r][e];
                 }
                 weights[m][r][0] = transposed(Type<T>::pair(s[m][r][0], s[m][r][1]));

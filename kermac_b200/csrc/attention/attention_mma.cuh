@@ -57,6 +57,20 @@ constexpr float F16_WEIGHT = 256.0f, F16_WEIGHT_LOG2 = 8.0f;
 template <typename T> constexpr float weight_log2 = is_f16<T> ? F16_WEIGHT_LOG2 : 0.0f;
 template <typename T> constexpr float per_weight  = is_f16<T> ? 1.0f / F16_WEIGHT : 1.0f;
 
+// One fma forms a weight's exponent, (s - top) c.  The rounding of top c is a factor on all of a row's weights, until it leaves the type's range: where
+// top c is 2^26 and more the next power of two takes the place of c, whose product with top is exact, and float16 weights stay as they are.  Scores
+// there lie 4 and more apart in c, so that only weights of 2^-4 and less change, by less than the last bit of their score does.
+template <typename T>
+struct Exponent {
+    float by, up;            // weight = 2^(s by + up - top by)
+    __device__ __forceinline__ void raise(float top, float c) {
+        const bool huge = fabsf(top * c) >= 0x1p26f;
+        by = huge ? __uint_as_float((__float_as_uint(c) + 0x7fffffu) & 0x7f800000u) : c, up = huge ? 0.0f : weight_log2<T>;
+    }
+    // what sums are multiplied by at the end
+    __device__ __forceinline__ float per() const { return up == 0.0f ? 1.0f : per_weight<T>; }
+};
+
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 __device__ __forceinline__ void mma_16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const __nv_bfloat16*) {

@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const Attention
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                s[j][e] = ex2_approx(s[j][e] - (base[e >> 1] - weight_log2<T>));
+                s[j][e] = ex2_approx(s[j][e] - base[e >> 1] + weight_log2<T>);
                 sum[e >> 1] += s[j][e];
             }
         product_nn<T, DP, NT, CT>(o, s, tile_k + S::KEYS * TL::LD);

@@ -113,6 +113,7 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
             // slack: how far a row's maximum may grow; -inf where nothing but scores of -inf has come, whose maximum of 0 any other replaces
             constexpr float SLACK = is_f16<T> ? 5.0f : 8.0f;
             float top = 0.0f, sum = 0.0f, slack = SLACK;
+            Exponent<T> exponent = {c, weight_log2<T>};
             for (int i = 0; i < n_tiles; ++i) {
                 const int first = w.first + i * TC_ROWS;
                 wait(s_full(t), i & 1);
@@ -135,13 +136,15 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
                         best[e] = fmaxf(fmaxf(best[e], __uint_as_float(x[j + e])), __uint_as_float(x[j + 4 + e]));
                 const float high = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
                 if (i == 0) {
-                    if (high == -INFINITY) slack = -INFINITY; else top = high;      // a row that sees nothing: exp2(-inf - 0) = 0
+                    if (high == -INFINITY) slack = -INFINITY; else top = high, exponent.raise(top, c);      // a row that sees nothing: exp2(-inf - 0) = 0
                 } else {
                     const bool grown = (high - top) * c > slack;
                     if (__any_sync(0xffffffffu, grown)) {
                         // the products into O that were issued before this S are complete
-                        const float shrink = grown && slack > 0.0f ? ex2_approx((top - high) * c) : 1.0f;
-                        if (grown) top = high, slack = SLACK;
+                        const float from = top, up = exponent.up;
+                        if (grown) top = high, exponent.raise(top, c);
+                        const float shrink = grown && slack > 0.0f ? ex2_approx((from - high) * c + (exponent.up - up)) : 1.0f;
+                        if (grown) slack = SLACK;
                         sum *= shrink;
 #pragma unroll
                         for (int j = 0; j < DP; j += 32) {
@@ -155,7 +158,8 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
                         }
                     }
                 }
-                const u64 c2 = pack2(c, c), m2 = pack2(weight_log2<T> - top * c, weight_log2<T> - top * c);
+                const float minus = exponent.up - top * exponent.by;
+                const u64 c2 = pack2(exponent.by, exponent.by), m2 = pack2(minus, minus);
                 u64 total[2] = {0, 0};
 #pragma unroll
                 for (int j = 0; j < 64; j += 32) {
@@ -194,8 +198,8 @@ attention_tensor_kernel(const __grid_constant__ AttentionParams p, const __grid_
             wait(o_full(t), 0);
             tc::fence_after_sync();
             const bool  good = *reinterpret_cast<volatile int*>(&s_expired) == 0 && at < w.rows;
-            sum *= per_weight<T>;
-            const float by  = sum == 0.0f ? 0.0f : per_weight<T> / sum;
+            sum *= exponent.per();
+            const float by  = sum == 0.0f ? 0.0f : exponent.per() / sum;
             if (good) put_stats(p, w, row, top * c, sum);
             if (p.parts > 1 || p.vec_out) {
                 // the warp's rows of Q have been used for the last time

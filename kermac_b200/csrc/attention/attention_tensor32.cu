@@ -202,7 +202,7 @@ attention_tensor32_kernel(const __grid_constant__ AttentionParams p, const __gri
                 sum *= shrink;
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] *= shrink;
-                const u64 c2 = pack2(c, c), m2 = pack2(-from * c, -from * c);
+                const u64 c2 = pack2(c, c), m2 = pack2(-from, -from);
                 u64 total[2] = {0, 0};
 #pragma unroll
                 for (int chunk = 0; chunk < 2; ++chunk) {
@@ -213,7 +213,7 @@ attention_tensor32_kernel(const __grid_constant__ AttentionParams p, const __gri
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             float lo, hi;
-                            unpack2(fma2(pack2(__uint_as_float(x[2 * (j + e)]), __uint_as_float(x[2 * (j + e) + 1])), c2, m2), lo, hi);
+                            unpack2(mul2(add2(pack2(__uint_as_float(x[2 * (j + e)]), __uint_as_float(x[2 * (j + e) + 1])), m2), c2), lo, hi);
                             lo = ex2_approx(lo), hi = ex2_approx(hi);
                             total[e & 1] = add2(total[e & 1], pack2(lo, hi));
 #pragma unroll

@@ -823,3 +823,16 @@ def test_float32_forms_are_no_less_accurate_than_fp32_products(shape):
     want, fp32 = (prefixed(*(t.to(x) for t in (q, kp, vp, own_k, own_v))) for x in (torch.float64, torch.float32))
     ours, theirs = ((t.double() - want).square().mean().sqrt() for t in (kermac.prefix_attention(q, kp, vp, own_k, own_v), fp32))
     assert ours <= 1.25 * theirs + chopped * want.square().mean().sqrt(), float(ours / theirs)
+
+
+@pytest.mark.parametrize("dtype, size", [(torch.float16, 4096.0), (torch.float16, 5000.0), (torch.float16, 30000.0), (torch.bfloat16, 1.2e6), (torch.bfloat16, 1.0e12),
+                                         (torch.float32, 1.2345e6), (torch.float32, 1.0e12)], ids=str)
+@pytest.mark.parametrize("N, D", [(1, 64), (150, 64), (1, 128), (150, 128), (1, 136), (150, 136)])
+def test_huge_scores_that_are_equal(dtype, size, N, D):
+    # the product of a score of 1e9 and more with a scale is rounded by more than float16's exponents hold, of 1e10 by more than float32's
+    M = 700
+    q, k = torch.full((1, N, 2, D), size, device="cuda").to(dtype), torch.full((1, M, 2, D), size, device="cuda").to(dtype)
+    v = make(3, 1, M, 2, D, dtype=dtype)
+    got = kermac.cross_attention(q, k, v)
+    want, _, bound, _ = ao.attention(q * 0.0, k * 0.0, v)
+    assert_within(got, want, bound, "equal weights")
