@@ -251,7 +251,8 @@ def cross_attention_grad(
     states behind `lengths` get zeros.  grad_q, grad_k, grad_v: destinations of those shapes, which share memory with nothing else that
     the call is given, allocated when None.
 
-    Sums are 32-bit and in a fixed order: equal calls give equal bits.  Takes scratch from torch's allocator for the duration
+    Sums are 32-bit and in a fixed order: equal calls give equal bits.  Weights are taken from `lse`, whose rounding to float32 is a
+    factor on all of a row's: 3 % where scores are of size 10^6.  Takes scratch from torch's allocator for the duration
     of the call: 4 bytes a query and head (float16: some more), another 4 D where q is broadcast over the batch, and partial sums where
     sums over states or queries are divided (at most 256 MB for each gradient).
     """

@@ -836,3 +836,31 @@ def test_huge_scores_that_are_equal(dtype, size, N, D):
     got = kermac.cross_attention(q, k, v)
     want, _, bound, _ = ao.attention(q * 0.0, k * 0.0, v)
     assert_within(got, want, bound, "equal weights")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("D", [64, 136])
+def test_captured_gradients_follow_the_lengths(dtype, D):
+    # which sequences have few keys is known on the device alone; other inputs, another size of the values and other lengths in the captured buffers
+    L, N, M, H, Hk = 3, 70, 700, 4, 2
+    q, k, v, g = (make(s, L, n, h, D, dtype=dtype) for s, n, h in ((1, N, H), (2, M, Hk), (3, M, Hk), (9, N, H)))
+    lengths = torch.tensor([700, 2, 64], dtype=torch.int32, device="cuda")
+
+    def step():
+        out, lse = kermac.cross_attention(q, k, v, lengths=lengths, return_lse=True)
+        return (out, lse, *kermac.cross_attention_grad(q, k, v, out, lse, g, lengths=lengths))
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for new, by in (([700, 2, 64], 1.0), ([5, 700, 130], 0.01), ([0, 65, 128], 100.0)):
+        lengths.copy_(torch.tensor(new, dtype=torch.int32))
+        v.copy_(make(13, L, M, Hk, D, dtype=dtype, by=by))
+        spoil(v, new)
+        for t in captured:
+            t.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(step(), captured))
+        assert all(torch.isfinite(t).all() for t in captured[2:])
