@@ -352,14 +352,6 @@ int attention_few_launch(const AttentionParams& p, int type, int rows, cudaStrea
     return type == ATT_BF16 ? launch_few_type<__nv_bfloat16>(p, maps, rows, keys, st) : launch_few_type<__half>(p, maps, rows, keys, st);
 }
 
-int attention_few_take_wait_flag() {
-    int flag = 0;
-    if (cudaMemcpyFromSymbol(&flag, att::g_attention_few_wait_expired, sizeof(flag)) != cudaSuccess) return -1;
-    if (flag) {
-        const int zero = 0;
-        if (cudaMemcpyToSymbol(att::g_attention_few_wait_expired, &zero, sizeof(zero)) != cudaSuccess) return -1;
-    }
-    return flag ? 1 : 0;
-}
+int attention_few_take_wait_flag() { return att::take_wait_flag(att::g_attention_few_wait_expired); }
 
 }  // namespace km

@@ -607,14 +607,6 @@ int attention_grad_tensor_launch(const AttentionGradParams& p, int type, cudaStr
     return p.D <= 64 ? launch_grad_tensor<__half, 64>(p, maps, st) : launch_grad_tensor<__half, 128>(p, maps, st);
 }
 
-int attention_grad_tensor_take_wait_flag() {
-    int flag = 0;
-    if (cudaMemcpyFromSymbol(&flag, att::g_attention_grad_wait_expired, sizeof(flag)) != cudaSuccess) return -1;
-    if (flag) {
-        const int zero = 0;
-        if (cudaMemcpyToSymbol(att::g_attention_grad_wait_expired, &zero, sizeof(zero)) != cudaSuccess) return -1;
-    }
-    return flag ? 1 : 0;
-}
+int attention_grad_tensor_take_wait_flag() { return att::take_wait_flag(att::g_attention_grad_wait_expired); }
 
 }  // namespace km

@@ -95,6 +95,15 @@ __device__ __forceinline__ void issue_commit(uint32_t bar) {
     __syncwarp();
 }
 
+// Host: 1 if a wait of the kernel has run out since the last call (the flag is then taken back), 0 if not, -1 if the device did not tell.
+inline int take_wait_flag(const int& flag_on_device) {
+    int flag = 0;
+    if (cudaMemcpyFromSymbol(&flag, flag_on_device, sizeof(flag)) != cudaSuccess) return -1;
+    const int zero = 0;
+    if (flag && cudaMemcpyToSymbol(flag_on_device, &zero, sizeof(zero)) != cudaSuccess) return -1;
+    return flag ? 1 : 0;
+}
+
 // One row (lane) of 32 columns.  The values may be used behind wait_loaded() of the same registers.
 __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t* r) {
     asm volatile(

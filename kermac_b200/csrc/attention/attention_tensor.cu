@@ -325,14 +325,6 @@ int attention_tensor_launch(const AttentionParams& p, int type, cudaStream_t st)
     return p.D <= 64 ? launch_tensor<__half, 64>(p, maps, queries, boxes, st) : launch_tensor<__half, 128>(p, maps, queries, boxes, st);
 }
 
-int attention_tensor_take_wait_flag() {
-    int flag = 0;
-    if (cudaMemcpyFromSymbol(&flag, att::g_attention_wait_expired, sizeof(flag)) != cudaSuccess) return -1;
-    if (flag) {
-        const int zero = 0;
-        if (cudaMemcpyToSymbol(att::g_attention_wait_expired, &zero, sizeof(zero)) != cudaSuccess) return -1;
-    }
-    return flag ? 1 : 0;
-}
+int attention_tensor_take_wait_flag() { return att::take_wait_flag(att::g_attention_wait_expired); }
 
 }  // namespace km

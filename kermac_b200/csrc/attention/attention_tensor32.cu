@@ -414,14 +414,6 @@ int attention_tensor32_launch(const AttentionParams& p, void* planes, cudaStream
     return rc;
 }
 
-int attention_tensor32_take_wait_flag() {
-    int flag = 0;
-    if (cudaMemcpyFromSymbol(&flag, att::g_attention_tensor32_wait_expired, sizeof(flag)) != cudaSuccess) return -1;
-    if (flag) {
-        const int zero = 0;
-        if (cudaMemcpyToSymbol(att::g_attention_tensor32_wait_expired, &zero, sizeof(zero)) != cudaSuccess) return -1;
-    }
-    return flag ? 1 : 0;
-}
+int attention_tensor32_take_wait_flag() { return att::take_wait_flag(att::g_attention_tensor32_wait_expired); }
 
 }  // namespace km
