@@ -6,7 +6,7 @@
 // token.  Q stays in registers; P^T passes from accumulator to operand layout by movmatrix.
 //
 // Measured at 64 sequences x 1 x 4096 keys (ragged), 32 heads of 128, 8 key heads, float16, 674 MB, back-to-back passes over three sets of
-// inputs: 111 to 113 us, 6.0 to 6.1 TB/s, 92 to 94 % of a plain copy.  While it was written, one pass at a time: copies by the lanes (cp.async, 480 of some 700
+// inputs: 110 to 114 us, 5.9 to 6.1 TB/s, 91 to 94 % of a plain copy.  While it was written, one pass at a time: copies by the lanes (cp.async, 480 of some 700
 // instructions a tile) with 16 rows an instruction 294 us, this 105; two warps a block and two blocks an SM 118.
 //
 // Two blocks an SM hide what a block does before its first and behind its last tile.  Up to 64 channels they fit; above, tiles of 16

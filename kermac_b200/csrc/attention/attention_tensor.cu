@@ -8,7 +8,7 @@
 // than 2^8, so that weights are at most 256 (the first tile sets it; after that it seldom happens).  float16 weights, which are 2^8 times as large, see
 // attention_mma.cuh, have 2^5, an eighth of that type's range.
 //
-// 4 x 4096 x 8192, 16 heads of 128, bf16: 1006 to 1019 us, 1.08 PFLOP/s, in passes that follow one another, 947 to 1024 in single ones, by the clock that
+// 4 x 4096 x 8192, 16 heads of 128, bf16: 1006 to 1025 us, 1.08 PFLOP/s, in passes that follow one another, 947 to 1024 in single ones, by the clock that
 // the power limit leaves.  In one run at 1.65 GHz, which the figures below are from, 887, and the products alone, without a softmax, 783.  A step (two tiles of rows, 128 keys) is 3440 cycles for products of 2048.  Tried: two threads a row (eight
 // warps a tile, 960 us), 2 to 5 of 8 pairs of exponentials on the FP32 pipe (952 to 1023), polling waits, K and V in one slot (no gain).
 #include <algorithm>
